@@ -1,0 +1,418 @@
+"""Timed cases of the operators around the MoE layer: root-mean-square norm with the residual's addition (bf16 or 8-bit output,
+backward), 8-bit floating point products with a scale per block of 128 (quantizer, product, linear layer with its gradients) and
+the MoE layer and router for a few tokens.
+
+Shapes are those of the repository's configurations - Qwen3-MoE-shaped (hidden 2048, 128 experts of 768, top-8), Mixtral-shaped
+(hidden 4096, 8 experts of 14336, top-2), DeepSeek-V3-shaped (hidden 7168, experts of 2048, top-8, 32 of 256 on one rank) - or
+generic odd ones.
+
+`run` computes either the plain form (elementary torch operations in 32 bits, rounded once) or, with `own`, calls the framework.
+Values held in 8 bits are returned as the bf16 values that codes and scales stand for, and the scales.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.0
+EPS = 1e-6
+
+
+def _mok():
+    package = os.path.join(os.getcwd(), "mixture-of-kittens_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import mok
+    return mok
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# cases
+# ---------------------------------------------------------------------------------------------------------------------
+QWEN3 = dict(hidden=2048, intermediate=768, experts=128, total=128, topk=8)
+MIXTRAL = dict(hidden=4096, intermediate=14336, experts=8, total=8, topk=2)
+DEEPSEEK = dict(hidden=7168, intermediate=2048, experts=32, total=256, topk=8)   # one rank's experts of 256
+
+
+def listed():
+    return [
+        # one decoded token: the residual stream's addition and the norm in front of a layer, bound by latency
+        dict(name="norm_t1", op="norm", tokens=1, hidden=2048, residual=True, form="bf16"),
+        # a small batch whose norm feeds an 8-bit product
+        dict(name="norm_fp8_t333", op="norm", tokens=333, hidden=7168, residual=True, form="fp8"),
+        # training: forward and backward over a full batch, gradient of the residual stream included
+        dict(name="norm_train_t16384", op="norm", tokens=16384, hidden=7168, residual=True, form="train"),
+        # a decode batch through gate and up projection side by side: bound by the weights' bytes
+        dict(name="matmul_m16", op="matmul", rows=16, cols=4096, depth=7168, b_rows=128),
+        # ragged: no size divides a tile, the last block of 128 is short in every direction
+        dict(name="matmul_odd_m1000", op="matmul", rows=1000, cols=1544, depth=1808, b_rows=128),
+        # prefill through a projection
+        dict(name="matmul_m8192", op="matmul", rows=8192, cols=7168, depth=2048, b_rows=128),
+        # weights quantized after an optimizer step, for the forward and (transposed) for the backward
+        dict(name="quantize_weight", op="quantize", rows=7168, cols=2048, tile_rows=128, transpose=True),
+        # a training step of a projection: quantization of x, w and dy, the product and both gradients
+        dict(name="linear_train_t4096", op="linear", rows=4096, cols=4096, depth=2048),
+        # one token through a whole layer: router and experts, the smallest serving step
+        dict(name="moe_route_t1", op="moe", tokens=1, fp8=False, shared=True, route=True, limit=0.0, **QWEN3),
+        # a decode batch, router and experts: nearly every expert is used by a few tokens
+        dict(name="moe_route_t32", op="moe", tokens=32, fp8=False, shared=True, route=True, limit=0.0, **QWEN3),
+        # few wide experts, an odd number of tokens, clamped, no shared expert
+        dict(name="moe_wide_t7", op="moe", tokens=7, fp8=False, shared=False, route=False, limit=7.0, **MIXTRAL),
+        # one rank of eight: 8-bit experts, most routes of a token lie on other ranks
+        dict(name="moe_fp8_t64", op="moe", tokens=64, fp8=True, shared=True, route=False, limit=0.0, **DEEPSEEK),
+    ]
+
+
+def _log(rng, low, high, step=1):
+    return max(low, min(high, round(math.exp(rng.uniform(math.log(low), math.log(high))) / step) * step))
+
+
+def draw(rng):
+    op = rng.choice(("norm", "norm", "matmul", "matmul", "quantize", "linear", "moe", "moe", "moe"))
+    while True:
+        if op == "norm":
+            c = dict(op=op, tokens=_log(rng, 1, 16384), hidden=_log(rng, 256, 7168, 8), residual=rng.random() < 0.7,
+                     form=rng.choice(("bf16", "fp8", "train")))
+        elif op == "matmul":
+            c = dict(op=op, rows=_log(rng, 1, 8192), cols=_log(rng, 128, 7168, rng.choice((1, 8, 128))),
+                     depth=_log(rng, 128, 7168, 16), b_rows=rng.choice((1, 128, 128)))
+            if c["rows"] * c["cols"] * c["depth"] > 8192 * 7168 * 2048:
+                continue
+        elif op == "quantize":
+            c = dict(op=op, rows=_log(rng, 1, 8192), cols=_log(rng, 128, 7168, 8), tile_rows=rng.choice((1, 128)),
+                     transpose=rng.random() < 0.5)
+            if c["rows"] * c["cols"] > 7168 * 2048:
+                continue
+        elif op == "linear":
+            c = dict(op=op, rows=_log(rng, 128, 8192), cols=_log(rng, 256, 7168, 16), depth=_log(rng, 256, 7168, 16))
+            if c["rows"] * c["cols"] * c["depth"] > 4096 * 4096 * 2048:
+                continue
+        else:
+            total = _log(rng, 4, 256)
+            c = dict(op=op, tokens=_log(rng, 1, 256), hidden=_log(rng, 256, 7168, 64), intermediate=_log(rng, 128, 4096, 64),
+                     total=total, topk=rng.randint(1, min(8, total)), fp8=rng.random() < 0.5, shared=rng.random() < 0.6,
+                     route=rng.random() < 0.4, limit=rng.choice((0.0, 0.0, 7.0)))
+            c["experts"] = total if c["route"] else max(1, total // rng.choice((1, 2, 8)))
+            # no more weights than the widest listed layer has, and no more work of the plain form, which takes every expert
+            if c["experts"] * c["hidden"] * c["intermediate"] > 8 * 4096 * 14336:
+                continue
+            if c["tokens"] * c["experts"] * c["hidden"] * c["intermediate"] > 64 * 32 * 7168 * 2048:
+                continue
+        return c
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda", torch.cuda.current_device())
+    gen = torch.Generator(device=dev).manual_seed(seed)
+
+    def normal(*shape, std=1.0, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device=dev).normal_(0.0, std, generator=gen)
+
+    def codes(*shape):
+        return normal(*shape, std=100.0, dtype=torch.float32).clamp_(-E4M3_MAX, E4M3_MAX).to(E4M3)
+
+    def scales(*shape, around):
+        return torch.empty(shape, device=dev).uniform_(0.5 * around, 1.5 * around, generator=gen)
+
+    s = dict(case=case)
+    if case["op"] == "norm":
+        T, H = case["tokens"], case["hidden"]
+        s["x"], s["weight"] = normal(T, H), (1.0 + normal(H, std=0.1, dtype=torch.float32)).bfloat16()
+        s["residual"] = normal(T, H, std=2.0) if case["residual"] else None
+        if case["form"] == "train":
+            s["d_y"] = normal(T, H)
+            s["d_hidden"] = normal(T, H) if case["residual"] else None
+            for k in ("x", "weight", "residual"):
+                if s[k] is not None:
+                    s[k].requires_grad_()
+    elif case["op"] == "matmul":
+        M, N, K = case["rows"], case["cols"], case["depth"]
+        kb = -(-K // 128)
+        s["a"], s["a_scales"] = codes(M, K), scales(kb, M, around=0.01).t()
+        s["b"] = codes(N, K)
+        s["b_scales"] = scales(-(-N // 128), kb, around=2e-4) if case["b_rows"] == 128 else scales(kb, N, around=2e-4).t()
+    elif case["op"] == "quantize":
+        s["x"] = normal(case["rows"], case["cols"], std=0.02)
+    elif case["op"] == "linear":
+        M, N, K = case["rows"], case["cols"], case["depth"]
+        s["x"], s["w"], s["d_y"] = normal(M, K).requires_grad_(), normal(N, K, std=K ** -0.5).requires_grad_(), normal(M, N)
+    else:
+        T, H, I, E, K = (case[k] for k in ("tokens", "hidden", "intermediate", "experts", "topk"))
+        s["x"], s["limit"] = normal(T, H), case["limit"] or None
+        shapes = ((E, I, H), (E, I, H), (E, H, I))
+        if case["fp8"]:
+            s["routed"] = [(codes(*z), scales(E, -(-z[1] // 128), -(-z[2] // 128), around=0.01 * z[2] ** -0.5)) for z in shapes]
+        else:
+            s["routed"] = [normal(*z, std=z[2] ** -0.5) for z in shapes]
+        s["shared"] = [normal(*z[1:], std=z[2] ** -0.5) for z in shapes] if case["shared"] else [None] * 3
+        if case["route"]:
+            s["router"] = normal(case["total"], H, std=H ** -0.5, dtype=torch.float32)
+        else:
+            skew = normal(case["total"], std=0.5, dtype=torch.float32)
+            weights, routes = torch.topk(normal(T, case["total"], dtype=torch.float32) + skew, K, dim=1)
+            s["top_experts"], s["router_weights"] = routes.to(torch.int32), torch.softmax(weights, dim=1)
+            s["first"] = (case["total"] - E) // 2   # this rank's experts: [first, first + E)
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# plain forms
+# ---------------------------------------------------------------------------------------------------------------------
+def _blocks(x, rows, cols):
+    """[M, N] -> [M / rows, rows, N / cols, cols], padded with zeros."""
+    M, N = x.shape
+    x = torch.nn.functional.pad(x, (0, -N % cols, 0, -M % rows))
+    return x.view(x.shape[0] // rows, rows, x.shape[1] // cols, cols)
+
+
+def _plain_quantize(x, rows):
+    """(values that the codes stand for in fp32, scales): the smallest power of two per `rows` x 128 that brings them to 448."""
+    b = _blocks(x.float(), rows, 128)
+    big = b.abs().amax(dim=(1, 3), keepdim=True)
+    fraction, exponent = torch.frexp(big)   # 448 = 0.875 * 2 ** 9
+    exponent = torch.where(fraction > 0.875, exponent - 8, exponent - 9).clamp_min(-126)
+    scale = torch.ldexp(torch.ones_like(big), torch.where(big > 0, exponent, -126))
+    q = (b / scale).to(E4M3).float() * scale
+    return q.reshape(b.shape[0] * rows, -1)[: x.shape[0], : x.shape[1]], scale[:, 0, :, 0]
+
+
+def _plain_norm(s):
+    x, w, r = s["x"].detach().float(), s["weight"].detach().float(), s["residual"]
+    z = x if r is None else x + r.detach().float()
+    rho = torch.rsqrt(z.square().mean(1, keepdim=True) + EPS)
+    return z, rho, z * rho * w, w
+
+
+def _spread(scales, like, rows):
+    """One scale per element of `like` [..., N, K] from one per rows x 128."""
+    if rows > 1:
+        scales = scales.repeat_interleave(rows, dim=-2)[..., : like.shape[-2], :]
+    return scales.repeat_interleave(128, dim=-1)[..., : like.shape[-1]]
+
+
+def _plain_moe(s):
+    c, x = s["case"], s["x"].float()
+    T, E = x.shape[0], c["experts"]
+    out = {}
+    if c["route"]:
+        logits = s["x"].double() @ s["router"].double().t()
+        v, routes = torch.topk(logits, c["topk"], dim=1)
+        weights, first = torch.softmax(v, dim=1).float(), 0
+        out = dict(routes=routes.to(torch.int32), weights=weights)
+    else:
+        routes, weights, first = s["top_experts"].long(), s["router_weights"], s["first"]
+    local = (routes >= first) & (routes < first + E)
+    share = torch.zeros(T, E + 1, device=x.device)   # column E takes what lies on other ranks
+    share.scatter_add_(1, torch.where(local, routes - first, E), weights)
+
+    def dense(w):
+        return w[0].float() * _spread(w[1], w[0], 128) if isinstance(w, tuple) else w.float()
+
+    def hidden(g, u):
+        if s["limit"] is not None:
+            g, u = g.clamp(max=s["limit"]), u.clamp(-s["limit"], s["limit"])
+        return g / (1.0 + torch.exp(-g)) * u
+
+    xe = x.expand(E, T, x.shape[1])
+    h = hidden(torch.bmm(xe, dense(s["routed"][0]).transpose(1, 2)), torch.bmm(xe, dense(s["routed"][1]).transpose(1, 2)))
+    y = torch.bmm(h, dense(s["routed"][2]).transpose(1, 2))
+    total = (y * share[:, :E].t()[:, :, None]).sum(0)
+    if s["shared"][0] is not None:
+        wg, wu, wd = (w.float() for w in s["shared"])
+        total = total + hidden(x @ wg.t(), x @ wu.t()) @ wd.t()
+    return dict(out, out=total.bfloat16())
+
+
+def _plain(s):
+    c = s["case"]
+    if c["op"] == "norm":
+        z, rho, y, w = _plain_norm(s)
+        out = {"hidden": z.bfloat16()} if c["residual"] else {}
+        if c["form"] == "fp8":
+            q, scales = _plain_quantize(y, 1)
+            return dict(out, y=q.bfloat16(), scales=scales)
+        out["y"] = y.bfloat16()
+        if c["form"] == "train":
+            d_y = s["d_y"].float()
+            g = d_y * w
+            d_x = rho * (g - z * rho.square() * (g * z).mean(1, keepdim=True))
+            if c["residual"]:
+                d_x = d_x + s["d_hidden"].float()
+            out["d_x"], out["d_weight"] = d_x.bfloat16(), (d_y * z * rho).sum(0).bfloat16()
+        return out
+    if c["op"] == "matmul":
+        a = s["a"].float() * _spread(s["a_scales"], s["a"], 1)
+        return (a @ (s["b"].float() * _spread(s["b_scales"], s["b"], c["b_rows"])).t()).bfloat16()
+    if c["op"] == "quantize":
+        q, scales = _plain_quantize(s["x"], c["tile_rows"])
+        out = dict(values=q.bfloat16(), scales=scales)
+        if c["transpose"]:
+            q, scales = _plain_quantize(s["x"].t(), c["tile_rows"])
+            out.update(values_t=q.bfloat16(), scales_t=scales)
+        return out
+    if c["op"] == "linear":
+        x, w, d_y = (s[k].detach() for k in ("x", "w", "d_y"))
+        qw = _plain_quantize(w, 128)[0]
+        y = _plain_quantize(x, 1)[0] @ qw.t()
+        d_x = _plain_quantize(d_y, 1)[0] @ qw
+        d_w = _plain_quantize(d_y.t(), 1)[0] @ _plain_quantize(x.t(), 1)[0].t()
+        return dict(y=y.bfloat16(), d_x=d_x.bfloat16(), d_w=d_w.bfloat16())
+    return _plain_moe(s)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the framework's calls
+# ---------------------------------------------------------------------------------------------------------------------
+def _values(codes, scales, rows):
+    return (codes.float() * _spread(scales, codes, rows)).bfloat16()
+
+
+def _framework(s):
+    c, mok = s["case"], _mok()
+    if c["op"] == "norm":
+        if c["form"] == "fp8":
+            (codes, scales), hidden = mok.rms_norm_quantized(s["x"], s["weight"], s["residual"], eps=EPS)
+            out = dict(y=_values(codes, scales, 1), scales=scales)
+            return dict(out, hidden=hidden) if c["residual"] else out
+        y = mok.rms_norm(s["x"], s["weight"], s["residual"], eps=EPS)
+        y, hidden = y if c["residual"] else (y, None)
+        out = {"hidden": hidden.detach()} if c["residual"] else {}
+        out["y"] = y.detach()
+        if c["form"] == "train":
+            ends, grads = ((y, hidden), (s["d_y"], s["d_hidden"])) if c["residual"] else ((y,), (s["d_y"],))
+            out["d_x"], out["d_weight"] = torch.autograd.grad(ends, (s["x"], s["weight"]), grads)
+        return out
+    if c["op"] == "matmul":
+        return mok.block_matmul((s["a"], s["a_scales"]), (s["b"], s["b_scales"]))
+    if c["op"] == "quantize":
+        if not c["transpose"]:
+            codes, scales = mok.quantize_blocks(s["x"], tile_rows=c["tile_rows"])
+            return dict(values=_values(codes, scales, c["tile_rows"]), scales=scales)
+        (codes, scales), (codes_t, scales_t) = mok.quantize_blocks(s["x"], tile_rows=c["tile_rows"], transpose=True)
+        return dict(values=_values(codes, scales, c["tile_rows"]), scales=scales,
+                    values_t=_values(codes_t, scales_t, c["tile_rows"]), scales_t=scales_t)
+    if c["op"] == "linear":
+        y = mok.fp8_linear(s["x"], s["w"])
+        d_x, d_w = torch.autograd.grad(y, (s["x"], s["w"]), s["d_y"])
+        return dict(y=y.detach(), d_x=d_x, d_w=d_w)
+    out = {}
+    if c["route"]:
+        routes, weights = mok.route_decode(s["x"], s["router"], topk=c["topk"])
+        out, first = dict(routes=routes, weights=weights), 0
+    else:
+        routes, weights, first = s["top_experts"], s["router_weights"], s["first"]
+    out["out"] = mok.moe_decode(s["x"], routes, weights, *s["shared"], *s["routed"], first_expert=first, swiglu_limit=s["limit"])
+    return out
+
+
+def run(state):
+    return _framework(state) if own else _plain(state)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# what a pass cannot do without, and its result in 64 bits
+# ---------------------------------------------------------------------------------------------------------------------
+def work(case):
+    c = case
+    if c["op"] == "norm":
+        n = c["tokens"] * c["hidden"]
+        r = 2 if c["residual"] else 0
+        forward = n * (2 + 2 * r) + n * (1 + 4 / 128 if c["form"] == "fp8" else 2)
+        backward = n * (2 + 2 + r + 2) if c["form"] == "train" else 0   # dy, z, d_hidden in; dx out
+        return {"bytes": forward + backward, "flops": n * (6 if c["form"] != "train" else 18)}
+    if c["op"] == "matmul":
+        M, N, K = c["rows"], c["cols"], c["depth"]
+        return {"bytes": M * K + N * K + 2 * M * N + 4 * (M + -(-N // c["b_rows"])) * -(-K // 128), "flops": 2 * M * N * K}
+    if c["op"] == "quantize":
+        n = c["rows"] * c["cols"]
+        return {"bytes": n * (2 + (2 if c["transpose"] else 1)), "flops": 4 * n}
+    if c["op"] == "linear":
+        M, N, K = c["rows"], c["cols"], c["depth"]
+        return {"bytes": 2 * (M * K + N * K + 2 * M * N) + 2 * (M * K + N * K), "flops": 6 * M * N * K}
+    T, H, I, E, K = (c[k] for k in ("tokens", "hidden", "intermediate", "experts", "topk"))
+    used = E * (1.0 - (1.0 - K / c["total"]) ** T)   # distinct experts of this rank, balanced routes
+    routes = T * K * E / c["total"]
+    per = 3 * H * I
+    size = used * per * (1 + 4 / 128 ** 2 if c["fp8"] else 2) + (2 * per if c["shared"] else 0) + 4 * T * H
+    if c["route"]:
+        size += 4 * c["total"] * H
+    return {"bytes": size, "flops": 2 * per * (routes + (T if c["shared"] else 0)) + (2 * T * H * c["total"] if c["route"] else 0)}
+
+
+def _exact_codes(x, rows, cols):
+    """Values that a matrix stands for after quantization, every step but the rounding to e4m3 in 64 bits."""
+    x = x.double()
+    M, N = x.shape
+    big = torch.nn.functional.max_pool2d(torch.nn.functional.pad(x.abs(), (0, -N % cols, 0, -M % rows))[None], (rows, cols))[0]
+    scale = torch.exp2(torch.ceil(torch.log2(big / E4M3_MAX)).clamp_min(-126.0))
+    at = torch.arange(M, device=x.device)[:, None] // rows, torch.arange(N, device=x.device)[None, :] // cols
+    every = scale[at]
+    return (x / every).to(E4M3).double() * every, scale
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    c = case
+    if c["op"] == "norm":
+        x, w = s["x"].detach().double().requires_grad_(), s["weight"].detach().double().requires_grad_()
+        z = x + (s["residual"].detach().double() if c["residual"] else 0.0)
+        y = w * z / torch.linalg.vector_norm(torch.cat((z * c["hidden"] ** -0.5, torch.full_like(z[:, :1], EPS ** 0.5)), 1), dim=1,
+                                             keepdim=True)
+        out = {"hidden": z.detach()} if c["residual"] else {}
+        if c["form"] == "fp8":
+            q, scale = _exact_codes(y.detach(), 1, 128)
+            return dict(out, y=q, scales=scale)
+        out["y"] = y.detach()
+        if c["form"] == "train":
+            ends, grads = [y], [s["d_y"].double()]
+            if c["residual"]:
+                ends, grads = ends + [z], grads + [s["d_hidden"].double()]
+            out["d_x"], out["d_weight"] = torch.autograd.grad(ends, (x, w), grads)
+        return out
+    if c["op"] == "matmul":
+        M, N, K = c["rows"], c["cols"], c["depth"]
+        total = torch.zeros(M, N, dtype=torch.float64, device=s["a"].device)
+        column = torch.arange(N, device=total.device) // c["b_rows"]
+        for i, k in enumerate(range(0, K, 128)):
+            part = s["a"][:, k:k + 128].double() @ s["b"][:, k:k + 128].double().t()
+            total += part * s["a_scales"][:, i].double()[:, None] * s["b_scales"][column, i].double()[None, :]
+        return total
+    if c["op"] == "quantize":
+        out = dict(zip(("values", "scales"), _exact_codes(s["x"], c["tile_rows"], 128)))
+        if c["transpose"]:
+            out.update(zip(("values_t", "scales_t"), _exact_codes(s["x"].t(), c["tile_rows"], 128)))
+        return out
+    if c["op"] == "linear":
+        x, w, d_y = (s[k].detach() for k in ("x", "w", "d_y"))
+        qx, qw, qd = _exact_codes(x, 1, 128)[0], _exact_codes(w, 128, 128)[0], _exact_codes(d_y, 1, 128)[0]
+        d_w = torch.einsum("nt,kt->nk", _exact_codes(d_y.t(), 1, 128)[0], _exact_codes(x.t(), 1, 128)[0])
+        return dict(y=torch.einsum("tk,nk->tn", qx, qw), d_x=torch.einsum("tn,nk->tk", qd, qw), d_w=d_w)
+    x, out = s["x"].double(), {}
+    if c["route"]:
+        logits = torch.einsum("th,eh->te", x, s["router"].double())
+        order = torch.argsort(logits, dim=1, descending=True, stable=True)[:, : c["topk"]]
+        best = torch.exp(torch.gather(logits, 1, order) - logits.amax(1, keepdim=True))
+        routes, weights, first = order, best / best.sum(1, keepdim=True), 0
+        out = dict(routes=routes.to(torch.int32), weights=weights)
+    else:
+        routes, weights, first = s["top_experts"].long(), s["router_weights"].double(), s["first"]
+
+    def expert(rows, w, e):
+        g, u, d = ((v[0][e].double() * v[1][e].double()[torch.arange(v[0].shape[1], device=rows.device)[:, None] // 128,
+                                                        torch.arange(v[0].shape[2], device=rows.device)[None, :] // 128]
+                    if isinstance(v, tuple) else v[e].double()) for v in w)
+        gate, up = torch.einsum("th,ih->ti", rows, g), torch.einsum("th,ih->ti", rows, u)
+        if s["limit"] is not None:
+            gate, up = torch.clamp_max(gate, s["limit"]), torch.clamp(up, -s["limit"], s["limit"])
+        return torch.einsum("ti,hi->th", gate * torch.sigmoid(gate) * up, d)
+
+    total = expert(x, [w[None] for w in s["shared"]], 0) if c["shared"] else torch.zeros_like(x)
+    for e in range(c["experts"]):
+        token, slot = torch.nonzero(routes == first + e, as_tuple=True)
+        if token.numel():
+            total.index_add_(0, token, expert(x[token], s["routed"], e) * weights[token, slot].double()[:, None])
+    return dict(out, out=total)
