@@ -348,7 +348,9 @@ def _exact_codes(x, rows, cols):
     x = x.double()
     M, N = x.shape
     big = torch.nn.functional.max_pool2d(torch.nn.functional.pad(x.abs(), (0, -N % cols, 0, -M % rows))[None], (rows, cols))[0]
-    scale = torch.exp2(torch.ceil(torch.log2(big / E4M3_MAX)).clamp_min(-126.0))
+    fraction, exponent = torch.frexp(big / E4M3_MAX)
+    exponent = torch.where(fraction > 0.5, exponent, exponent - 1).clamp_min(-126)
+    scale = torch.ldexp(torch.ones_like(big), torch.where(big > 0, exponent, -126))
     at = torch.arange(M, device=x.device)[:, None] // rows, torch.arange(N, device=x.device)[None, :] // cols
     every = scale[at]
     return (x / every).to(E4M3).double() * every, scale
