@@ -383,6 +383,53 @@ int mok_router_backward(const void* x, const void* w_hi, const int32_t* top_expe
                         const float* d_router_weights, int64_t num_tokens, int hidden, int num_experts, int padded_experts,
                         int topk, void* d_logits, void* d_x, float* d_w, float* d_bias, uint32_t* status, mok_stream_t stream);
 
+/*
+ * Operators around the layer.  None of them has a counterpart among the reference's operators, which begin with the activations
+ * and end with the layer's output.  Strides count elements; a pointer is 16-byte aligned unless stated.
+ *
+ * Root-mean-square norm with the residual's addition: z = x + residual (fp32; residual may be NULL), inv_rms = (mean z^2 + eps)^-1/2,
+ * y = z * inv_rms * weight.  Outputs, each optional but one of y and codes: hidden_out = bf16(z) [rows, hidden] (only with a
+ * residual), y bf16 [rows, hidden], codes + scales = y in e4m3 with a scale per 128 columns (codes 8-byte aligned with a row stride
+ * that is a multiple of 8), inv_rms fp32 [rows].  weight is fp32 or bf16 [hidden].  hidden % 8 == 0, at most 16384; x and residual
+ * may have any row stride that is a multiple of 8.  Inputs in the subnormal range of fp32 count as zero.
+ */
+int mok_rms_norm_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                         int weight_is_f32, int64_t rows, int hidden, float eps, void* hidden_out, void* y, void* codes,
+                         int64_t codes_stride, float* scales, int64_t scale_row_stride, int64_t scale_block_stride, float* inv_rms,
+                         mok_stream_t stream);
+/*
+ * Its backward: z = the forward's hidden_out (or its x, without a residual); d_x [rows, hidden] is the gradient of x and of the
+ * residual, d_hidden (may be NULL) what arrives through the residual stream; d_weight [hidden] has the weight's type and is summed
+ * in a fixed order.  scratch: mok_rms_norm_scratch_bytes().
+ */
+int64_t mok_rms_norm_scratch_bytes(int64_t rows, int hidden);
+int mok_rms_norm_backward(const void* d_y, const void* d_hidden, const void* z, int64_t z_stride, const void* weight,
+                          int weight_is_f32, const float* inv_rms, int64_t rows, int hidden, void* d_x, void* d_weight,
+                          float* scratch, mok_stream_t stream);
+
+/*
+ * bf16 [rows, cols] -> e4m3 codes and fp32 scales of blocks of 1 x 128 (tile_rows 1) or 128 x 128 (tile_rows 128), of the matrix
+ * (codes, scales) and / or of its transpose (codes_t, scales_t; its blocks of 1 x 128 run along the rows of x).  value = scale *
+ * code; the scale is the smallest power of two, at least 2^-126, that brings the block to 448 or less; a block with an infinity
+ * or a NaN is NaN as a whole.  cols and the row strides of codes are multiples of 8; rows is any number: the transpose's rows
+ * are written in units of 8, with zeros behind the last.
+ */
+int mok_block_quantize(const void* x, int64_t x_stride, int64_t rows, int cols, int tile_rows, void* codes, int64_t codes_stride,
+                       float* scales, int64_t scale_row_stride, int64_t scale_block_stride, void* codes_t, int64_t codes_t_stride,
+                       float* scales_t, int64_t scale_t_row_stride, int64_t scale_t_block_stride, mok_stream_t stream);
+
+/*
+ * D [rows, cols] (bf16) = A [rows, depth] * B [cols, depth]^T, both e4m3 with fp32 scales per 128 of depth: a_scales per row of A,
+ * b_scales per row of B (b_tile_rows 1) or per 128 rows (b_tile_rows 128); any scale values.  Row strides of A and B are
+ * multiples of 16; the sizes are arbitrary.  out needs the alignment of its type only.  scratch: mok_block_matmul_scratch_bytes()
+ * (0: may be NULL).
+ */
+int64_t mok_block_matmul_scratch_bytes(int64_t rows, int cols, int depth);
+int mok_block_matmul(const void* a, int64_t a_stride, const float* a_scales, int64_t a_scale_row_stride,
+                     int64_t a_scale_block_stride, const void* b, int64_t b_stride, const float* b_scales,
+                     int64_t b_scale_row_stride, int64_t b_scale_block_stride, int b_tile_rows, int64_t rows, int cols, int depth,
+                     void* out, int64_t out_stride, void* scratch, uint32_t* status, mok_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,456 @@
+// Product of two matrices held in e4m3 with fp32 scales per block of 128:
+//   D[m, n] = sum over blocks kb of sa[m, kb] * sb[n or n / 128, kb] * (sum over k in kb of a[m, k] * b[n, k]),  D in bf16.
+//
+// The scales are fp32 numbers of any value, so the tensor cores cannot apply them: every block of 128 along K is accumulated on
+// its own in tensor memory (four tcgen05.mma of K = 32, kind::f8f6f4) and added, scaled, to fp32 registers.  CTA pairs own 256 x
+// 256 tiles, each CTA stages 128 rows of A and 128 of B per block by TMA (32 KB, 5 stages); two 256-column accumulators let the
+// MMAs of one block run while eight epilogue warps scale the block before (a warp: 32 rows x 128 columns, 128 registers of
+// sums).  Rows, columns and depth that are not multiples of the tile are zeros from TMA and are not stored.
+//
+// Few tiles (a short grid and a long K): the blocks along K are cut into `splits` shares, every share writes its fp32 sums, and
+// a second kernel adds them in order.
+#include "block_scale.cuh"
+#include "gemm_tiles.cuh"
+
+namespace mok {
+namespace {
+
+using namespace tiles;
+
+constexpr int BK = 128;
+constexpr int kStages = 5;
+constexpr int kThreads = 384;                 // one warpgroup with the TMA producer and the MMA issuer, two of the epilogue
+// Registers of the warpgroups: 384 threads start with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kIssueRegisters = 40;
+constexpr int kEpilogueRegisters = 232;
+constexpr int kOperandBytes = 128 * BK;       // 16 KB
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kGroup = 8;                     // m tiles that walk the columns together
+
+struct Layout {
+    static constexpr int kFull = kStages * kStageBytes;
+    static constexpr int kEmpty = kFull + 8 * kStages;
+    static constexpr int kAccFull = kEmpty + 8 * kStages;
+    static constexpr int kAccEmpty = kAccFull + 16;
+    static constexpr int kTmemPtr = kAccEmpty + 16;
+    static constexpr int kAbort = kTmemPtr + 4;
+    static constexpr int kScales = (kAbort + 4 + 127) / 128 * 128;   // [8 warps][2][128] fp32: column scales of a block
+    static constexpr int kPatch = kScales + 8 * 2 * 128 * 4;
+    static constexpr int kBytes = kPatch + 8 * kEpiWarpBytes;
+};
+static_assert(Layout::kBytes + 1024 <= kMaxDynamicSmem, "shared memory");
+
+struct Product {
+    const float *sa, *sb;
+    long long sa_row, sa_block, sb_row, sb_block;
+    bf16* out;
+    float* partial;          // [splits, rows, cols] when splits > 1
+    long long out_stride;
+    int rows, cols, k_blocks;
+    int m_tiles, n_tiles, splits;
+    uint32_t* status;
+};
+
+// Instruction descriptor for kind::f8f6f4, e4m3 x e4m3 -> fp32, both operands K-major: D format (1 = fp32) at 4, A / B formats
+// (0 = e4m3) at 7 / 10, N >> 3 at 17, M >> 4 at 24.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
+    return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 16 consecutive fp32 columns as eight pairs.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Two fp32 operations per instruction (sm_100).
+__device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) {
+    unsigned long long d;
+    // volatile: stays behind the wait for the tensor-memory load that fills its operands
+    asm volatile("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ unsigned long long pair_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long pair_mul(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void pair_split(unsigned long long d, uint32_t& lo, uint32_t& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(d));
+}
+
+struct Work {
+    int m0, n0, split, kb0, kb1;
+};
+// Tile t: groups of kGroup m tiles walk the columns together (their A panels stay in L2), the shares of K innermost.
+__device__ __forceinline__ Work decode(const Product& p, int t) {
+    Work w;
+    w.split = t % p.splits;
+    t /= p.splits;
+    const int per_group = kGroup * p.n_tiles;
+    const int g = t / per_group, rem = t - g * per_group;
+    const int width = min(kGroup, p.m_tiles - g * kGroup);
+    const int n = rem / width;
+    w.m0 = (g * kGroup + rem - n * width) * BM;
+    w.n0 = n * BN;
+    w.kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * w.split / p.splits);
+    w.kb1 = static_cast<int>(static_cast<long long>(p.k_blocks) * (w.split + 1) / p.splits);
+    return w;
+}
+
+// COLUMN_SCALES: sb holds one scale per column instead of one per 128.
+template <bool COLUMN_SCALES>
+__global__ void __launch_bounds__(kThreads, 1)
+block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bar_full = base + Layout::kFull, bar_empty = base + Layout::kEmpty;
+    const uint32_t bar_acc_full = base + Layout::kAccFull, bar_acc_empty = base + Layout::kAccEmpty;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + Layout::kTmemPtr);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + Layout::kAbort);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cta = static_cast<int>(cluster_cta_rank());
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles = p.m_tiles * p.n_tiles * p.splits;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_acc_full + 8 * b, 1);
+            mbar_init(bar_acc_empty + 8 * b, 16);   // eight epilogue warps of both CTAs
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
+        if (warp == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                const Work w = decode(p, t);
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        const uint32_t full = bar_full + 8 * stage, dst = base + stage * kStageBytes;
+                        if (cta == 0) mbar_expect_tx(full, 2 * kStageBytes);
+                        tma_load_4d_pair(dst, &map_a, full & kPairLeaderMask, kb * BK, w.m0 + cta * BM_CTA, 0, 0);
+                        tma_load_4d_pair(dst + kOperandBytes, &map_b, full & kPairLeaderMask, kb * BK, w.n0 + cta * BN_CTA, 0, 0);
+                    }
+                    __syncwarp();
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        } else if (warp == 1) {
+            if (cta == 0) {
+                int stage = 0;
+                uint32_t phase = 0, block = 0;   // block: blocks of K done so far; accumulator block & 1
+                bool ok = true;
+                for (int t = pair; t < tiles && ok; t += pairs) {
+                    const Work w = decode(p, t);
+                    for (int kb = w.kb0; kb < w.kb1; ++kb, ++block) {
+                        const uint32_t buf = block & 1u;
+                        ok = mbar_wait(bar_acc_empty + 8 * buf, ((block >> 1) & 1u) ^ 1u, abort_flag, p.status) &&
+                             mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        if (lane == 0) {
+                            const uint32_t a = base + stage * kStageBytes;
+                            const uint64_t a_desc = umma_smem_desc(a, 16, 1024), b_desc = umma_smem_desc(a + kOperandBytes, 16, 1024);
+    #pragma unroll
+                            for (int k = 0; k < BK / 32; ++k)
+                                umma_e4m3_pair(tmem + buf * BN, a_desc + k * 2u, b_desc + k * 2u, idesc_e4m3(BM, BN), k != 0 ? 1u : 0u);
+                            umma_commit_pair(bar_empty + 8 * stage);
+                            umma_commit_pair(bar_acc_full + 8 * buf);
+                        }
+                        __syncwarp();
+                        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegisters));
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        float* col_scales = reinterpret_cast<float*>(gen + Layout::kScales) + (warp - 4) * 256;
+        uint8_t* patch = gen + Layout::kPatch + (warp - 4) * kEpiWarpBytes;
+        uint32_t block = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles; t += pairs) {
+            const Work w = decode(p, t);
+            const int row0 = w.m0 + cta * BM_CTA + quarter * 32, row = row0 + lane;
+            const int col0 = w.n0 + half * 128;
+            const float* sa = p.sa + static_cast<long long>(min(row, p.rows - 1)) * p.sa_row;
+            // COLUMN_SCALES: the lane fetches columns lane, lane + 32, ... of the warp's 128; otherwise all four are the block's
+            const float* sb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                sb[j] = p.sb + static_cast<long long>(COLUMN_SCALES ? min(col0 + 32 * j + lane, p.cols - 1) : min(col0, p.cols - 1) / 128) * p.sb_row;
+            float next_a = sa[w.kb0 * p.sa_block], next_b[4];
+#pragma unroll
+            for (int j = 0; j < (COLUMN_SCALES ? 4 : 1); ++j) next_b[j] = sb[j][w.kb0 * p.sb_block];
+            unsigned long long acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
+            for (int kb = w.kb0; kb < w.kb1; ++kb, ++block) {
+                const uint32_t buf = block & 1u;
+                float scale = next_a;
+                const float* cols = col_scales + buf * 128;
+                if (COLUMN_SCALES) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) col_scales[buf * 128 + 32 * j + lane] = next_b[j];
+                    __syncwarp();   // two buffers: this one was read before the previous block's barrier
+                } else {
+                    scale *= next_b[0];
+                }
+                if (kb + 1 < w.kb1) {
+                    next_a = sa[(kb + 1) * p.sa_block];
+#pragma unroll
+                    for (int j = 0; j < (COLUMN_SCALES ? 4 : 1); ++j) next_b[j] = sb[j][(kb + 1) * p.sb_block];
+                }
+                ok = mbar_wait(bar_acc_full + 8 * buf, (block >> 1) & 1u, abort_flag, p.status);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
+                const unsigned long long s2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+                uint32_t v[2][16];
+                tmem_ld_32x16(taddr, v[0]);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < 8) tmem_ld_32x16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
+                    if (c == 7) {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_leader(bar_acc_empty + 8 * buf);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const unsigned long long d = pair_of(v[c & 1][2 * i], v[c & 1][2 * i + 1]);
+                        if (COLUMN_SCALES) {
+                            const unsigned long long cs = *reinterpret_cast<const unsigned long long*>(cols + c * 16 + 2 * i);
+                            acc[c * 8 + i] = pair_fma(d, pair_mul(cs, s2), acc[c * 8 + i]);
+                        } else {
+                            acc[c * 8 + i] = pair_fma(d, s2, acc[c * 8 + i]);
+                        }
+                    }
+                }
+            }
+            if (!ok) {   // a wait ran out (reported in the status word): this tile and the ones that follow are NaN
+                const unsigned long long nan2 = 0x7FC000007FC00000ull;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) acc[i] = nan2;
+            }
+            if (p.splits > 1) {
+                // one row per lane, 16 bytes at a time; a line is filled by eight stores of one lane and merges in L2
+                if (row < p.rows) {
+                    float* out = p.partial + (static_cast<long long>(w.split) * p.rows + row) * p.cols;
+                    const bool whole = (p.cols & 3) == 0;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        uint32_t f[4];
+                        pair_split(acc[2 * i], f[0], f[1]);
+                        pair_split(acc[2 * i + 1], f[2], f[3]);
+                        const int col = col0 + 4 * i;
+                        if (whole && col < p.cols) {
+                            *reinterpret_cast<uint4*>(out + col) = make_uint4(f[0], f[1], f[2], f[3]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (col + j < p.cols) out[col + j] = __uint_as_float(f[j]);
+                        }
+                    }
+                }
+            } else {
+                const bool whole = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4* mine = reinterpret_cast<uint4*>(patch + lane * kEpiRowPitch);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t f[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) pair_split(acc[h * 32 + i * 4 + j], f[2 * j], f[2 * j + 1]);
+                        mine[i] = pack8_bf16(f);
+                    }
+                    __syncwarp();
+                    const int seg = lane & 7, col = col0 + h * 64 + seg * 8;
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int r = it * 4 + (lane >> 3);
+                        const uint4 q = *reinterpret_cast<const uint4*>(patch + r * kEpiRowPitch + seg * 16);
+                        if (row0 + r >= p.rows || col >= p.cols) continue;
+                        bf16* dst = p.out + static_cast<long long>(row0 + r) * p.out_stride + col;
+                        if (whole && col + 8 <= p.cols) {
+                            *reinterpret_cast<uint4*>(dst) = q;
+                        } else {
+                            const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (col + j < p.cols)
+                                    reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(j & 1 ? word[j >> 1] >> 16 : word[j >> 1]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+
+    if (*abort_flag) {
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem, TMEM_COLS);
+    }
+}
+
+// out = bf16(sum of the shares, in order).
+__global__ void __launch_bounds__(256) sum_shares_kernel(const float* __restrict__ partial, int splits, long long count, int cols,
+                                                         bf16* __restrict__ out, long long out_stride) {
+    const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+    if (i >= count) return;
+    if ((cols & 3) == 0) {
+        float4 s = *reinterpret_cast<const float4*>(partial + i);
+        for (int k = 1; k < splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(partial + k * count + i);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        const long long row = i / cols;
+        bf16* dst = out + row * out_stride + (i - row * cols);
+        if ((out_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+        } else {
+            dst[0] = __float2bfloat16(s.x); dst[1] = __float2bfloat16(s.y);
+            dst[2] = __float2bfloat16(s.z); dst[3] = __float2bfloat16(s.w);
+        }
+    } else {
+        for (int j = 0; j < 4 && i + j < count; ++j) {
+            float s = 0.0f;
+            for (int k = 0; k < splits; ++k) s += partial[k * count + i + j];
+            const long long row = (i + j) / cols;
+            out[row * out_stride + (i + j - row * cols)] = __float2bfloat16(s);
+        }
+    }
+}
+
+int code_map(CUtensorMap* map, const void* base, long long stride, long long rows, int depth) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(depth), static_cast<cuuint64_t>(rows), 1, 1};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(stride), static_cast<cuuint64_t>(stride * rows),
+                                   static_cast<cuuint64_t>(stride * rows)};
+    const cuuint32_t box[4] = {BK, 128, 1, 1};
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int div_up(long long a, int b) { return static_cast<int>((a + b - 1) / b); }
+
+// Shares of K: enough to give every CTA pair a tile, each at least four blocks long (shorter shares pay more for their sums in
+// memory than they save).
+int shares(int tiles, int k_blocks) {
+    const int pairs = sm_count() / 2;
+    int s = pairs / tiles;
+    if (s > k_blocks / 4) s = k_blocks / 4;
+    return s < 1 ? 1 : s;
+}
+
+int plan_splits(long long rows, int cols, int depth) {
+    return shares(div_up(rows, BM) * div_up(cols, BN), div_up(depth, BK));
+}
+
+}  // namespace
+}  // namespace mok
+
+extern "C" int64_t mok_block_matmul_scratch_bytes(int64_t rows, int cols, int depth) {
+    if (rows <= 0 || rows > 0x7fffffffLL || cols <= 0 || depth <= 0) return 0;
+    const int splits = mok::plan_splits(rows, cols, depth);
+    return splits > 1 ? static_cast<int64_t>(splits) * rows * cols * 4 : 0;
+}
+
+extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_scales, int64_t a_scale_row_stride,
+                                int64_t a_scale_block_stride, const void* b, int64_t b_stride, const float* b_scales,
+                                int64_t b_scale_row_stride, int64_t b_scale_block_stride, int b_tile_rows, int64_t rows, int cols,
+                                int depth, void* out, int64_t out_stride, void* scratch, uint32_t* status, mok_stream_t stream) {
+    using namespace mok;
+    if (rows < 0 || cols <= 0 || depth <= 0 || (b_tile_rows != 1 && b_tile_rows != 128)) return MOK_ERR_INVALID_ARGUMENT;
+    if (rows > (1 << 24) || cols > (1 << 24)) return MOK_ERR_TOO_LARGE;
+    if (rows == 0) return MOK_OK;
+    if (!a || !a_scales || !b || !b_scales || !out) return MOK_ERR_INVALID_ARGUMENT;
+    if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) != 0 || a_stride % 16 != 0 || b_stride % 16 != 0 ||
+        a_stride < depth || b_stride < depth || out_stride < cols)
+        return MOK_ERR_INVALID_ARGUMENT;
+    Product p{};
+    p.sa = a_scales;
+    p.sa_row = a_scale_row_stride;
+    p.sa_block = a_scale_block_stride;
+    p.sb = b_scales;
+    p.sb_row = b_scale_row_stride;
+    p.sb_block = b_scale_block_stride;
+    p.out = static_cast<bf16*>(out);
+    p.out_stride = out_stride;
+    p.rows = static_cast<int>(rows);
+    p.cols = cols;
+    p.k_blocks = div_up(depth, BK);
+    p.m_tiles = div_up(rows, BM);
+    p.n_tiles = div_up(cols, BN);
+    p.splits = plan_splits(rows, cols, depth);
+    p.partial = static_cast<float*>(scratch);
+    p.status = status;
+    if (p.splits > 1 && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0)) return MOK_ERR_INVALID_ARGUMENT;
+    if (static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits > 0x7fffffffLL) return MOK_ERR_TOO_LARGE;
+    CUtensorMap map_a, map_b;
+    MOK_TRY(code_map(&map_a, a, a_stride, rows, depth));
+    MOK_TRY(code_map(&map_b, b, b_stride, cols, depth));
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const int tiles = p.m_tiles * p.n_tiles * p.splits;
+    if (b_tile_rows == 1) {
+        static int resident[16] = {0};
+        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<true>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, p));
+    } else {
+        static int resident[16] = {0};
+        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<false>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, p));
+    }
+    if (p.splits > 1) {
+        const long long count = rows * cols;
+        sum_shares_kernel<<<static_cast<unsigned>((count + 1023) / 1024), 256, 0, s>>>(p.partial, p.splits, count, cols, p.out, out_stride);
+        MOK_LAUNCH_CHECK("sum_shares_kernel");
+    }
+    return MOK_OK;
+}

@@ -2,6 +2,7 @@
 `torch.compile(fullgraph=True)` see the same outputs the CUDA ops allocate (reference: mok/_fake_impls.py)."""
 import torch
 
+from . import block_ops as _block_ops
 from . import ops as _ops  # noqa: F401  (the ops must be defined before their fakes are registered)
 
 _FP8 = torch.float8_e4m3fn
@@ -164,3 +165,32 @@ def _(x, w_router, bias, topk):
 def _(x, w_router, top_experts, router_weights, d_router_weights, has_bias):
     E, H = w_router.shape
     return (torch.empty_like(x), x.new_empty((E, H), dtype=torch.float32), x.new_empty((E,), dtype=torch.float32))
+
+
+@torch.library.register_fake("mok::rms_norm_fwd")
+def _(x, weight, residual, eps):
+    return (x.new_empty(x.shape), x.new_empty(x.shape if residual is not None else (0,)), x.new_empty(x.shape[:1], dtype=torch.float32))
+
+
+@torch.library.register_fake("mok::rms_norm_fp8_fwd")
+def _(x, weight, residual, eps):
+    T, H = x.shape
+    return (_block_ops._new_codes(x, T, H), _block_ops._new_scales(x, T, H, 1), x.new_empty(x.shape if residual is not None else (0,)))
+
+
+@torch.library.register_fake("mok::rms_norm_bwd")
+def _(d_y, d_hidden, z, weight, inv_rms):
+    return z.new_empty(z.shape), weight.new_empty(weight.shape)
+
+
+@torch.library.register_fake("mok::block_quantize")
+def _(x, tile_rows, transpose):
+    M, N = x.shape
+    t = ((_block_ops._new_codes(x, N, M), _block_ops._new_scales(x, N, M, tile_rows)) if transpose
+         else (x.new_empty((0,), dtype=_FP8), x.new_empty((0,), dtype=torch.float32)))
+    return (_block_ops._new_codes(x, M, N), _block_ops._new_scales(x, M, N, tile_rows)) + t
+
+
+@torch.library.register_fake("mok::block_matmul")
+def _(a, a_scales, b, b_scales):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=torch.bfloat16)

@@ -116,6 +116,20 @@ def lib() -> ctypes.CDLL:
         L.mok_router_backward.argtypes = [c_void_p] * 5 + [c_int64] + [c_int] * 4 + [c_void_p] * 6
         L.mok_router_forward.restype = c_int
         L.mok_router_backward.restype = c_int
+        L.mok_rms_norm_forward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_void_p,
+                                           c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p]
+        L.mok_rms_norm_scratch_bytes.argtypes = [c_int64, c_int]
+        L.mok_rms_norm_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int,
+                                            c_void_p, c_void_p, c_void_p, c_void_p]
+        L.mok_block_quantize.argtypes = [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                         c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p]
+        L.mok_block_matmul_scratch_bytes.argtypes = [c_int64, c_int, c_int]
+        L.mok_block_matmul.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                       c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
+        for name in ("mok_rms_norm_scratch_bytes", "mok_block_matmul_scratch_bytes"):
+            getattr(L, name).restype = c_int64
+        for name in ("mok_rms_norm_forward", "mok_rms_norm_backward", "mok_block_quantize", "mok_block_matmul"):
+            getattr(L, name).restype = c_int
         for name in ("mok_schedule", "mok_all_gather_top_experts", "mok_barrier_all", "mok_fwd_epilogue", "mok_bwd_epilogue",
                      "mok_mxfp8_quantize", "mok_moe_forward_bf16", "mok_moe_recompute_bf16", "mok_moe_backward_bf16",
                      "mok_grouped_gemm_bf16", "mok_grouped_wgrad_bf16"):
@@ -135,6 +149,19 @@ def check(rc: int, what: str) -> None:
 
 def stream_ptr(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(what: str, function, device: torch.device, *args) -> None:
+    """Calls an entry point whose last argument is the stream, on `device` (made current for the call) and its current stream.
+    Tensors are passed as addresses (`Tensor.data_ptr()`, None = NULL): small operators are bound by this path."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != MOK_OK:
+        check(rc, what)
 
 
 def ptr(t: torch.Tensor | None) -> c_void_p:
