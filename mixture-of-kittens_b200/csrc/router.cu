@@ -104,6 +104,67 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const bf16* __restrict_
     }
 }
 
+// Logits for a few tokens, in fp32 throughout: the block's threads share the depth, a thread keeps EXPERTS x TOKENS sums.  One
+// token: bound by latency, so every expert gets a block of its own.  More than 8: 4 x 8 sums per thread, so that the router matrix
+// is read once per 8 tokens and the tokens once per 4 experts (from L2).  The tensor-core form of router_fwd needs 256 rows a tile.
+template <int EXPERTS, int TOKENS, bool W32>
+__global__ void __launch_bounds__(256) few_logits_kernel(const bf16* __restrict__ x, long long x_stride, const void* __restrict__ w, int tokens,
+                                                         int hidden, int experts, float* __restrict__ logits) {
+    __shared__ float part[8][EXPERTS * TOKENS];
+    const int e0 = blockIdx.x * EXPERTS, t0 = blockIdx.y * TOKENS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float acc[EXPERTS][TOKENS];
+#pragma unroll
+    for (int e = 0; e < EXPERTS; ++e)
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) acc[e][t] = 0.0f;
+    for (int k = threadIdx.x * 8; k < hidden; k += 2048) {
+        float wv[EXPERTS][8];
+#pragma unroll
+        for (int e = 0; e < EXPERTS; ++e) {
+            const long long at = static_cast<long long>(min(e0 + e, experts - 1)) * hidden + k;
+            if (W32) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + at));
+                const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + at + 4));
+                wv[e][0] = a.x; wv[e][1] = a.y; wv[e][2] = a.z; wv[e][3] = a.w;
+                wv[e][4] = b.x; wv[e][5] = b.y; wv[e][6] = b.z; wv[e][7] = b.w;
+            } else {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const bf16*>(w) + at));
+                const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+                wv[e][0] = a.x; wv[e][1] = a.y; wv[e][2] = b.x; wv[e][3] = b.y;
+                wv[e][4] = c.x; wv[e][5] = c.y; wv[e][6] = d.x; wv[e][7] = d.y;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + min(t0 + t, tokens - 1) * x_stride + k));
+            const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+            const float xv[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+#pragma unroll
+            for (int e = 0; e < EXPERTS; ++e)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[e][t] = fmaf(xv[j], wv[e][j], acc[e][t]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EXPERTS; ++e)
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) {
+            float v = acc[e][t];
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+            if (lane == 0) part[warp][e * TOKENS + t] = v;
+        }
+    __syncthreads();
+    if (threadIdx.x < EXPERTS * TOKENS) {
+        const int e = e0 + threadIdx.x / TOKENS, t = t0 + threadIdx.x % TOKENS;
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += part[i][threadIdx.x];
+        if (e < experts && t < tokens) logits[static_cast<long long>(t) * experts + e] = v;
+    }
+}
+
 GemmProblem dense_problem(int tokens, uint32_t* status) {
     GemmProblem p;
     p.num_experts = 1;
@@ -119,6 +180,32 @@ int warp_grid(int tokens) {
     long long blocks = (static_cast<long long>(tokens) + 7) / 8;
     const long long cap = static_cast<long long>(sm_count()) * 8;
     return static_cast<int>(blocks < cap ? blocks : cap);
+}
+
+int launch_topk(const float* logits, const float* bias, int T, int num_experts, int ld, int topk, int32_t* top_experts, float* router_weights,
+                cudaStream_t s) {
+    const int grid = warp_grid(T);
+    const int per_lane = (num_experts + 31) / 32;
+#define MOK_TOPK_CASE(N)                                                                                                   \
+    topk_softmax_kernel<N><<<grid, 256, 0, s>>>(logits, bias, T, num_experts, ld, topk, top_experts, router_weights)
+    if (per_lane <= 1) MOK_TOPK_CASE(1);
+    else if (per_lane <= 2) MOK_TOPK_CASE(2);
+    else if (per_lane <= 4) MOK_TOPK_CASE(4);
+    else if (per_lane <= 8) MOK_TOPK_CASE(8);
+    else if (per_lane <= 16) MOK_TOPK_CASE(16);
+    else MOK_TOPK_CASE(32);
+#undef MOK_TOPK_CASE
+    MOK_LAUNCH_CHECK("topk_softmax_kernel");
+    return MOK_OK;
+}
+
+template <bool W32>
+int launch_few_logits(const bf16* x, long long x_stride, const void* w, int T, int hidden, int experts, float* logits, cudaStream_t s) {
+    if (T == 1) few_logits_kernel<1, 1, W32><<<experts, 256, 0, s>>>(x, x_stride, w, T, hidden, experts, logits);
+    else if (T <= 8) few_logits_kernel<1, 8, W32><<<experts, 256, 0, s>>>(x, x_stride, w, T, hidden, experts, logits);
+    else few_logits_kernel<4, 8, W32><<<dim3((experts + 3) / 4, (T + 7) / 8), 256, 0, s>>>(x, x_stride, w, T, hidden, experts, logits);
+    MOK_LAUNCH_CHECK("few_logits_kernel");
+    return MOK_OK;
 }
 
 }  // namespace
@@ -137,19 +224,7 @@ extern "C" int mok_router_forward(const void* x, const void* w_hi, const void* w
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int T = static_cast<int>(num_tokens);
     MOK_TRY(launch_rows_gemm_f32(dense_problem(T, status), x, hidden, w_hi, w_lo, logits, padded_experts, s));
-    const int grid = warp_grid(T);
-    const int per_lane = (num_experts + 31) / 32;
-#define MOK_TOPK_CASE(N)                                                                                                   \
-    topk_softmax_kernel<N><<<grid, 256, 0, s>>>(logits, bias, T, num_experts, padded_experts, topk, top_experts, router_weights)
-    if (per_lane <= 1) MOK_TOPK_CASE(1);
-    else if (per_lane <= 2) MOK_TOPK_CASE(2);
-    else if (per_lane <= 4) MOK_TOPK_CASE(4);
-    else if (per_lane <= 8) MOK_TOPK_CASE(8);
-    else if (per_lane <= 16) MOK_TOPK_CASE(16);
-    else MOK_TOPK_CASE(32);
-#undef MOK_TOPK_CASE
-    MOK_LAUNCH_CHECK("topk_softmax_kernel");
-    return MOK_OK;
+    return launch_topk(logits, bias, T, num_experts, padded_experts, topk, top_experts, router_weights, s);
 }
 
 extern "C" int mok_router_backward(const void* x, const void* w_hi, const int32_t* top_experts, const float* router_weights,
@@ -178,4 +253,20 @@ extern "C" int mok_router_backward(const void* x, const void* w_hi, const int32_
         MOK_LAUNCH_CHECK("column_sum_kernel");
     }
     return MOK_OK;
+}
+
+extern "C" int mok_router_decode(const void* x, int64_t x_stride, const void* w, int w_is_f32, const float* bias, int num_tokens, int hidden,
+                                 int num_experts, int topk, float* logits, int32_t* top_experts, float* router_weights, mok_stream_t stream) {
+    using namespace mok;
+    if (!x || !w || !logits || !top_experts || !router_weights) return MOK_ERR_INVALID_ARGUMENT;
+    if (num_tokens <= 0 || hidden <= 0 || hidden % 8 != 0 || num_experts <= 0 || topk <= 0 || topk > num_experts || topk > kMaxRouterTopk)
+        return MOK_ERR_INVALID_ARGUMENT;
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) != 0 || x_stride % 8 != 0 || x_stride < 0)
+        return MOK_ERR_INVALID_ARGUMENT;
+    if (num_experts > kMaxRouterExperts || num_tokens > 256) return MOK_ERR_TOO_LARGE;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const bf16* xb = static_cast<const bf16*>(x);
+    MOK_TRY(w_is_f32 ? launch_few_logits<true>(xb, x_stride, w, num_tokens, hidden, num_experts, logits, s)
+                     : launch_few_logits<false>(xb, x_stride, w, num_tokens, hidden, num_experts, logits, s));
+    return launch_topk(logits, bias, num_tokens, num_experts, num_experts, topk, top_experts, router_weights, s);
 }

@@ -3,6 +3,7 @@
 import torch
 
 from . import block_ops as _block_ops
+from . import decode as _decode  # noqa: F401
 from . import ops as _ops  # noqa: F401  (the ops must be defined before their fakes are registered)
 
 _FP8 = torch.float8_e4m3fn
@@ -194,3 +195,14 @@ def _(x, tile_rows, transpose):
 @torch.library.register_fake("mok::block_matmul")
 def _(a, a_scales, b, b_scales):
     return a.new_empty((a.shape[0], b.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.register_fake("mok::router_decode")
+def _(x, w_router, bias, topk):
+    return x.new_empty((x.shape[0], topk), dtype=torch.int32), x.new_empty((x.shape[0], topk), dtype=torch.float32)
+
+
+@torch.library.register_fake("mok::moe_decode")
+def _(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, w_routed_gate, w_routed_gate_sc, w_routed_up,
+      w_routed_up_sc, w_routed_down, w_routed_down_sc, first_expert, swiglu_limit):
+    return x.new_empty(x.shape)

@@ -126,9 +126,15 @@ def lib() -> ctypes.CDLL:
         L.mok_block_matmul_scratch_bytes.argtypes = [c_int64, c_int, c_int]
         L.mok_block_matmul.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                        c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
-        for name in ("mok_rms_norm_scratch_bytes", "mok_block_matmul_scratch_bytes"):
+        L.mok_router_decode.argtypes = [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                        c_void_p, c_void_p]
+        L.mok_moe_decode_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int]
+        L.mok_moe_decode.argtypes = ([c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int]
+                                     + [c_void_p] * 6 + [c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
+        for name in ("mok_rms_norm_scratch_bytes", "mok_block_matmul_scratch_bytes", "mok_moe_decode_scratch_bytes"):
             getattr(L, name).restype = c_int64
-        for name in ("mok_rms_norm_forward", "mok_rms_norm_backward", "mok_block_quantize", "mok_block_matmul"):
+        for name in ("mok_rms_norm_forward", "mok_rms_norm_backward", "mok_block_quantize", "mok_block_matmul", "mok_router_decode",
+                     "mok_moe_decode"):
             getattr(L, name).restype = c_int
         for name in ("mok_schedule", "mok_all_gather_top_experts", "mok_barrier_all", "mok_fwd_epilogue", "mok_bwd_epilogue",
                      "mok_mxfp8_quantize", "mok_moe_forward_bf16", "mok_moe_recompute_bf16", "mok_moe_backward_bf16",

@@ -13,6 +13,8 @@ import torch.distributed as dist
 
 from . import functional as F
 from . import ops
+from .block_ops import quantize_blocks
+from .decode import moe_decode, route_decode
 
 
 def quantize_routed_weights(w_routed_gate: torch.Tensor, w_routed_up: torch.Tensor, w_routed_down: torch.Tensor):
@@ -114,6 +116,7 @@ class MoKMoE(torch.nn.Module):
         self.config = config or F.MoKConfig()
         self.swiglu_limit, self.recompute, self.mxfp8 = swiglu_limit, recompute, mxfp8
         self._quantized = None
+        self._quantized_blocks = None
         self.cache_quantized = cache_quantized
         e_loc = num_experts // ep
 
@@ -126,10 +129,11 @@ class MoKMoE(torch.nn.Module):
         self.w_routed_down = param(e_loc, hidden_size, intermediate_size)
 
     def invalidate_quantized(self) -> None:
-        """Drops the cached MXFP8 copies of the routed weights; the next forward quantizes again.  Call it after any
+        """Drops the cached 8-bit copies of the routed weights; the next forward or decode quantizes again.  Call it after any
         weight update the version counters cannot see: writes through `param.data` (fused or foreach optimizers that
         hold flat buffers, ZeRO-style shards, `param.data.copy_`)."""
         self._quantized = None
+        self._quantized_blocks = None
 
     def _quantized_weights(self):
         """MXFP8 copies of the routed weights, rebuilt only after one of them changed (optimizer step, load_state_dict).
@@ -149,3 +153,29 @@ class MoKMoE(torch.nn.Module):
                          self.w_routed_gate, self.w_routed_up, self.w_routed_down, group=self.group, config=self.config,
                          swiglu_limit=self.swiglu_limit, recompute=self.recompute, mxfp8=self.mxfp8,
                          quantized_weights=self._quantized_weights() if self.mxfp8 else None)
+
+    def _block_weights(self):
+        """8-bit copies of the routed weights with scales per 128 x 128, kept like those of `_quantized_weights`."""
+        params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
+        key = tuple((p.data_ptr(), p._version) for p in params)
+        if not self.cache_quantized or self._quantized_blocks is None or self._quantized_blocks[0] != key:
+            with torch.no_grad():
+                self._quantized_blocks = (key, tuple(quantize_blocks(p, tile_rows=128) for p in params))
+        return self._quantized_blocks[1]
+
+    @torch.no_grad()
+    def decode(self, x: torch.Tensor, *, fp8: bool = False) -> torch.Tensor:
+        """The layer for a serving step of 1 to 256 tokens (`moe_decode`), router included; not differentiable.  With `fp8` the
+        routed experts are read from 8-bit copies with a scale per 128 x 128, made on the first call and again after a weight
+        changed.
+
+        With several expert-parallel ranks every rank passes the same tokens; each adds its own experts' part, rank 0 the shared
+        expert's, and the parts (rounded to bf16, as they travel) are summed over the group."""
+        experts, weights = route_decode(x, self.router, topk=self.topk)
+        rank, e_loc = dist.get_rank(self.group), self.w_routed_gate.shape[0]
+        shared = (self.w_shared_gate, self.w_shared_up, self.w_shared_down) if rank == 0 else (None, None, None)
+        routed = self._block_weights() if fp8 else (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
+        out = moe_decode(x, experts, weights, *shared, *routed, first_expert=rank * e_loc, swiglu_limit=self.swiglu_limit)
+        if e_loc != self.num_experts:
+            dist.all_reduce(out, group=self.group)
+        return out
