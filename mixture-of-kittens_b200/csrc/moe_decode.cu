@@ -132,7 +132,7 @@ struct Piece {
     int expert, row, count, from, tokens;
 };
 
-// Calls f for every piece of the gate / up kernel that belongs to this block, in order.
+// Calls f for every piece of the gate / up kernel that belongs to this block, in order, until it returns false.
 template <typename F>
 __device__ __forceinline__ void for_gate_up_pieces(const Decode& p, const Routing& r, F&& f) {
     constexpr int kPairs = kPieceRows / 2;
@@ -145,7 +145,7 @@ __device__ __forceinline__ void for_gate_up_pieces(const Decode& p, const Routin
             q.count = min(kPairs, end - q.row);
             for (q.from = 0; q.from < p.tokens; q.from += p.token_cap) {
                 q.tokens = min(p.token_cap, p.tokens - q.from);
-                f(q);
+                if (!f(q)) return;
             }
         }
     }
@@ -158,7 +158,7 @@ __device__ __forceinline__ void for_gate_up_pieces(const Decode& p, const Routin
         q.count = static_cast<int>(min(static_cast<long long>(min(kPairs, p.intermediate - q.row)), end - at));
         for (q.from = r.begin[a]; q.from < r.begin[a + 1]; q.from += p.token_cap) {
             q.tokens = min(p.token_cap, r.begin[a + 1] - q.from);
-            f(q);
+            if (!f(q)) return;
         }
         at += q.count;
     }
@@ -177,7 +177,7 @@ __device__ __forceinline__ void for_down_pieces(const Decode& p, const Routing& 
             q.count = first + (end - first) * (i + 1) / pieces - q.row;
             for (q.from = from; q.from < to; q.from += p.token_cap) {
                 q.tokens = min(p.token_cap, to - q.from);
-                f(q);
+                if (!f(q)) return;
             }
         }
     }
@@ -210,29 +210,6 @@ __device__ __forceinline__ Block set_up(const Decode& p, uint8_t* smem, uint64_t
     return b;
 }
 
-// Waits that ran out leave copies in flight, which must land before the block's shared memory is given away.
-__device__ __forceinline__ void leave(const Block& b) {
-    if (*b.abort_flag)
-        for (int i = 0; i < 64; ++i) __nanosleep(2000);
-    __syncthreads();
-}
-
-// The producer's side of a piece: one chunk after the other, weights and tokens.
-template <typename F>
-__device__ __forceinline__ bool produce(Ring& ring, const Block& b, const Rows& rows, int k_total, int lane, uint32_t* status) {
-    for (int k0 = 0; k0 < k_total; k0 += F::kChunk) {
-        if (!mbar_wait(ring.empty + 8 * ring.stage, ring.phase ^ 1u, b.abort_flag, status)) return false;
-        const int len = min(F::kChunk, k_total - k0);
-        const uint32_t weight_bytes = len * (F::kRowBytes / F::kChunk), token_bytes = len * (F::kTokenBytes / F::kChunk);
-        if (lane == 0) mbar_expect_tx(ring.full + 8 * ring.stage, rows.weights * weight_bytes + rows.tokens * token_bytes);
-        __syncwarp();
-        load_weights<F>(ring, rows, k0, lane, weight_bytes);
-        load_tokens<F>(ring, ring.stage, rows.token, k0, lane, token_bytes);
-        ring.advance();
-    }
-    return true;
-}
-
 template <bool W8, int NT>
 __device__ __forceinline__ void consume_gate_up(Ring& ring, const Block& b, const Decode& p, const Piece& q, int warp, int lane,
                                                 float (&acc)[2][NT][4]) {
@@ -261,26 +238,35 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_gate_up_kernel(
     Block b = set_up<NT>(p, smem, bars, &abort_flag, 0, false);
     find_experts<false>(p, b.routing);   // its barriers also publish the ring
     Ring ring = b.ring;
-    if (warp == kConsumers) {
+    if (warp >= kConsumers) {
+        const int producer = warp - kConsumers;
         bool ok = true;
         for_gate_up_pieces(p, b.routing, [&](const Piece& q) {
-            if (!ok) return;
-            const bool w8 = W8 && q.expert >= 0;
-            const int pair = (lane >> 4) * 8 + (lane & 7);
-            Rows rows;
-            rows.weights = 2 * q.count;
-            rows.tokens = q.tokens;
-            const uint8_t* w = q.expert < 0 ? reinterpret_cast<const uint8_t*>(lane & 8 ? p.shared_up : p.shared_gate) : (lane & 8 ? p.up : p.gate);
-            const long long row = (q.expert < 0 ? 0 : static_cast<long long>(q.expert) * p.intermediate) + q.row + pair;
-            rows.weight = pair < q.count ? w + row * p.hidden_size * (w8 ? 1 : 2) : nullptr;
-            rows.token = nullptr;
-            if (lane < q.tokens) {
-                const int token = q.expert < 0 ? q.from + lane : b.routing.list[q.from + lane] / p.topk;
-                rows.token = reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride);
+            const bool shared = q.expert < 0, w8 = W8 && !shared;
+            Feed<NT> f;
+            const long long row_bytes = p.hidden_size * (w8 ? 1 : 2);
+            const uint8_t* gate = shared ? reinterpret_cast<const uint8_t*>(p.shared_gate) : p.gate;
+            const uint8_t* up = shared ? reinterpret_cast<const uint8_t*>(p.shared_up) : p.up;
+            const long long at = ((shared ? 0 : static_cast<long long>(q.expert) * p.intermediate) + q.row) * row_bytes + lane * 16;
+#pragma unroll
+            for (int j = 0; j < Feed<NT>::kWeights; ++j) {   // m tile m of the piece: eight gate rows from 8 m on and the same up rows
+                const int i = producer + j * kProducers, pair = (i >> 4) * 8 + (i & 7);
+                f.weight[j] = pair < q.count ? (i & 8 ? up : gate) + at + pair * row_bytes : nullptr;
             }
-            ok = w8 ? produce<Form<W8, false>>(ring, b, rows, p.hidden_size, lane, p.status)
-                    : produce<Form<false, false>>(ring, b, rows, p.hidden_size, lane, p.status);
+#pragma unroll
+            for (int j = 0; j < Feed<NT>::kTokens; ++j) {
+                const int i = producer + j * kProducers;
+                f.token[j] = nullptr;
+                if (i < q.tokens) {
+                    const int token = shared ? q.from + i : b.routing.list[q.from + i] / p.topk;
+                    f.token[j] = reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride) + lane * 16;
+                }
+            }
+            if (w8) ok = produce<Form<W8, false>, NT>(ring, b.abort_flag, p.status, f, 0, p.hidden_size, producer, lane);
+            else ok = produce<Form<false, false>, NT>(ring, b.abort_flag, p.status, f, 0, p.hidden_size, producer, lane);
+            return ok;
         });
+        wait_copies();
     } else {
         for_gate_up_pieces(p, b.routing, [&](const Piece& q) {
             float acc[2][NT][4];
@@ -302,9 +288,9 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_gate_up_kernel(
                 else p.hidden[static_cast<long long>(b.routing.list[q.from + c]) * p.intermediate + q.row + pair] = h;
             }
             consumer_barrier();
+            return true;
         });
     }
-    leave(b);
 }
 
 template <bool W8, int NT>
@@ -326,13 +312,6 @@ __device__ __forceinline__ void consume_down(Ring& ring, const Block& b, const D
     consume<W8, false, NT>(ring, b.stages, b.abort_flag, p.status, depth, (q.count + 15) / 16, (q.tokens + 7) / 8, s, warp, lane, acc);
 }
 
-// Hidden rows that wait for the gate / up kernel: the first stages carry weights only until then.
-struct Held {
-    const uint8_t* token;
-    int k0;
-    uint32_t bytes;
-};
-
 template <bool W8, int NT>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_down_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -346,60 +325,65 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_down_kernel(con
     for (int i = threadIdx.x; i < p.tokens * cols; i += kThreads) b.sums[i] = 0.0f;
     find_experts<true>(p, b.routing);
     Ring ring = b.ring;
-    if (warp == kConsumers) {
-        bool ok = true, released = false;
-        int held = 0;
-        Held hold[kMaxStages];
-        bool hold_w8[kMaxStages];
-        auto release = [&]() {
-            wait_previous_kernel();
-            asm volatile("fence.proxy.async;" ::: "memory");   // hidden rows were written by ordinary stores
-            for (int i = 0; i < held; ++i) {
-                if (hold_w8[i]) load_tokens<Form<W8, false>>(ring, i, hold[i].token, hold[i].k0, lane, hold[i].bytes);
-                else load_tokens<Form<false, false>>(ring, i, hold[i].token, hold[i].k0, lane, hold[i].bytes);
+    if (warp >= kConsumers) {
+        const int producer = warp - kConsumers;
+        // Until the gate / up kernel is done the stages of an empty ring get their weights only; the hidden rows follow.
+        bool ok = true;
+        int early = 0;   // stages that have their weights
+        auto feed = [&](const Piece& q, Feed<NT>& f) {
+            const bool shared = q.expert < 0;
+            const int depth = shared ? p.shared_intermediate : p.intermediate;
+            const long long row_bytes = depth * (W8 && !shared ? 1 : 2);
+            const uint8_t* w = shared ? reinterpret_cast<const uint8_t*>(p.shared_down) : p.down;
+            const bf16* h = shared ? p.hidden_shared : p.hidden;
+            w += ((shared ? 0 : static_cast<long long>(q.expert) * p.hidden_size) + q.row) * row_bytes + lane * 16;
+#pragma unroll
+            for (int j = 0; j < Feed<NT>::kWeights; ++j) {
+                const int i = producer + j * kProducers;
+                f.weight[j] = i < q.count ? w + i * row_bytes : nullptr;
             }
-            released = true;
+#pragma unroll
+            for (int j = 0; j < Feed<NT>::kTokens; ++j) {
+                const int i = producer + j * kProducers;
+                f.token[j] = nullptr;
+                if (i < q.tokens) {
+                    const long long row = shared ? q.from + i : b.routing.list[q.from + i];
+                    f.token[j] = reinterpret_cast<const uint8_t*>(h + row * depth) + lane * 16;
+                }
+            }
+            return depth;
+        };
+        auto run_early = [&](const Feed<NT>& f, int depth, auto form) {
+            typedef decltype(form) F;
+            for (int k0 = 0; k0 < depth && early < ring.stages; k0 += F::kChunk, ++early)
+                copy_weights<F, NT>(ring.base + early * ring.stage_bytes, f, k0, min(F::kChunk, depth - k0), producer, lane);
         };
         for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
-            if (!ok) return;
-            const bool w8 = W8 && q.expert >= 0;
-            const int depth = q.expert < 0 ? p.shared_intermediate : p.intermediate;
-            Rows rows;
-            rows.weights = q.count;
-            rows.tokens = q.tokens;
-            const uint8_t* w = q.expert < 0 ? reinterpret_cast<const uint8_t*>(p.shared_down) : p.down;
-            const long long row = (q.expert < 0 ? 0 : static_cast<long long>(q.expert) * p.hidden_size) + q.row + lane;
-            rows.weight = lane < q.count ? w + row * depth * (w8 ? 1 : 2) : nullptr;
-            rows.token = nullptr;
-            if (lane < q.tokens) {
-                if (q.expert < 0) rows.token = reinterpret_cast<const uint8_t*>(p.hidden_shared + static_cast<long long>(q.from + lane) * depth);
-                else rows.token = reinterpret_cast<const uint8_t*>(p.hidden + static_cast<long long>(b.routing.list[q.from + lane]) * depth);
-            }
-            auto run = [&](auto form) {
-                typedef decltype(form) F;
-                int k0 = 0;
-                for (; k0 < depth && !released; k0 += F::kChunk) {   // the ring is empty: nothing to wait for
-                    const int len = min(F::kChunk, depth - k0);
-                    const uint32_t weight_bytes = len * (F::kRowBytes / F::kChunk), token_bytes = len * 2;
-                    if (lane == 0) mbar_expect_tx(ring.full + 8 * ring.stage, rows.weights * weight_bytes + rows.tokens * token_bytes);
-                    __syncwarp();
-                    load_weights<F>(ring, rows, k0, lane, weight_bytes);
-                    hold[held] = Held{rows.token, k0, token_bytes};
-                    hold_w8[held] = w8;
-                    ring.advance();
-                    if (++held == ring.stages) release();
-                }
-                if (k0 < depth) {
-                    Rows rest = rows;
-                    if (rest.weight != nullptr) rest.weight += static_cast<long long>(k0) * (F::kRowBytes / F::kChunk);
-                    if (rest.token != nullptr) rest.token += static_cast<long long>(k0) * 2;
-                    ok = produce<F>(ring, b, rest, depth - k0, lane, p.status);
-                }
-            };
-            if (w8) run(Form<W8, false>());
-            else run(Form<false, false>());
+            Feed<NT> f;
+            const int depth = feed(q, f);
+            if (W8 && q.expert >= 0) run_early(f, depth, Form<W8, false>());
+            else run_early(f, depth, Form<false, false>());
+            return early < ring.stages;
         });
-        if (!released) release();
+        wait_previous_kernel();
+        auto run = [&](const Feed<NT>& f, int depth, auto form) {
+            typedef decltype(form) F;
+            int k0 = 0;
+            for (; k0 < depth && early > 0; k0 += F::kChunk, --early) {
+                copy_tokens<F, NT>(ring.base + ring.stage * ring.stage_bytes, f, k0, min(F::kChunk, depth - k0), producer, lane);
+                arrive_when_copied(ring.full + 8 * ring.stage);
+                ring.advance();
+            }
+            ok = produce<F, NT>(ring, b.abort_flag, p.status, f, k0, depth, producer, lane);
+        };
+        for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
+            Feed<NT> f;
+            const int depth = feed(q, f);
+            if (W8 && q.expert >= 0) run(f, depth, Form<W8, false>());
+            else run(f, depth, Form<false, false>());
+            return ok;
+        });
+        wait_copies();
     } else {
         for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
             float acc[2][NT][4];
@@ -420,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_down_kernel(con
                 *sum = fmaf(w, sum_of<NT>(b.scratch, row, c), *sum);
             }
             consumer_barrier();
+            return true;
         });
         wait_previous_kernel();   // its word on how it went
         const bool bad = p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0;
@@ -429,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_down_kernel(con
                 __float2bfloat16(bad ? __uint_as_float(0x7FC00000u) : b.sums[i]);
         }
     }
-    leave(b);
 }
 
 // ---------------------------------------------------------------------------------------------------------

@@ -1,10 +1,11 @@
 // Products of weight rows with a few tokens, for kernels that are bound by reading the weights once: out[row, token] = sum over k
 // of W[row, k] * x[token, k].
 //
-// A block has one producer warp and eight consumer warps.  The producer copies pieces of up to 32 weight rows and the rows of up
-// to 32 tokens, kChunk elements of k at a time, into a ring of stages with untiled bulk copies (one per row: any row count, stride
-// and gather, no tensor map), and runs ahead of the consumers as far as the ring reaches; about 100 KB in flight per SM is what
-// HBM needs.  The consumers split k: a warp takes every eighth slice of a chunk, multiplies it with mma.sync (weights on the M
+// A block has four producer warps and eight consumer warps.  The producers copy pieces of up to 32 weight rows and the rows of up
+// to 32 tokens, kChunk elements of k at a time, into a ring of stages with cp.async (a warp's 32 x 16 bytes are one row of a chunk:
+// any row count, stride and gather), and run ahead of the consumers as far as the ring reaches; about 100 KB in flight per SM is
+// what HBM needs.  Bulk copies, one per row, were measured first: an SM issues about one in 60 clocks, so 512-byte rows came in at
+// 1.4 - 1.8 TB/s and 1024-byte rows at 2.2 - 3.4 TB/s.  The consumers split k: a warp takes every eighth slice of a chunk, multiplies it with mma.sync (weights on the M
 // side, tokens on the N side of 8) and keeps its own sums, which the eight warps add in a fixed order when a piece is done.
 // tcgen05 would need 128 rows a tile, which leaves SMs idle at these sizes; the tensor work here is a few percent of the time.
 //
@@ -20,7 +21,9 @@ namespace stream {
 
 constexpr int kConsumers = 8;                       // warps
 constexpr int kConsumerThreads = kConsumers * 32;
-constexpr int kThreads = kConsumerThreads + 32;
+constexpr int kProducers = 4;
+constexpr int kProducerThreads = kProducers * 32;
+constexpr int kThreads = kConsumerThreads + kProducerThreads;
 constexpr int kPieceRows = 32;                      // weight rows of a piece: two m16 tiles
 constexpr int kMaxStages = 8;
 
@@ -36,10 +39,14 @@ struct Form {
     static constexpr int stage_bytes(int tokens) { return kPieceRows * kRowPitch + tokens * kTokenPitch; }
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// One arrival once every copy that this thread has issued so far is done.
+__device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -62,30 +69,60 @@ struct Ring {
     }
     __device__ __forceinline__ void init() const {   // one thread
         for (int s = 0; s < stages; ++s) {
-            mbar_init(full + 8 * s, 1);
+            mbar_init(full + 8 * s, kProducerThreads);
             mbar_init(empty + 8 * s, kConsumers);
         }
         mbar_fence_init();
     }
 };
 
-// One lane's share of a piece: its weight row and its token row (nullptr: none), and how many rows the warp copies in all.
-struct Rows {
-    const uint8_t *weight, *token;
-    int weights, tokens;
+// What a producer warp copies of a piece: every kProducers-th weight row and token row, as this lane's address in the row at k = 0
+// (nullptr: no such row).  Found once per piece, so that a chunk costs its producers little more than the copies themselves: with
+// addresses worked out chunk by chunk they were the bottleneck (1500 clocks a chunk, 2.2 TB/s).
+template <int NT>
+struct Feed {
+    static constexpr int kWeights = kPieceRows / kProducers, kTokens = 8 * NT / kProducers;
+    const uint8_t *weight[kWeights], *token[kTokens];
 };
-
-template <typename F>
-__device__ __forceinline__ void load_weights(const Ring& r, const Rows& rows, int k0, int lane, uint32_t weight_bytes) {
-    if (rows.weight != nullptr)
-        bulk_load(r.base + r.stage * r.stage_bytes + lane * F::kRowPitch, rows.weight + static_cast<long long>(k0) * (F::kRowBytes / F::kChunk),
-                  weight_bytes, r.full + 8 * r.stage);
+template <typename F, int NT>
+__device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<NT>& f, int k0, int len, int producer, int lane) {
+    constexpr int kBytes = F::kRowBytes / F::kChunk;
+    static_assert(F::kRowBytes == 512, "one copy of 16 bytes per lane");
+    const long long at = static_cast<long long>(k0) * kBytes;
+    const uint32_t dst = stage + producer * F::kRowPitch + lane * 16;
+    if (lane * 16 < len * kBytes) {
+#pragma unroll
+        for (int j = 0; j < Feed<NT>::kWeights; ++j)
+            if (f.weight[j] != nullptr) copy16(dst + j * kProducers * F::kRowPitch, f.weight[j] + at);
+    }
 }
-template <typename F>
-__device__ __forceinline__ void load_tokens(const Ring& r, int stage, const uint8_t* token, int k0, int lane, uint32_t token_bytes) {
-    if (token != nullptr)
-        bulk_load(r.base + stage * r.stage_bytes + kPieceRows * F::kRowPitch + lane * F::kTokenPitch,
-                  token + static_cast<long long>(k0) * (F::kTokenBytes / F::kChunk), token_bytes, r.full + 8 * stage);
+template <typename F, int NT>
+__device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<NT>& f, int k0, int len, int producer, int lane) {
+    constexpr int kBytes = F::kTokenBytes / F::kChunk;
+    const long long at = static_cast<long long>(k0) * kBytes;
+    const uint32_t dst = stage + kPieceRows * F::kRowPitch + producer * F::kTokenPitch + lane * 16;
+#pragma unroll
+    for (int half = 0; half < F::kTokenBytes / 512; ++half)
+        if (half * 512 + lane * 16 < len * kBytes) {
+#pragma unroll
+            for (int j = 0; j < Feed<NT>::kTokens; ++j)
+                if (f.token[j] != nullptr) copy16(dst + j * kProducers * F::kTokenPitch + half * 512, f.token[j] + at + half * 512);
+        }
+}
+// The producers' side of a piece from k0 on, chunk by chunk.  False: a wait ran out.
+template <typename F, int NT>
+__device__ __forceinline__ bool produce(Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed<NT>& f, int k0, int k_total, int producer,
+                                        int lane) {
+    for (; k0 < k_total; k0 += F::kChunk) {
+        if (!mbar_wait(ring.empty + 8 * ring.stage, ring.phase ^ 1u, abort_flag, status)) return false;
+        const int len = min(F::kChunk, k_total - k0);
+        const uint32_t stage = ring.base + ring.stage * ring.stage_bytes;
+        copy_weights<F, NT>(stage, f, k0, len, producer, lane);
+        copy_tokens<F, NT>(stage, f, k0, len, producer, lane);
+        arrive_when_copied(ring.full + 8 * ring.stage);
+        ring.advance();
+    }
+    return true;
 }
 
 // ---- consumer -----------------------------------------------------------------------------------------------------
