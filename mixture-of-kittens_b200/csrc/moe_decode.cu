@@ -2,15 +2,17 @@
 // W_down (silu(W_gate x) * (W_up x)), in two kernels.  With a handful of tokens the layer is the reading of its experts' weights
 // (3 H I elements each, once); padding every expert to 256 rows, staging and combining would cost more than that.
 //
-//   gate / up: the rows of all experts in use lie end to end and are cut evenly, to the row, over the SMs; a piece is 16 gate rows
-//              and the same 16 up rows, so that a lane of the mma holds both and forms hidden = silu(gate) * up itself.
+//   gate / up: the rows of all experts in use lie end to end and are cut evenly, to the row, over the SMs; a piece is 8 gate rows and
+//              the same 8 up rows, so that hidden = silu(gate) * up is formed where the sums end up.
 //   down:      every SM owns a slice of the output's columns and walks all experts, so a token's sum over its experts happens in
-//              one place, in shared memory, in a fixed order: shared expert, then experts by number.  No atomics, no partial rows.
+//              one place, in shared memory, in a fixed order: shared expert, then experts by number.  No atomics on values, no
+//              partial rows.  The warp that completes an expert's sum adds it while the others are at the next experts: when the
+//              whole block met for every expert, 2000 of 2500 clocks an expert were latency (hidden 2048, intermediate 768).
 //
 // The second kernel is launched while the first runs, next to it on each SM, fills its ring with down weights and waits for the
 // hidden rows in hardware (programmatic dependent launch): no spinning, and nothing has to be co-resident for it to finish.
-// Every block finds out by itself which experts are in use and by whom (at most 4096 routes, in shared memory); hidden rows are
-// kept by route number, so the order in which that happens does not matter.
+// Every block finds out by itself which experts are in use and by whom, while its producers already copy the shared expert's
+// weights; hidden rows are kept by route number, so the order in which that happens does not matter.
 #include "swiglu_math.cuh"
 #include "weight_stream.cuh"
 
@@ -22,6 +24,8 @@ using namespace stream;
 constexpr int kMaxTokens = 256;
 constexpr int kMaxTopk = 32;
 constexpr int kMaxRoutes = 4096;
+constexpr int kPairs = kRows / 2;
+constexpr int kNobody = 0xFFFF;
 
 struct Decode {
     const bf16* x;
@@ -39,91 +43,96 @@ struct Decode {
     int stages, stage_bytes, token_cap;   // the ring; tokens of a stage
 };
 
-// Which experts are in use: active[i] and the range [begin[i], begin[i + 1]) of its routes in list.
+// Which experts are in use: active[i], and the range [begin[i], begin[i + 1]) of its routes in list (with their tokens and weights
+// beside).  An expert that a token names more than once is listed once, with the sum of the weights.  passes[i]: how often the
+// experts before i are read in all, when token_cap of their tokens fit a stage.
 struct Routing {
-    int* counts;        // [experts], then the next free place of each
-    uint16_t* active;   // [experts]
-    uint16_t* begin;    // [experts + 1], 4096 at most
-    uint16_t* list;     // [routes]
-    float* weights;     // [routes], beside list (down kernel)
     int* num_active;
+    int* next;               // [experts] counts, then the next free place in list
+    float* weights;          // [routes]
+    uint16_t *expert;        // [routes] of this rank, or kNobody
+    uint16_t *active, *begin, *passes, *list;   // [experts], [experts + 1], [experts + 1], [routes]
+    uint8_t* token;          // [routes]
 };
-__host__ __device__ __forceinline__ int routing_bytes(int experts, int routes, bool weights) {
-    return 16 + 4 * experts + (weights ? 4 * routes : 0) + 2 * (2 * experts + 1 + routes) + 16;
+__host__ __device__ __forceinline__ int routing_bytes(int experts, int routes) {
+    return 16 + 4 * experts + 4 * routes + 2 * (routes + 3 * experts + 2 + routes) + routes + 16;
 }
-__device__ __forceinline__ Routing carve_routing(uint8_t* smem, int experts, int routes, bool weights) {
+__device__ __forceinline__ Routing carve_routing(uint8_t* smem, int experts, int routes) {
     Routing r;
     r.num_active = reinterpret_cast<int*>(smem);
-    r.counts = reinterpret_cast<int*>(smem + 16);
-    r.weights = reinterpret_cast<float*>(r.counts + experts);
-    r.active = reinterpret_cast<uint16_t*>(r.weights + (weights ? routes : 0));
+    r.next = reinterpret_cast<int*>(smem + 16);
+    r.weights = reinterpret_cast<float*>(r.next + experts);
+    r.expert = reinterpret_cast<uint16_t*>(r.weights + routes);
+    r.active = r.expert + routes;
     r.begin = r.active + experts;
-    r.list = r.begin + experts + 1;
+    r.passes = r.begin + experts + 1;
+    r.list = r.passes + experts + 1;
+    r.token = reinterpret_cast<uint8_t*>(r.list + routes);
     return r;
 }
 
-// The expert of route i on this rank if the route counts: -1 for other ranks' experts, and for an expert that the token named
-// before (the first occurrence carries the sum of the weights).
-__device__ __forceinline__ int local_expert(const Decode& p, int i) {
-    const int route = p.routes[i];
-    const uint32_t e = static_cast<uint32_t>(route) - static_cast<uint32_t>(p.first_expert);
-    if (e >= static_cast<uint32_t>(p.experts)) return -1;
-    for (int j = i / p.topk * p.topk; j < i; ++j)
-        if (p.routes[j] == route) return -1;
-    return static_cast<int>(e);
-}
-// All threads of the block.
-template <bool WEIGHTS>
+// The consumer threads of the block.
 __device__ __forceinline__ void find_experts(const Decode& p, const Routing& r) {
     const int routes = p.tokens * p.topk;
-    for (int e = threadIdx.x; e < p.experts; e += kThreads) r.counts[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < routes; i += kThreads) {
-        const int e = local_expert(p, i);
-        if (e >= 0) atomicAdd(&r.counts[e], 1);
+    for (int i = threadIdx.x; i < routes; i += kConsumerThreads) {
+        const uint32_t e = static_cast<uint32_t>(p.routes[i]) - static_cast<uint32_t>(p.first_expert);
+        r.expert[i] = static_cast<uint16_t>(e < static_cast<uint32_t>(p.experts) ? e : kNobody);
     }
-    __syncthreads();
-    if (threadIdx.x < 32) {   // experts in use and their ranges, by number; counts becomes the first place of each
+    for (int e = threadIdx.x; e < p.experts; e += kConsumerThreads) r.next[e] = 0;
+    consumer_barrier();
+    auto counts = [&](int i, int token) {   // whether route i is its token's first to that expert
+        const int e = r.expert[i];
+        bool first = e != kNobody;
+        for (int j = token * p.topk; j < i; ++j) first = first && r.expert[j] != e;
+        return first;
+    };
+    for (int i = threadIdx.x; i < routes; i += kConsumerThreads)
+        if (counts(i, i / p.topk)) atomicAdd(&r.next[r.expert[i]], 1);
+    consumer_barrier();
+    if (threadIdx.x < 32) {   // experts in use and their ranges, by number
         const int lane = threadIdx.x;
-        int used = 0, total = 0;
+        int used = 0, total = 0;   // total: routes, and passes from bit 16 on (4096 at most of either)
         for (int base = 0; base < p.experts; base += 32) {
             const int e = base + lane;
-            const int c = e < p.experts ? r.counts[e] : 0;
+            const int c = e < p.experts ? r.next[e] : 0;
             const uint32_t here = __ballot_sync(0xffffffffu, c > 0);
-            int sum = c;
+            if (here == 0) continue;
+            const int mine = c | (c + p.token_cap - 1) / p.token_cap << 16;
+            int sum = mine;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int n = __shfl_up_sync(0xffffffffu, sum, off);
                 if (lane >= off) sum += n;
             }
             if (c > 0) {
-                const int at = used + __popc(here & ((1u << lane) - 1u));
+                const int at = used + __popc(here & ((1u << lane) - 1u)), before = total + sum - mine;
                 r.active[at] = static_cast<uint16_t>(e);
-                r.begin[at] = static_cast<uint16_t>(total + sum - c);
-                r.counts[e] = total + sum - c;
+                r.begin[at] = static_cast<uint16_t>(before & 0xFFFF);
+                r.passes[at] = static_cast<uint16_t>(before >> 16);
+                r.next[e] = before & 0xFFFF;
             }
             used += __popc(here);
             total += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (lane == 0) {
-            r.begin[used] = static_cast<uint16_t>(total);
+            r.begin[used] = static_cast<uint16_t>(total & 0xFFFF);
+            r.passes[used] = static_cast<uint16_t>(total >> 16);
             *r.num_active = used;
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < routes; i += kThreads) {
-        const int e = local_expert(p, i);
-        if (e < 0) continue;
-        const int at = atomicAdd(&r.counts[e], 1);
+    consumer_barrier();
+    for (int i = threadIdx.x; i < routes; i += kConsumerThreads) {
+        const int token = i / p.topk;
+        if (!counts(i, token)) continue;
+        float w = p.route_weights[i];
+        for (int j = i + 1; j < (token + 1) * p.topk; ++j)
+            if (r.expert[j] == r.expert[i]) w += p.route_weights[j];
+        const int at = atomicAdd(&r.next[r.expert[i]], 1);   // any order: a column's sums do not depend on its place
         r.list[at] = static_cast<uint16_t>(i);
-        if (WEIGHTS) {
-            float w = p.route_weights[i];
-            for (int j = i + 1; j < (i / p.topk + 1) * p.topk; ++j)
-                if (p.routes[j] == p.routes[i]) w += p.route_weights[j];
-            r.weights[at] = w;
-        }
+        r.token[at] = static_cast<uint8_t>(token);
+        r.weights[at] = w;
     }
-    __syncthreads();
+    consumer_barrier();
 }
 
 // A piece as both sides see it: rows [row, row + count) of an expert (-1: the shared one) times tokens [from, from + tokens) of
@@ -132,313 +141,361 @@ struct Piece {
     int expert, row, count, from, tokens;
 };
 
-// Calls f for every piece of the gate / up kernel that belongs to this block, in order, until it returns false.
+// Calls f for every piece of the gate / up kernel that belongs to this block, in order, until it returns false: first the shared
+// expert's, which need no routing, then the others.
 template <typename F>
-__device__ __forceinline__ void for_gate_up_pieces(const Decode& p, const Routing& r, F&& f) {
-    constexpr int kPairs = kPieceRows / 2;
-    const long long b = blockIdx.x, n = gridDim.x;
+__device__ __forceinline__ bool for_shared_pieces(const Decode& p, F&& f) {
+    if (p.shared_gate == nullptr) return true;
     Piece q;
-    if (p.shared_gate != nullptr) {
-        const int end = static_cast<int>(p.shared_intermediate * (b + 1) / n);
-        q.expert = -1;
-        for (q.row = static_cast<int>(p.shared_intermediate * b / n); q.row < end; q.row += kPairs) {
-            q.count = min(kPairs, end - q.row);
-            for (q.from = 0; q.from < p.tokens; q.from += p.token_cap) {
-                q.tokens = min(p.token_cap, p.tokens - q.from);
-                if (!f(q)) return;
-            }
+    const int end = static_cast<int>(static_cast<long long>(p.shared_intermediate) * (blockIdx.x + 1) / gridDim.x);
+    q.expert = -1;
+    for (q.row = static_cast<int>(static_cast<long long>(p.shared_intermediate) * blockIdx.x / gridDim.x); q.row < end; q.row += kPairs) {
+        q.count = min(kPairs, end - q.row);
+        for (q.from = 0; q.from < p.tokens; q.from += p.token_cap) {
+            q.tokens = min(p.token_cap, p.tokens - q.from);
+            if (!f(q)) return false;
         }
     }
-    const long long rows = static_cast<long long>(*r.num_active) * p.intermediate;
-    const long long end = rows * (b + 1) / n;
-    for (long long at = rows * b / n; at < end;) {
-        const int a = static_cast<int>(at / p.intermediate);
-        q.expert = r.active[a];
-        q.row = static_cast<int>(at - static_cast<long long>(a) * p.intermediate);
-        q.count = static_cast<int>(min(static_cast<long long>(min(kPairs, p.intermediate - q.row)), end - at));
-        for (q.from = r.begin[a]; q.from < r.begin[a + 1]; q.from += p.token_cap) {
-            q.tokens = min(p.token_cap, r.begin[a + 1] - q.from);
-            if (!f(q)) return;
-        }
-        at += q.count;
-    }
+    return true;
 }
-// The same for the down kernel: this block's columns of the output, [first, end).
+// The routed rows, each counted once per pass over its expert (an expert of many tokens is read, from L2, more than once), are cut
+// into equal shares.
 template <typename F>
-__device__ __forceinline__ void for_down_pieces(const Decode& p, const Routing& r, int first, int end, F&& f) {
+__device__ __forceinline__ void for_routed_pieces(const Decode& p, const Routing& r, F&& f) {
     const int active = *r.num_active;
-    const int pieces = (end - first + kPieceRows - 1) / kPieceRows;
+    const long long rows = static_cast<long long>(r.passes[active]) * p.intermediate;
+    const long long first = rows * blockIdx.x / gridDim.x, last = rows * (blockIdx.x + 1) / gridDim.x;
+    if (first == last) return;
+    int a = 0;
+    for (int n = active; n - a > 1;) {   // the expert that `first` lies in
+        const int mid = (a + n) >> 1;
+        if (static_cast<long long>(r.passes[mid]) * p.intermediate <= first) a = mid;
+        else n = mid;
+    }
     Piece q;
-    for (int a = p.shared_gate != nullptr ? -1 : 0; a < active; ++a) {
-        q.expert = a < 0 ? -1 : r.active[a];
-        const int from = a < 0 ? 0 : r.begin[a], to = a < 0 ? p.tokens : r.begin[a + 1];
-        for (int i = 0; i < pieces; ++i) {
-            q.row = first + (end - first) * i / pieces;
-            q.count = first + (end - first) * (i + 1) / pieces - q.row;
-            for (q.from = from; q.from < to; q.from += p.token_cap) {
-                q.tokens = min(p.token_cap, to - q.from);
+    for (; a < active; ++a) {
+        const long long before = static_cast<long long>(r.passes[a]) * p.intermediate;
+        if (before >= last) return;
+        const int passes = r.passes[a + 1] - r.passes[a];
+        const int from = first > before ? static_cast<int>(first - before) / passes : 0;
+        const int to = static_cast<int>(min(last - before, static_cast<long long>(passes) * p.intermediate)) / passes;
+        q.expert = r.active[a];
+        for (q.row = from; q.row < to; q.row += kPairs) {
+            q.count = min(kPairs, to - q.row);
+            for (q.from = r.begin[a]; q.from < r.begin[a + 1]; q.from += p.token_cap) {
+                q.tokens = min(p.token_cap, r.begin[a + 1] - q.from);
                 if (!f(q)) return;
             }
         }
     }
 }
 
-struct Block {
-    Ring ring;
-    const uint8_t* stages;
-    volatile int* abort_flag;
-    float *scratch, *sums;   // sums: the down kernel's [tokens][columns of the block]
-    Routing routing;
-};
-template <int NT>
-__device__ __forceinline__ Block set_up(const Decode& p, uint8_t* smem, uint64_t* bars, int* abort_flag, int sums, bool weights) {
-    Block b;
-    b.stages = smem;
-    b.ring.base = smem_u32(smem);
-    b.ring.full = smem_u32(bars);
-    b.ring.empty = smem_u32(bars + kMaxStages);
-    b.ring.stage_bytes = p.stage_bytes;
-    b.ring.stages = p.stages;
-    b.abort_flag = abort_flag;
-    b.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
-    b.sums = b.scratch + scratch_floats<NT>();
-    b.routing = carve_routing(reinterpret_cast<uint8_t*>(b.sums + (sums + 3) / 4 * 4), p.experts, p.tokens * p.topk, weights);
-    if (threadIdx.x == 0) {
-        *abort_flag = 0;
-        b.ring.init();
-    }
-    return b;
-}
-
+// ---- gate / up --------------------------------------------------------------------------------------------------------
 template <bool W8, int NT>
-__device__ __forceinline__ void consume_gate_up(Ring& ring, const Block& b, const Decode& p, const Piece& q, int warp, int lane,
-                                                float (&acc)[2][NT][4]) {
-    Scales<W8, false, NT> s;
-    if (W8) {
-        const int blocks = (p.hidden_size + 127) / 128, row_blocks = (p.intermediate + 127) / 128;
-        s.row_block = 1;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {   // m tile: eight gate rows and the same up rows
-            const int row = min(q.row + m * 8 + (lane >> 2), p.intermediate - 1);
-            const long long at = (static_cast<long long>(q.expert) * row_blocks + row / 128) * blocks;
-            s.lo[m] = p.gate_scales + at;
-            s.hi[m] = p.up_scales + at;
-        }
-    }
-    consume<W8, false, NT>(ring, b.stages, b.abort_flag, p.status, p.hidden_size, (q.count + 7) / 8, (q.tokens + 7) / 8, s, warp, lane, acc);
-}
-
-template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_gate_up_kernel(const Decode p) {
+__global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages];
-    __shared__ int abort_flag;
+    __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     allow_next_kernel();
-    Block b = set_up<NT>(p, smem, bars, &abort_flag, 0, false);
-    find_experts<false>(p, b.routing);   // its barriers also publish the ring
-    Ring ring = b.ring;
+    Ring ring = set_up_ring(bars, smem, p.stage_bytes, p.stages, kConsumerThreads);
+    Deposit sums;
+    sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
+    const Routing r = carve_routing(reinterpret_cast<uint8_t*>(sums.scratch + deposit_floats<NT>()), p.experts, p.tokens * p.topk);
+    const int chunks = Form<false, false>::chunks(p.hidden_size), chunks8 = Form<true, false>::chunks(p.hidden_size);
     if (warp >= kConsumers) {
-        const int producer = warp - kConsumers;
-        bool ok = true;
-        for_gate_up_pieces(p, b.routing, [&](const Piece& q) {
+        int turn = warp - kConsumers;   // this producer's next chunk, counted from the piece's first
+        auto run = [&](const Piece& q) {
             const bool shared = q.expert < 0, w8 = W8 && !shared;
-            Feed<NT> f;
-            const long long row_bytes = p.hidden_size * (w8 ? 1 : 2);
-            const uint8_t* gate = shared ? reinterpret_cast<const uint8_t*>(p.shared_gate) : p.gate;
-            const uint8_t* up = shared ? reinterpret_cast<const uint8_t*>(p.shared_up) : p.up;
-            const long long at = ((shared ? 0 : static_cast<long long>(q.expert) * p.intermediate) + q.row) * row_bytes + lane * 16;
+            Feed<8 * NT> f;
+            f.row_bytes = p.hidden_size * (w8 ? 1 : 2);
+            f.rows_low = f.rows_high = q.count;
+            const long long at = ((shared ? 0 : static_cast<long long>(q.expert) * p.intermediate) + q.row) * f.row_bytes + lane * 16;
+            f.low = (shared ? reinterpret_cast<const uint8_t*>(p.shared_gate) : p.gate) + at;
+            f.high = (shared ? reinterpret_cast<const uint8_t*>(p.shared_up) : p.up) + at;
 #pragma unroll
-            for (int j = 0; j < Feed<NT>::kWeights; ++j) {   // m tile m of the piece: eight gate rows from 8 m on and the same up rows
-                const int i = producer + j * kProducers, pair = (i >> 4) * 8 + (i & 7);
-                f.weight[j] = pair < q.count ? (i & 8 ? up : gate) + at + pair * row_bytes : nullptr;
-            }
-#pragma unroll
-            for (int j = 0; j < Feed<NT>::kTokens; ++j) {
-                const int i = producer + j * kProducers;
+            for (int j = 0; j < 8 * NT; ++j) {
                 f.token[j] = nullptr;
-                if (i < q.tokens) {
-                    const int token = shared ? q.from + i : b.routing.list[q.from + i] / p.topk;
-                    f.token[j] = reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride) + lane * 16;
-                }
+                if (j < q.tokens) f.token[j] = reinterpret_cast<const uint8_t*>(p.x + (shared ? q.from + j : r.token[q.from + j]) * p.x_stride) + lane * 16;
             }
-            if (w8) ok = produce<Form<W8, false>, NT>(ring, b.abort_flag, p.status, f, 0, p.hidden_size, producer, lane);
-            else ok = produce<Form<false, false>, NT>(ring, b.abort_flag, p.status, f, 0, p.hidden_size, producer, lane);
+            const bool ok = w8 ? produce<Form<W8, false>>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, lane)
+                               : produce<Form<false, false>>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, lane);
+            const int n = w8 ? chunks8 : chunks;
+            turn = (turn - n) & (kProducers - 1);
+            ring.next_piece(n);
             return ok;
-        });
+        };
+        if (for_shared_pieces(p, run) && mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) for_routed_pieces(p, r, run);
         wait_copies();
     } else {
-        for_gate_up_pieces(p, b.routing, [&](const Piece& q) {
-            float acc[2][NT][4];
-            if (W8 && q.expert >= 0) consume_gate_up<W8, NT>(ring, b, p, q, warp, lane, acc);
-            else consume_gate_up<false, NT>(ring, b, p, q, warp, lane, acc);
-            store_sums<NT>(b.scratch, acc, (q.count + 7) / 8, (q.tokens + 7) / 8, warp, lane);
-            consumer_barrier();
-            for (int i = threadIdx.x; i < 16 * q.tokens; i += kConsumerThreads) {
-                const int pair = i & 15, c = i >> 4;
-                if (pair >= q.count) continue;
-                const int row = (pair >> 3) * 16 + (pair & 7);
-                float g = sum_of<NT>(b.scratch, row, c), u = sum_of<NT>(b.scratch, row + 8, c);
-                if (p.clamp) {   // comparisons that let a NaN through
-                    g = g > p.limit ? p.limit : g;
-                    u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+        find_experts(p, r);
+        mbar_arrive(smem_u32(&bars.routed));
+        int turn = warp;   // this warp's next chunk, counted from the piece's first
+        auto run = [&](const Piece& q) {
+            const bool shared = q.expert < 0, w8 = W8 && !shared;
+            const int n = w8 ? chunks8 : chunks, tiles = (q.tokens + 7) >> 3, slots = min(n, kConsumers);
+            const int slot = turn;
+            if (slot < n) {
+                float acc[NT][4];
+                clear(acc);
+                Scales<false, NT> s;
+                if (w8) {
+                    const int blocks = (p.hidden_size + 127) / 128, row_blocks = (p.intermediate + 127) / 128;
+                    const int row = min(q.row + (lane >> 2), p.intermediate - 1);   // rows g and g + 8: gate and up of one pair
+                    const long long at = (static_cast<long long>(q.expert) * row_blocks + row / 128) * blocks;
+                    s.lo = p.gate_scales + at;
+                    s.hi = p.up_scales + at;
+                    s.row_block = 1;
+                    for (int c = slot; c < n; c += kConsumers)
+                        consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, s, lane, acc);
+                } else {
+                    for (int c = slot; c < n; c += kConsumers)
+                        consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, s, lane, acc);
                 }
-                const bf16 h = __float2bfloat16(g * sigmoid_fast(g) * u);
-                if (q.expert < 0) p.hidden_shared[static_cast<long long>(q.from + c) * p.shared_intermediate + q.row + pair] = h;
-                else p.hidden[static_cast<long long>(b.routing.list[q.from + c]) * p.intermediate + q.row + pair] = h;
+                if (deposit<NT>(sums, bars, p.status, acc, slot, slots, tiles, lane)) {
+                    for (int i = lane; i < kPairs * q.tokens; i += 32) {
+                        const int pair = i & (kPairs - 1), c = i / kPairs;
+                        if (pair >= q.count) continue;
+                        float g = sum_of<NT>(sums, slots, pair, c), u = sum_of<NT>(sums, slots, pair + 8, c);
+                        if (p.clamp) {   // comparisons that let a NaN through
+                            g = g > p.limit ? p.limit : g;
+                            u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+                        }
+                        const bf16 h = __float2bfloat16(g * sigmoid_fast(g) * u);
+                        if (shared) p.hidden_shared[static_cast<long long>(q.from + c) * p.shared_intermediate + q.row + pair] = h;
+                        else p.hidden[static_cast<long long>(r.list[q.from + c]) * p.intermediate + q.row + pair] = h;
+                    }
+                    release(sums, bars, lane);
+                }
             }
-            consumer_barrier();
+            ++sums.piece;
+            ring.next_piece(n);
+            turn = (turn - n) & (kConsumers - 1);
             return true;
-        });
+        };
+        for_shared_pieces(p, run);
+        for_routed_pieces(p, r, run);
     }
 }
 
-template <bool W8, int NT>
-__device__ __forceinline__ void consume_down(Ring& ring, const Block& b, const Decode& p, const Piece& q, int warp, int lane,
-                                             float (&acc)[2][NT][4]) {
-    Scales<W8, false, NT> s;
-    const int depth = q.expert < 0 ? p.shared_intermediate : p.intermediate;
-    if (W8) {
-        const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
-        s.row_block = 1;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const int lo = min(q.row + m * 16 + (lane >> 2), p.hidden_size - 1), hi = min(lo + 8, p.hidden_size - 1);
-            const long long at = static_cast<long long>(q.expert) * row_blocks;
-            s.lo[m] = p.down_scales + (at + lo / 128) * blocks;
-            s.hi[m] = p.down_scales + (at + hi / 128) * blocks;
+// ---- down -------------------------------------------------------------------------------------------------------------
+// Rows of the output's slice that this block owns, in `pieces` pieces.
+struct Slice {
+    int first, end, pieces;
+    __device__ __forceinline__ explicit Slice(const Decode& p)
+        : first(static_cast<int>(static_cast<long long>(p.hidden_size) * blockIdx.x / gridDim.x)),
+          end(static_cast<int>(static_cast<long long>(p.hidden_size) * (blockIdx.x + 1) / gridDim.x)), pieces((end - first + kRows - 1) / kRows) {}
+    __device__ __forceinline__ int row(int i) const { return first + (end - first) * i / pieces; }
+};
+// Calls f for every piece of rows [row, row + count), in order, until it returns false.  `shared_only`: those that need no routing.
+template <typename F>
+__device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, int row, int count, bool shared_only, F&& f) {
+    const int active = shared_only ? 0 : *r.num_active;
+    Piece q;
+    q.row = row;
+    q.count = count;
+    for (int a = p.shared_gate != nullptr ? -1 : 0; a < active; ++a) {
+        q.expert = a < 0 ? -1 : r.active[a];
+        const int to = a < 0 ? p.tokens : r.begin[a + 1];
+        for (q.from = a < 0 ? 0 : r.begin[a]; q.from < to; q.from += p.token_cap) {
+            q.tokens = min(p.token_cap, to - q.from);
+            if (!f(q)) return false;
         }
     }
-    consume<W8, false, NT>(ring, b.stages, b.abort_flag, p.status, depth, (q.count + 15) / 16, (q.tokens + 7) / 8, s, warp, lane, acc);
+    return true;
+}
+
+// The producers.  Until the gate / up kernel is done the stages of the empty ring get their weights only; the hidden rows follow.
+template <bool W8, int NT>
+__device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, const Slice& slice, const Ring& start, Bars& bars, int producer, int lane) {
+    constexpr int CAP = 8 * NT;
+    auto depth_of = [&](const Piece& q) { return q.expert < 0 ? p.shared_intermediate : p.intermediate; };
+    auto weights_of = [&](const Piece& q, Feed<CAP>& f) {
+        const bool shared = q.expert < 0;
+        f.row_bytes = depth_of(q) * (W8 && !shared ? 1 : 2);
+        f.rows_low = q.count;
+        f.rows_high = q.count - 8;
+        f.low = (shared ? reinterpret_cast<const uint8_t*>(p.shared_down) : p.down) +
+                ((shared ? 0 : static_cast<long long>(q.expert) * p.hidden_size) + q.row) * f.row_bytes + lane * 16;
+        f.high = f.low + 8 * f.row_bytes;
+    };
+    auto tokens_of = [&](const Piece& q, Feed<CAP>& f) {
+        const bool shared = q.expert < 0;
+        const bf16* h = shared ? p.hidden_shared : p.hidden;
+#pragma unroll
+        for (int j = 0; j < CAP; ++j) {
+            f.token[j] = nullptr;
+            if (j < q.tokens)
+                f.token[j] = reinterpret_cast<const uint8_t*>(h + static_cast<long long>(shared ? q.from + j : r.list[q.from + j]) * depth_of(q)) + lane * 16;
+        }
+    };
+    // this producer's chunks among the first `stages` of the sequence, from chunk number `done` on
+    int met = 0;
+    auto early = [&](const Piece& q, int done, auto form) {
+        typedef decltype(form) F;
+        const int depth = depth_of(q);
+        Feed<CAP> f;
+        weights_of(q, f);
+        for (int c = 0; c * F::kChunk < depth && met < start.stages; ++c, ++met)
+            if (met >= done && (met & (kProducers - 1)) == producer)
+                copy_weights<F>(start.base + met * start.stage_bytes, f, c * F::kChunk, min(F::kChunk, depth - c * F::kChunk), lane);
+        return met < start.stages;
+    };
+    auto early_pieces = [&](bool shared_only, int done) {
+        met = 0;
+        for (int i = 0; i < (shared_only ? 1 : slice.pieces); ++i)
+            if (!for_experts(p, r, slice.row(i), slice.row(i + 1) - slice.row(i), shared_only, [&](const Piece& q) {
+                    return W8 && q.expert >= 0 ? early(q, done, Form<W8, false>()) : early(q, done, Form<false, false>());
+                }))
+                break;
+        return met;
+    };
+    const int done = early_pieces(true, 0);
+    if (!mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) {
+        wait_copies();
+        return;
+    }
+    if (done < start.stages) early_pieces(false, done);
+    wait_previous_kernel();
+    Ring ring = start;
+    int turn = producer;
+    auto rest = [&](const Piece& q, auto form) {
+        typedef decltype(form) F;
+        const int depth = depth_of(q), n = F::chunks(depth);
+        Feed<CAP> f;
+        weights_of(q, f);
+        tokens_of(q, f);
+        int c = turn;
+        for (; c < n && ring.round == 0 && ring.at + c < ring.stages; c += kProducers) {   // the weights are on their way
+            copy_tokens<F>(ring.base + (ring.at + c) * ring.stage_bytes, f, c * F::kChunk, min(F::kChunk, depth - c * F::kChunk), lane);
+            arrive_when_copied(ring.full + 8 * (ring.at + c));
+        }
+        const bool ok = produce<F>(ring, &bars.abort_flag, p.status, f, c, depth, lane);
+        turn = (turn - n) & (kProducers - 1);
+        ring.next_piece(n);
+        return ok;
+    };
+    for (int i = 0; i < slice.pieces; ++i)
+        if (!for_experts(p, r, slice.row(i), slice.row(i + 1) - slice.row(i), false, [&](const Piece& q) {
+                return W8 && q.expert >= 0 ? rest(q, Form<W8, false>()) : rest(q, Form<false, false>());
+            }))
+            break;
+    wait_copies();
 }
 
 template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) moe_down_kernel(const Decode p) {
+__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages];
-    __shared__ int abort_flag;
+    __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int first = static_cast<int>(static_cast<long long>(p.hidden_size) * blockIdx.x / gridDim.x);
-    const int end = static_cast<int>(static_cast<long long>(p.hidden_size) * (blockIdx.x + 1) / gridDim.x);
-    const int cols = end - first;
-    Block b = set_up<NT>(p, smem, bars, &abort_flag, p.tokens * cols, true);
-    for (int i = threadIdx.x; i < p.tokens * cols; i += kThreads) b.sums[i] = 0.0f;
-    find_experts<true>(p, b.routing);
-    Ring ring = b.ring;
+    const Slice slice(p);
+    Ring ring = set_up_ring(bars, smem, p.stage_bytes, p.stages, kConsumerThreads);
+    Deposit sums;
+    sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
+    float* out = sums.scratch + deposit_floats<NT>();   // [token][row of the piece]
+    const int values = p.tokens * kRows;
+    const Routing r = carve_routing(reinterpret_cast<uint8_t*>(out + values), p.experts, p.tokens * p.topk);
     if (warp >= kConsumers) {
-        const int producer = warp - kConsumers;
-        // Until the gate / up kernel is done the stages of an empty ring get their weights only; the hidden rows follow.
-        bool ok = true;
-        int early = 0;   // stages that have their weights
-        auto feed = [&](const Piece& q, Feed<NT>& f) {
-            const bool shared = q.expert < 0;
-            const int depth = shared ? p.shared_intermediate : p.intermediate;
-            const long long row_bytes = depth * (W8 && !shared ? 1 : 2);
-            const uint8_t* w = shared ? reinterpret_cast<const uint8_t*>(p.shared_down) : p.down;
-            const bf16* h = shared ? p.hidden_shared : p.hidden;
-            w += ((shared ? 0 : static_cast<long long>(q.expert) * p.hidden_size) + q.row) * row_bytes + lane * 16;
-#pragma unroll
-            for (int j = 0; j < Feed<NT>::kWeights; ++j) {
-                const int i = producer + j * kProducers;
-                f.weight[j] = i < q.count ? w + i * row_bytes : nullptr;
-            }
-#pragma unroll
-            for (int j = 0; j < Feed<NT>::kTokens; ++j) {
-                const int i = producer + j * kProducers;
-                f.token[j] = nullptr;
-                if (i < q.tokens) {
-                    const long long row = shared ? q.from + i : b.routing.list[q.from + i];
-                    f.token[j] = reinterpret_cast<const uint8_t*>(h + row * depth) + lane * 16;
+        produce_down<W8, NT>(p, r, slice, ring, bars, warp - kConsumers, lane);
+        return;
+    }
+    find_experts(p, r);
+    mbar_arrive(smem_u32(&bars.routed));
+    int turn = warp;
+    for (int i = 0; i < slice.pieces; ++i) {
+        for (int k = threadIdx.x; k < values; k += kConsumerThreads) out[k] = 0.0f;
+        consumer_barrier();
+        const int row0 = slice.row(i), count = slice.row(i + 1) - row0;
+        for_experts(p, r, row0, count, false, [&](const Piece& q) {
+            const bool shared = q.expert < 0, w8 = W8 && !shared;
+            const int depth = shared ? p.shared_intermediate : p.intermediate, tiles = (q.tokens + 7) >> 3;
+            const int n = w8 ? Form<W8, false>::chunks(depth) : Form<false, false>::chunks(depth), slots = min(n, kConsumers);
+            const int slot = turn;
+            if (slot < n) {
+                float acc[NT][4];
+                clear(acc);
+                Scales<false, NT> s;
+                if (w8) {
+                    const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
+                    const int lo = min(q.row + (lane >> 2), p.hidden_size - 1), hi = min(lo + 8, p.hidden_size - 1);
+                    const long long at = static_cast<long long>(q.expert) * row_blocks;
+                    s.lo = p.down_scales + (at + lo / 128) * blocks;
+                    s.hi = p.down_scales + (at + hi / 128) * blocks;
+                    s.row_block = 1;
+                    for (int c = slot; c < n; c += kConsumers)
+                        consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
+                } else {
+                    for (int c = slot; c < n; c += kConsumers)
+                        consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
+                }
+                if (deposit<NT>(sums, bars, p.status, acc, slot, slots, tiles, lane)) {
+                    wait_turn(sums, bars, p.status);
+                    for (int k = lane; k < kRows * q.tokens; k += 32) {   // a token is listed once
+                        const int row = k & (kRows - 1), c = k / kRows;
+                        float* at = out + (shared ? q.from + c : r.token[q.from + c]) * kRows + row;
+                        *at = fmaf(shared ? 1.0f : r.weights[q.from + c], sum_of<NT>(sums, slots, row, c), *at);
+                    }
+                    end_turn(sums, bars, lane);
+                    release(sums, bars, lane);
                 }
             }
-            return depth;
-        };
-        auto run_early = [&](const Feed<NT>& f, int depth, auto form) {
-            typedef decltype(form) F;
-            for (int k0 = 0; k0 < depth && early < ring.stages; k0 += F::kChunk, ++early)
-                copy_weights<F, NT>(ring.base + early * ring.stage_bytes, f, k0, min(F::kChunk, depth - k0), producer, lane);
-        };
-        for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
-            Feed<NT> f;
-            const int depth = feed(q, f);
-            if (W8 && q.expert >= 0) run_early(f, depth, Form<W8, false>());
-            else run_early(f, depth, Form<false, false>());
-            return early < ring.stages;
-        });
-        wait_previous_kernel();
-        auto run = [&](const Feed<NT>& f, int depth, auto form) {
-            typedef decltype(form) F;
-            int k0 = 0;
-            for (; k0 < depth && early > 0; k0 += F::kChunk, --early) {
-                copy_tokens<F, NT>(ring.base + ring.stage * ring.stage_bytes, f, k0, min(F::kChunk, depth - k0), producer, lane);
-                arrive_when_copied(ring.full + 8 * ring.stage);
-                ring.advance();
-            }
-            ok = produce<F, NT>(ring, b.abort_flag, p.status, f, k0, depth, producer, lane);
-        };
-        for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
-            Feed<NT> f;
-            const int depth = feed(q, f);
-            if (W8 && q.expert >= 0) run(f, depth, Form<W8, false>());
-            else run(f, depth, Form<false, false>());
-            return ok;
-        });
-        wait_copies();
-    } else {
-        for_down_pieces(p, b.routing, first, end, [&](const Piece& q) {
-            float acc[2][NT][4];
-            if (W8 && q.expert >= 0) consume_down<W8, NT>(ring, b, p, q, warp, lane, acc);
-            else consume_down<false, NT>(ring, b, p, q, warp, lane, acc);
-            store_sums<NT>(b.scratch, acc, (q.count + 15) / 16, (q.tokens + 7) / 8, warp, lane);
-            consumer_barrier();
-            for (int i = threadIdx.x; i < 32 * q.tokens; i += kConsumerThreads) {
-                const int row = i & 31, c = i >> 5;
-                if (row >= q.count) continue;
-                int token = q.from + c;
-                float w = 1.0f;
-                if (q.expert >= 0) {
-                    w = b.routing.weights[token];
-                    token = b.routing.list[token] / p.topk;
-                }
-                float* sum = b.sums + token * cols + q.row - first + row;   // one thread per (token, column): a token is listed once
-                *sum = fmaf(w, sum_of<NT>(b.scratch, row, c), *sum);
-            }
-            consumer_barrier();
+            ++sums.piece;
+            ring.next_piece(n);
+            turn = (turn - n) & (kConsumers - 1);
             return true;
         });
+        consumer_barrier();
         wait_previous_kernel();   // its word on how it went
         const bool bad = p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0;
-        for (int i = threadIdx.x; i < p.tokens * cols; i += kConsumerThreads) {
-            const int token = i / cols;
-            p.out[static_cast<long long>(token) * p.hidden_size + first + i - token * cols] =
-                __float2bfloat16(bad ? __uint_as_float(0x7FC00000u) : b.sums[i]);
+        for (int k = threadIdx.x; k < values; k += kConsumerThreads) {
+            const int row = k & (kRows - 1), token = k / kRows;
+            if (row < count)
+                p.out[static_cast<long long>(token) * p.hidden_size + row0 + row] = __float2bfloat16(bad ? __uint_as_float(0x7FC00000u) : out[k]);
         }
+        consumer_barrier();
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kStatic = 1024 + 256;   // reserved per block + barriers
+constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kStatic = 1024 + 512;   // reserved per block + barriers
 
-// Ring of a kernel whose other shared memory is `other` bytes: as many stages as leave room for the second kernel's block next to
-// it on the SM, or, where that would be fewer than three, as many as fit at all.  0: does not fit.
+// Ring of a kernel whose other shared memory is `other` bytes: 8 or 16 stages, so that every consumer keeps its stages, with room for
+// the second kernel's block next to it on the SM, or else 8 that take what they need.  0: does not fit.
 int ring_stages(int stage, int other) {
-    int n = (kSmemPerSm / 2 - kStatic - other) / stage;
-    if (n < 3) n = (kSmemPerBlock - kStatic - other) / stage;
-    return n < 2 ? 0 : n > kMaxStages ? kMaxStages : n;
+    const int half = (kSmemPerSm / 2 - kStatic - other) / stage;
+    if (half >= kConsumers) return half >= 2 * kConsumers ? 2 * kConsumers : kConsumers;
+    return (kSmemPerBlock - kStatic - other) / stage >= kConsumers ? kConsumers : 0;
 }
 
-template <typename Kernel>
-int launch_decode(Kernel kernel, const char* name, const Decode& p, int smem, bool early, cudaStream_t stream) {
-    MOK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+// Tokens of a stage.  An expert that more tokens chose is read more than once (from L2 after the first time), so few suffice where
+// experts see few tokens, and eight stages of them fit an SM twice; with more tokens the second block's room goes to the stages.
+int token_cap(int tokens, bool w8) {
+    if (w8) return tokens <= 4 ? tokens : 8;
+    return tokens <= 6 ? tokens : tokens <= 32 ? 6 : 16;
+}
+
+template <bool W8, int NT, typename Kernel>
+int launch_decode(Kernel kernel, const char* name, int (&ready)[16], Decode p, int other, bool early, cudaStream_t stream) {
+    int dev = 0;
+    MOK_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 16) return MOK_ERR_UNSUPPORTED;
+    if (ready[dev] == 0) {
+        MOK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock - kStatic));
+        ready[dev] = 1;
+    }
+    // the shared expert is bf16 in either case; the rows of a stage's last n tile that no token has are read as what follows in memory
+    const int a = Form<false, false>::stage_bytes(p.token_cap), b = W8 ? Form<true, false>::stage_bytes(p.token_cap) : 0;
+    p.stage_bytes = a > b ? a : b;
+    p.stages = ring_stages(p.stage_bytes, other);
+    if (p.stages == 0) return MOK_ERR_TOO_LARGE;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sm_count());
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = other + p.stages * p.stage_bytes;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = early ? 1 : 0;
@@ -449,20 +506,12 @@ int launch_decode(Kernel kernel, const char* name, const Decode& p, int smem, bo
 }
 
 template <bool W8, int NT>
-int run_decode(Decode p, cudaStream_t stream) {
-    p.token_cap = 8 * NT;
-    p.stage_bytes = Form<false, false>::stage_bytes(p.token_cap);
-    if (W8) p.stage_bytes = p.stage_bytes > Form<true, false>::stage_bytes(p.token_cap) ? p.stage_bytes : Form<true, false>::stage_bytes(p.token_cap);
-    const int routes = p.tokens * p.topk, scratch = scratch_floats<NT>() * 4;
-    const int cols = (p.hidden_size + sm_count() - 1) / sm_count();
-    const int up = scratch + routing_bytes(p.experts, routes, false);
-    const int down = scratch + (p.tokens * cols + 3) / 4 * 16 + routing_bytes(p.experts, routes, true);
-    const int up_stages = ring_stages(p.stage_bytes, up), down_stages = ring_stages(p.stage_bytes, down);
-    if (up_stages == 0 || down_stages == 0) return MOK_ERR_TOO_LARGE;
-    p.stages = up_stages;
-    MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", p, up + up_stages * p.stage_bytes, false, stream));
-    p.stages = down_stages;
-    return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", p, down + down_stages * p.stage_bytes, true, stream);
+int run_decode(const Decode& p, cudaStream_t stream) {
+    static int gate_up_ready[16] = {0}, down_ready[16] = {0};
+    const int routing = routing_bytes(p.experts, p.tokens * p.topk);
+    MOK_TRY((launch_decode<W8, NT>(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, deposit_floats<NT>() * 4 + routing, false, stream)));
+    return launch_decode<W8, NT>(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, p, (deposit_floats<NT>() + p.tokens * kRows) * 4 + routing, true,
+                                 stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -521,12 +570,7 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.clamp = has_limit;
     p.limit = limit;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (w8) {
-        if (num_tokens <= 8) return run_decode<true, 1>(p, s);
-        if (num_tokens <= 16) return run_decode<true, 2>(p, s);
-        return run_decode<true, 4>(p, s);
-    }
-    if (num_tokens <= 8) return run_decode<false, 1>(p, s);
-    if (num_tokens <= 16) return run_decode<false, 2>(p, s);
-    return run_decode<false, 4>(p, s);
+    p.token_cap = token_cap(num_tokens, w8);
+    if (w8) return run_decode<true, 1>(p, s);
+    return p.token_cap <= 8 ? run_decode<false, 1>(p, s) : run_decode<false, 2>(p, s);
 }

@@ -1,18 +1,26 @@
 // Products of weight rows with a few tokens, for kernels that are bound by reading the weights once: out[row, token] = sum over k
 // of W[row, k] * x[token, k].
 //
-// A block has four producer warps and eight consumer warps.  The producers copy pieces of up to 32 weight rows and the rows of up
-// to 32 tokens, kChunk elements of k at a time, into a ring of stages with cp.async (a warp's 32 x 16 bytes are one row of a chunk:
-// any row count, stride and gather), and run ahead of the consumers as far as the ring reaches; about 100 KB in flight per SM is
-// what HBM needs.  Bulk copies, one per row, were measured first: an SM issues about one in 60 clocks, so 512-byte rows came in at
-// 1.4 - 1.8 TB/s and 1024-byte rows at 2.2 - 3.4 TB/s.  The consumers split k: a warp takes every eighth slice of a chunk, multiplies it with mma.sync (weights on the M
-// side, tokens on the N side of 8) and keeps its own sums, which the eight warps add in a fixed order when a piece is done.
-// tcgen05 would need 128 rows a tile, which leaves SMs idle at these sizes; the tensor work here is a few percent of the time.
+// A block has four producer warps and eight consumer warps around a ring of stages.  A stage is a chunk of a piece: 16 weight rows
+// and the rows of the tokens concerned, kChunk elements of k.  One producer warp fills it with cp.async (32 x 16 bytes lie in one
+// row: any row count, stride and gather), one consumer warp multiplies it with mma.sync (weights on the M side, tokens on the N
+// side of 8); chunks go round the producers and round the consumers in turn.  Producers run ahead as far as the ring reaches: about
+// 64 KB of weights in flight per block is what HBM needs.  tcgen05 would need 128 rows a tile, which leaves SMs idle at these
+// sizes; the tensor work here is a few percent of the time.
 //
-// The order of k within a slice is free as long as both operands use the same one: lane (g, t) of an mma takes elements 8 t .. 8 t
-// + 7 of rows g and g + 8, one 16-byte (8-byte in e4m3) shared-memory load per row, for two mma of K = 16.  Row pitches of 64 (32)
-// bytes modulo 128 make these loads free of bank conflicts.
+// The barriers of a stage tell rounds apart by one bit, so nobody may be two rounds ahead of a barrier: the number of stages is a
+// multiple of eight, so that a stage has one producer and one consumer, which have seen every round of it.
+//
+// What did not do: bulk copies, one per row (an SM issues one in about 60 clocks: 1.4 - 1.8 TB/s with rows of 512 bytes, 2.2 - 3.4
+// with 1024); every consumer taking an eighth of every chunk (all eight pay the waits and addresses of each chunk, 350 instructions
+// a warp for 21 KB of weights: 2.1 - 3.7 TB/s with experts of 768 rows).
+//
+// The order of k within a slice of 32 is free as long as both operands use the same one: lane (g, t) of an mma takes elements 8 t ..
+// 8 t + 7 of rows g and g + 8, one 16-byte (8-byte in e4m3) shared-memory load per row, for two mma of K = 16.  Row pitches of 64
+// (32) bytes modulo 128 make these loads free of bank conflicts.
 #pragma once
+
+#include <cuda_fp16.h>
 
 #include "mok_common.cuh"
 
@@ -22,21 +30,21 @@ namespace stream {
 constexpr int kConsumers = 8;                       // warps
 constexpr int kConsumerThreads = kConsumers * 32;
 constexpr int kProducers = 4;
-constexpr int kProducerThreads = kProducers * 32;
-constexpr int kThreads = kConsumerThreads + kProducerThreads;
-constexpr int kPieceRows = 32;                      // weight rows of a piece: two m16 tiles
-constexpr int kMaxStages = 8;
+constexpr int kThreads = kConsumerThreads + kProducers * 32;
+constexpr int kRows = 16;                           // weight rows of a piece
+constexpr int kMaxStages = 16;
+constexpr int kDeposits = 2;
 
 // W8 / X8: weights / tokens in e4m3 instead of bf16.
 template <bool W8, bool X8>
 struct Form {
     static constexpr int kChunk = W8 ? 512 : 256;               // elements of k per stage
-    static constexpr int kRowBytes = kChunk * (W8 ? 1 : 2);     // 512
+    static constexpr int kRowBytes = kChunk * (W8 ? 1 : 2);     // 512: one copy of 16 bytes per lane
     static constexpr int kRowPitch = kRowBytes + (W8 ? 32 : 64);
     static constexpr int kTokenBytes = kChunk * (X8 ? 1 : 2);
     static constexpr int kTokenPitch = kTokenBytes + (X8 ? 32 : 64);
-    static constexpr int kSlices = kChunk / 32 / kConsumers;    // slices of 32 per warp and chunk
-    static constexpr int stage_bytes(int tokens) { return kPieceRows * kRowPitch + tokens * kTokenPitch; }
+    static constexpr int stage_bytes(int tokens) { return kRows * kRowPitch + tokens * kTokenPitch; }
+    __device__ static __forceinline__ int chunks(int k_total) { return (k_total + kChunk - 1) / kChunk; }
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -55,72 +63,116 @@ __device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, %
 __device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Ring state that producer and consumers walk alike.
+struct Bars {
+    uint64_t full[kMaxStages], empty[kMaxStages], routed;
+    int count[kDeposits], done[kDeposits], finished;   // deposits of the piece so far; pieces that left the deposit; pieces in order
+    int abort_flag;
+};
+
+// The ring, and the place of a piece in the sequence of chunks that producers and consumers walk alike: its chunk 0 lies in stage
+// `at` of round `round`.
 struct Ring {
     uint32_t base, full, empty;   // shared addresses: stages, barriers
     int stage_bytes, stages;
-    int stage = 0;
-    uint32_t phase = 0;
-    __device__ __forceinline__ void advance() {
-        if (++stage == stages) {
-            stage = 0;
-            phase ^= 1u;
+    int at = 0, round = 0;
+    __device__ __forceinline__ void next_piece(int chunks) {
+        at += chunks;
+        while (at >= stages) {
+            at -= stages;
+            ++round;
         }
     }
-    __device__ __forceinline__ void init() const {   // one thread
-        for (int s = 0; s < stages; ++s) {
-            mbar_init(full + 8 * s, kProducerThreads);
-            mbar_init(empty + 8 * s, kConsumers);
+    // Stage and parity of chunk c.
+    __device__ __forceinline__ int stage(int c, uint32_t& parity) const {
+        int s = at + c, r = round;
+        while (s >= stages) {
+            s -= stages;
+            ++r;
         }
-        mbar_fence_init();
+        parity = r & 1;
+        return s;
     }
 };
 
-// What a producer warp copies of a piece: every kProducers-th weight row and token row, as this lane's address in the row at k = 0
-// (nullptr: no such row).  Found once per piece, so that a chunk costs its producers little more than the copies themselves: with
-// addresses worked out chunk by chunk they were the bottleneck (1500 clocks a chunk, 2.2 TB/s).
-template <int NT>
+__device__ __forceinline__ Ring set_up_ring(Bars& bars, const uint8_t* smem, int stage_bytes, int stages, int routed_arrivals) {
+    Ring r;
+    r.base = smem_u32(smem);
+    r.full = smem_u32(bars.full);
+    r.empty = smem_u32(bars.empty);
+    r.stage_bytes = stage_bytes;
+    r.stages = stages;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(r.full + 8 * s, 32);
+            mbar_init(r.empty + 8 * s, 1);
+        }
+        for (int d = 0; d < kDeposits; ++d) {
+            bars.count[d] = bars.done[d] = 0;
+        }
+        mbar_init(smem_u32(&bars.routed), routed_arrivals);
+        bars.finished = 0;
+        bars.abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    return r;
+}
+
+// ---- producer -----------------------------------------------------------------------------------------------------
+// Rows of a piece as a producer copies them, this lane's 16 bytes of each at k = 0.  Weights: rows 0 .. 7 from low and rows 8 .. 15
+// from high, row_bytes apart, `rows_low` and `rows_high` of them (the others stay as they are and are not used).  Found once per
+// piece: with addresses worked out chunk by chunk the producers were the bottleneck (1500 clocks a chunk, 2.2 TB/s).
+template <int CAP>
 struct Feed {
-    static constexpr int kWeights = kPieceRows / kProducers, kTokens = 8 * NT / kProducers;
-    const uint8_t *weight[kWeights], *token[kTokens];
+    const uint8_t *low, *high, *token[CAP];
+    long long row_bytes;
+    int rows_low, rows_high;
 };
-template <typename F, int NT>
-__device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<NT>& f, int k0, int len, int producer, int lane) {
+template <typename F, int CAP>
+__device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kRowBytes / F::kChunk;
-    static_assert(F::kRowBytes == 512, "one copy of 16 bytes per lane");
+    static_assert(F::kRowBytes == 512, "");
+    if (lane * 16 >= len * kBytes) return;
     const long long at = static_cast<long long>(k0) * kBytes;
-    const uint32_t dst = stage + producer * F::kRowPitch + lane * 16;
-    if (lane * 16 < len * kBytes) {
+    const uint8_t *low = f.low + at, *high = f.high + at;
+    const uint32_t dst = stage + lane * 16;
 #pragma unroll
-        for (int j = 0; j < Feed<NT>::kWeights; ++j)
-            if (f.weight[j] != nullptr) copy16(dst + j * kProducers * F::kRowPitch, f.weight[j] + at);
+    for (int i = 0; i < 8; ++i) {
+        if (i < f.rows_low) copy16(dst + i * F::kRowPitch, low);
+        if (i < f.rows_high) copy16(dst + (8 + i) * F::kRowPitch, high);
+        low += f.row_bytes;
+        high += f.row_bytes;
     }
 }
-template <typename F, int NT>
-__device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<NT>& f, int k0, int len, int producer, int lane) {
+template <typename F, int CAP>
+__device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kTokenBytes / F::kChunk;
     const long long at = static_cast<long long>(k0) * kBytes;
-    const uint32_t dst = stage + kPieceRows * F::kRowPitch + producer * F::kTokenPitch + lane * 16;
+    const uint32_t dst = stage + kRows * F::kRowPitch + lane * 16;
 #pragma unroll
-    for (int half = 0; half < F::kTokenBytes / 512; ++half)
-        if (half * 512 + lane * 16 < len * kBytes) {
+    for (int part = 0; part < F::kTokenBytes; part += 512)
+        if (part + lane * 16 < len * kBytes) {
 #pragma unroll
-            for (int j = 0; j < Feed<NT>::kTokens; ++j)
-                if (f.token[j] != nullptr) copy16(dst + j * kProducers * F::kTokenPitch + half * 512, f.token[j] + at + half * 512);
+            for (int j = 0; j < CAP; ++j) {
+                if (f.token[j] == nullptr) break;   // tokens come without gaps
+                copy16(dst + j * F::kTokenPitch + part, f.token[j] + at + part);
+            }
         }
 }
-// The producers' side of a piece from k0 on, chunk by chunk.  False: a wait ran out.
-template <typename F, int NT>
-__device__ __forceinline__ bool produce(Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed<NT>& f, int k0, int k_total, int producer,
+// A producer's chunks of a piece, from chunk `first` on: those whose number in the whole sequence is `producer` modulo kProducers.
+// False: a wait ran out.
+template <typename F, int CAP>
+__device__ __forceinline__ bool produce(const Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed<CAP>& f, int first, int k_total,
                                         int lane) {
-    for (; k0 < k_total; k0 += F::kChunk) {
-        if (!mbar_wait(ring.empty + 8 * ring.stage, ring.phase ^ 1u, abort_flag, status)) return false;
-        const int len = min(F::kChunk, k_total - k0);
-        const uint32_t stage = ring.base + ring.stage * ring.stage_bytes;
-        copy_weights<F, NT>(stage, f, k0, len, producer, lane);
-        copy_tokens<F, NT>(stage, f, k0, len, producer, lane);
-        arrive_when_copied(ring.full + 8 * ring.stage);
-        ring.advance();
+    for (int c = first; c * F::kChunk < k_total; c += kProducers) {
+        uint32_t parity;
+        const int s = ring.stage(c, parity);
+        if (!mbar_wait(ring.empty + 8 * s, parity ^ 1u, abort_flag, status)) return false;
+        const int k0 = c * F::kChunk, len = min(F::kChunk, k_total - k0);
+        const uint32_t stage = ring.base + s * ring.stage_bytes;
+        copy_weights<F>(stage, f, k0, len, lane);
+        copy_tokens<F>(stage, f, k0, len, lane);
+        arrive_when_copied(ring.full + 8 * s);
     }
     return true;
 }
@@ -141,17 +193,13 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_codes) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two_codes)));
     return h;
 }
-// Two of a word's four e4m3 codes as bf16: sign and the seven other bits moved to where bf16 has them read as the value times
-// 2^-120 (subnormal codes land among bf16's subnormal numbers), and one exact multiplication puts that right.  A NaN code would
-// read as +-480: nan_codes finds those.
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t word, uint32_t selector) {
-    const uint32_t p = __byte_perm(word, 0, selector);   // code << 8 in each half
-    const uint32_t v = ((p & 0x7F007F00u) >> 4) | (p & 0x80008000u);
-    const uint32_t two_to_120 = 0x7B807B80u;
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&two_to_120));
-    return *reinterpret_cast<const uint32_t*>(&r);
+// Two e4m3 codes as bf16 (exact, NaN stays NaN) by way of f16 and fp32.  Moving the bits and multiplying by 2^120 takes one
+// instruction more per pair, and a search for NaN codes, which that reads as 480.
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t two_codes) {
+    const uint32_t h = e4m3x2_to_f16x2(two_codes);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return pack_bf16x2(f.x, f.y);
 }
-__device__ __forceinline__ uint32_t nan_codes(uint32_t word) { return ((word & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 // The first `count` (may be <= 0) of eight codes, the others zero.
 __device__ __forceinline__ uint2 keep_codes(uint2 v, int count) {
@@ -160,190 +208,185 @@ __device__ __forceinline__ uint2 keep_codes(uint2 v, int count) {
     return v;
 }
 
-// Adds a warp's share of one stage to `acc`; `k_len` elements of the chunk are valid (a multiple of 32 unless X8).
-// nan: per m tile the NaN codes met in rows g (bit 7 of each byte) and, in [1], rows g + 8.
+template <int NT>
+__device__ __forceinline__ void clear(float (&acc)[NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+}
+
+// acc += 32 elements of k from element `k` of a stage on (of this lane: k + 8 t .. k + 8 t + 7).  `left`: valid elements from k on
+// (X8; the others hold multiples of 32).  `tiles`: n tiles in use.
 template <bool W8, bool X8, int NT>
-__device__ __forceinline__ void multiply(const uint8_t* stage, int k_len, int m_tiles, int n_tiles, int warp, int lane, float (&acc)[2][NT][4],
-                                         uint32_t (&nan)[2][2]) {
+__device__ __forceinline__ void multiply_slice(const uint8_t* weights, const uint8_t* tokens, int k, int left, int tiles, int t, float (&acc)[NT][4]) {
     typedef Form<W8, X8> F;
-    const int g = lane >> 2, t = lane & 3;
-    const uint8_t* weights = stage + g * F::kRowPitch;
-    const uint8_t* tokens = stage + kPieceRows * F::kRowPitch + g * F::kTokenPitch;
-#pragma unroll
-    for (int s = 0; s < F::kSlices; ++s) {
-        const int k = (warp * F::kSlices + s) * 32 + 8 * t;   // of this lane
-        if ((warp * F::kSlices + s) * 32 >= k_len) break;
-        uint32_t b[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n < n_tiles) {
-                if (X8) {
-                    const uint2 v = keep_codes(*reinterpret_cast<const uint2*>(tokens + n * 8 * F::kTokenPitch + k), k_len - k);
-                    b[n][0] = e4m3x2_to_f16x2(v.x); b[n][1] = e4m3x2_to_f16x2(v.x >> 16);
-                    b[n][2] = e4m3x2_to_f16x2(v.y); b[n][3] = e4m3x2_to_f16x2(v.y >> 16);
-                } else {
-                    const uint4 v = *reinterpret_cast<const uint4*>(tokens + n * 8 * F::kTokenPitch + k * 2);
-                    b[n][0] = v.x; b[n][1] = v.y; b[n][2] = v.z; b[n][3] = v.w;
-                }
+    uint32_t lo[4], hi[4];
+    if (W8) {
+        uint2 l = *reinterpret_cast<const uint2*>(weights + k);
+        uint2 h = *reinterpret_cast<const uint2*>(weights + 8 * F::kRowPitch + k);
+        if (X8) {
+            if (left < 32) {
+                l = keep_codes(l, left - 8 * t);
+                h = keep_codes(h, left - 8 * t);
             }
+            lo[0] = e4m3x2_to_f16x2(l.x); lo[1] = e4m3x2_to_f16x2(l.x >> 16); lo[2] = e4m3x2_to_f16x2(l.y); lo[3] = e4m3x2_to_f16x2(l.y >> 16);
+            hi[0] = e4m3x2_to_f16x2(h.x); hi[1] = e4m3x2_to_f16x2(h.x >> 16); hi[2] = e4m3x2_to_f16x2(h.y); hi[3] = e4m3x2_to_f16x2(h.y >> 16);
+        } else {
+            lo[0] = e4m3x2_to_bf16x2(l.x); lo[1] = e4m3x2_to_bf16x2(l.x >> 16); lo[2] = e4m3x2_to_bf16x2(l.y); lo[3] = e4m3x2_to_bf16x2(l.y >> 16);
+            hi[0] = e4m3x2_to_bf16x2(h.x); hi[1] = e4m3x2_to_bf16x2(h.x >> 16); hi[2] = e4m3x2_to_bf16x2(h.y); hi[3] = e4m3x2_to_bf16x2(h.y >> 16);
         }
+    } else {
+        const uint4 l = *reinterpret_cast<const uint4*>(weights + k * 2);
+        const uint4 h = *reinterpret_cast<const uint4*>(weights + 8 * F::kRowPitch + k * 2);
+        lo[0] = l.x; lo[1] = l.y; lo[2] = l.z; lo[3] = l.w;
+        hi[0] = h.x; hi[1] = h.y; hi[2] = h.z; hi[3] = h.w;
+    }
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            if (m >= m_tiles) break;
-            uint32_t lo[4], hi[4];
-            if (W8) {
-                uint2 l = *reinterpret_cast<const uint2*>(weights + (m * 16) * F::kRowPitch + k);
-                uint2 h = *reinterpret_cast<const uint2*>(weights + (m * 16 + 8) * F::kRowPitch + k);
-                if (X8) {
-                    l = keep_codes(l, k_len - k);
-                    h = keep_codes(h, k_len - k);
-                    lo[0] = e4m3x2_to_f16x2(l.x); lo[1] = e4m3x2_to_f16x2(l.x >> 16);
-                    lo[2] = e4m3x2_to_f16x2(l.y); lo[3] = e4m3x2_to_f16x2(l.y >> 16);
-                    hi[0] = e4m3x2_to_f16x2(h.x); hi[1] = e4m3x2_to_f16x2(h.x >> 16);
-                    hi[2] = e4m3x2_to_f16x2(h.y); hi[3] = e4m3x2_to_f16x2(h.y >> 16);
-                } else {
-                    lo[0] = e4m3x2_to_bf16x2(l.x, 0x1404); lo[1] = e4m3x2_to_bf16x2(l.x, 0x3424);
-                    lo[2] = e4m3x2_to_bf16x2(l.y, 0x1404); lo[3] = e4m3x2_to_bf16x2(l.y, 0x3424);
-                    hi[0] = e4m3x2_to_bf16x2(h.x, 0x1404); hi[1] = e4m3x2_to_bf16x2(h.x, 0x3424);
-                    hi[2] = e4m3x2_to_bf16x2(h.y, 0x1404); hi[3] = e4m3x2_to_bf16x2(h.y, 0x3424);
-                    nan[m][0] |= nan_codes(l.x) | nan_codes(l.y);
-                    nan[m][1] |= nan_codes(h.x) | nan_codes(h.y);
-                }
-            } else {
-                const uint4 l = *reinterpret_cast<const uint4*>(weights + (m * 16) * F::kRowPitch + k * 2);
-                const uint4 h = *reinterpret_cast<const uint4*>(weights + (m * 16 + 8) * F::kRowPitch + k * 2);
-                lo[0] = l.x; lo[1] = l.y; lo[2] = l.z; lo[3] = l.w;
-                hi[0] = h.x; hi[1] = h.y; hi[2] = h.z; hi[3] = h.w;
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (n < n_tiles) {
-                    if (X8) {
-                        mma_f16(acc[m][n], lo[0], hi[0], lo[1], hi[1], b[n][0], b[n][1]);
-                        mma_f16(acc[m][n], lo[2], hi[2], lo[3], hi[3], b[n][2], b[n][3]);
-                    } else {
-                        mma_bf16(acc[m][n], lo[0], hi[0], lo[1], hi[1], b[n][0], b[n][1]);
-                        mma_bf16(acc[m][n], lo[2], hi[2], lo[3], hi[3], b[n][2], b[n][3]);
-                    }
-                }
-            }
+    for (int n = 0; n < NT; ++n) {
+        if (n >= tiles) break;
+        uint32_t b[4];
+        if (X8) {
+            uint2 v = *reinterpret_cast<const uint2*>(tokens + n * 8 * F::kTokenPitch + k);
+            if (left < 32) v = keep_codes(v, left - 8 * t);
+            b[0] = e4m3x2_to_f16x2(v.x); b[1] = e4m3x2_to_f16x2(v.x >> 16); b[2] = e4m3x2_to_f16x2(v.y); b[3] = e4m3x2_to_f16x2(v.y >> 16);
+            mma_f16(acc[n], lo[0], hi[0], lo[1], hi[1], b[0], b[1]);
+            mma_f16(acc[n], lo[2], hi[2], lo[3], hi[3], b[2], b[3]);
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(tokens + n * 8 * F::kTokenPitch + k * 2);
+            mma_bf16(acc[n], lo[0], hi[0], lo[1], hi[1], v.x, v.y);
+            mma_bf16(acc[n], lo[2], hi[2], lo[3], hi[3], v.z, v.w);
         }
     }
 }
 
-// Scales of a lane's rows (g and g + 8 of each m tile) and, X8, of its tokens (2 t and 2 t + 1 of each n tile), one per 128 of k.
-template <bool W8, bool X8, int NT>
+// Scales of a lane's rows (g and g + 8) and, X8, of its tokens (2 t and 2 t + 1 of each n tile), one per 128 of k.
+template <bool X8, int NT>
 struct Scales {
-    const float *lo[2], *hi[2], *x[NT][2];
+    const float *lo, *hi, *x[X8 ? NT : 1][2];
     long long row_block, x_block;   // elements from one block of k to the next
-    struct Values {
-        float lo[2], hi[2], x[NT][2];
-    };
-    __device__ __forceinline__ void fetch(Values& v, int k, int n_tiles) const {
-        const int block = k / 128;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            v.lo[m] = __ldg(lo[m] + block * row_block);
-            v.hi[m] = __ldg(hi[m] + block * row_block);
-        }
-        if (X8) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                if (n < n_tiles) {
-                    v.x[n][0] = __ldg(x[n][0] + block * x_block);
-                    v.x[n][1] = __ldg(x[n][1] + block * x_block);
-                }
-        }
-    }
 };
 
-// A consumer warp's part of one piece: its share of the sums over k_total.  All consumers wait for the same stages; one whose wait
-// runs out goes on with what is there (every warp then meets the same barriers), and the status word tells.
+// Waits for a chunk and adds its products to acc.  A wait that runs out is reported in the status word and the warp goes on with what
+// is there, so that every warp still meets the same barriers.
 template <bool W8, bool X8, int NT>
-__device__ __forceinline__ void consume(Ring& ring, const uint8_t* stages, volatile int* abort_flag, uint32_t* status, int k_total, int m_tiles,
-                                        int n_tiles, const Scales<W8, X8, NT>& scales, int warp, int lane, float (&acc)[2][NT][4]) {
+__device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages, volatile int* abort_flag, uint32_t* status, int c, int k_total, int tiles,
+                                        const Scales<X8, NT>& scales, int lane, float (&acc)[NT][4]) {
     typedef Form<W8, X8> F;
-    uint32_t nan[2][2] = {{0, 0}, {0, 0}};
+    const int g = lane >> 2, t = lane & 3;
+    const int len = min(F::kChunk, k_total - c * F::kChunk);
+    constexpr int kBlocks = F::kChunk / 128;
+    float lo[kBlocks], hi[kBlocks];
+    if (W8) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+        for (int b = 0; b < kBlocks; ++b)
+            if (b * 128 < len) {
+                lo[b] = __ldg(scales.lo + (c * kBlocks + b) * scales.row_block);
+                hi[b] = __ldg(scales.hi + (c * kBlocks + b) * scales.row_block);
+            }
+    }
+    uint32_t parity;
+    const int s = ring.stage(c, parity);
+    mbar_wait(ring.full + 8 * s, parity, abort_flag, status);
+    const uint8_t* weights = stages + s * ring.stage_bytes + g * F::kRowPitch;
+    const uint8_t* tokens = stages + s * ring.stage_bytes + kRows * F::kRowPitch + g * F::kTokenPitch;
+    if (W8) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-    const int mine = warp * F::kSlices * 32;   // this warp's first k of a chunk; its slices lie in one block of 128
-    typename Scales<W8, X8, NT>::Values now, next;
-    if (W8) scales.fetch(now, min(mine, k_total - 1), n_tiles);
-    for (int k0 = 0; k0 < k_total; k0 += F::kChunk) {
-        if (W8 && k0 + F::kChunk < k_total) scales.fetch(next, min(k0 + F::kChunk + mine, k_total - 1), n_tiles);
-        mbar_wait(ring.full + 8 * ring.stage, ring.phase, abort_flag, status);
-        const uint8_t* stage = stages + ring.stage * ring.stage_bytes;
-        const int len = min(F::kChunk, k_total - k0);
-        if (W8) {
-            float part[2][NT][4];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
+        for (int b = 0; b < kBlocks; ++b) {
+            if (b * 128 >= len) break;
+            float part[NT][4];
+            clear(part);
+            float x[X8 ? NT : 1][2];
+            if (X8) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) part[m][n][i] = 0.0f;
-            multiply<W8, X8, NT>(stage, len, m_tiles, n_tiles, warp, lane, part, nan);
-            if (mine < len) {
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float x0 = X8 ? now.x[n][0] : 1.0f, x1 = X8 ? now.x[n][1] : 1.0f;
-                        if (m < m_tiles && n < n_tiles) {
-                            acc[m][n][0] = fmaf(part[m][n][0], X8 ? now.lo[m] * x0 : now.lo[m], acc[m][n][0]);
-                            acc[m][n][1] = fmaf(part[m][n][1], X8 ? now.lo[m] * x1 : now.lo[m], acc[m][n][1]);
-                            acc[m][n][2] = fmaf(part[m][n][2], X8 ? now.hi[m] * x0 : now.hi[m], acc[m][n][2]);
-                            acc[m][n][3] = fmaf(part[m][n][3], X8 ? now.hi[m] * x1 : now.hi[m], acc[m][n][3]);
-                        }
+                    if (n < tiles) {
+                        x[n][0] = __ldg(scales.x[n][0] + (c * kBlocks + b) * scales.x_block);
+                        x[n][1] = __ldg(scales.x[n][1] + (c * kBlocks + b) * scales.x_block);
                     }
             }
-            now = next;
-        } else {
-            multiply<W8, X8, NT>(stage, len, m_tiles, n_tiles, warp, lane, acc, nan);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ring.empty + 8 * ring.stage);
-        ring.advance();
-    }
-    if (W8 && !X8) {   // a NaN code makes its row NaN for every token; the lane that met it is one of four that hold the row
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+            for (int k = 0; k < 128; k += 32)
+                if (b * 128 + k < len) multiply_slice<W8, X8, NT>(weights, tokens, b * 128 + k + 8 * t, len - b * 128 - k, tiles, t, part);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t f = nan[m][h];
-                f |= __shfl_xor_sync(0xffffffffu, f, 1);
-                f |= __shfl_xor_sync(0xffffffffu, f, 2);
-                if (f != 0)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[m][n][2 * h] = acc[m][n][2 * h + 1] = __uint_as_float(0x7FC00000u);
+            for (int n = 0; n < NT; ++n) {
+                if (n >= tiles) break;
+                const float x0 = X8 ? x[X8 ? n : 0][0] : 1.0f, x1 = X8 ? x[X8 ? n : 0][1] : 1.0f;
+                acc[n][0] = fmaf(part[n][0], X8 ? lo[b] * x0 : lo[b], acc[n][0]);
+                acc[n][1] = fmaf(part[n][1], X8 ? lo[b] * x1 : lo[b], acc[n][1]);
+                acc[n][2] = fmaf(part[n][2], X8 ? hi[b] * x0 : hi[b], acc[n][2]);
+                acc[n][3] = fmaf(part[n][3], X8 ? hi[b] * x1 : hi[b], acc[n][3]);
             }
+        }
+    } else if (len == F::kChunk) {
+#pragma unroll
+        for (int k = 0; k < F::kChunk; k += 32) multiply_slice<W8, X8, NT>(weights, tokens, k + 8 * t, 32, tiles, t, acc);
+    } else {
+        for (int k = 0; k < len; k += 32) multiply_slice<W8, X8, NT>(weights, tokens, k + 8 * t, 32, tiles, t, acc);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ring.empty + 8 * s);
 }
 
-// A warp's sums of a piece -> shared memory [warp][m][n][4][32]; sum_of reads the value of (row, token) from all eight.
+// ---- sums of a piece over the consumers -----------------------------------------------------------------------------
+// Chunk c's sums go to slot c % 8 (whichever warp computed them), so the order of the final addition is that of k.  The warp that
+// deposits last adds the slots and goes on to what becomes of them; the others are at the next piece by then (two deposits in turn).
 template <int NT>
-constexpr int scratch_floats() { return kConsumers * 2 * NT * 128; }
+constexpr int deposit_floats() { return kDeposits * kConsumers * NT * 128; }
 
-template <int NT>
-__device__ __forceinline__ void store_sums(float* scratch, const float (&acc)[2][NT][4], int m_tiles, int n_tiles, int warp, int lane) {
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (m < m_tiles && n < n_tiles)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) scratch[((warp * 2 + m) * NT + n) * 128 + r * 32 + lane] = acc[m][n][r];
+struct Deposit {
+    float* scratch;
+    int piece = 0;      // pieces so far
+};
+// Waits, with the limit of all pipeline waits, until a counter in shared memory has a value.  Not a barrier of one bit: a warp may
+// have no part in many pieces and be far ahead.
+__device__ __forceinline__ void wait_count(int* counter, int value, Bars& bars, uint32_t* status) {
+    const long long start = clock64();
+    while (*static_cast<volatile int*>(counter) != value && !*static_cast<volatile int*>(&bars.abort_flag)) {
+        if (clock64() - start > kPipelineWaitCycles) {
+            *static_cast<volatile int*>(&bars.abort_flag) = 1;
+            if (status != nullptr) atomicOr(status, (uint32_t)MOK_STATUS_PIPELINE_TIMEOUT);
+        }
+    }
+    __threadfence_block();
+    __syncwarp();
 }
+__device__ __forceinline__ void set_count(int* counter, int value, int lane) {
+    __threadfence_block();
+    __syncwarp();
+    if (lane == 0) *static_cast<volatile int*>(counter) = value;
+}
+// True for the warp that has to finish the piece; `slots` of them were filled.  It calls release() afterwards.
 template <int NT>
-__device__ __forceinline__ float sum_of(const float* scratch, int row, int token) {
-    const float* at = scratch + ((row >> 4) * NT + (token >> 3)) * 128 + (((row >> 3) & 1) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
+__device__ __forceinline__ bool deposit(const Deposit& d, Bars& bars, uint32_t* status, const float (&acc)[NT][4], int slot, int slots, int tiles, int lane) {
+    const int which = d.piece & 1;
+    wait_count(&bars.done[which], d.piece >> 1, bars, status);
+    float* at = d.scratch + (which * kConsumers + slot) * NT * 128 + lane;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+        if (n < tiles)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) at[n * 128 + r * 32] = acc[n][r];
+    __threadfence_block();
+    __syncwarp();
+    int last = 0;
+    if (lane == 0) {
+        last = atomicAdd(&bars.count[which], 1) == slots - 1;
+        if (last) bars.count[which] = 0;
+    }
+    last = __shfl_sync(0xffffffffu, last, 0);
+    if (last) __threadfence_block();
+    return last != 0;
+}
+__device__ __forceinline__ void release(const Deposit& d, Bars& bars, int lane) { set_count(&bars.done[d.piece & 1], (d.piece >> 1) + 1, lane); }
+// Lets the finishing warps through in the order of their pieces.
+__device__ __forceinline__ void wait_turn(const Deposit& d, Bars& bars, uint32_t* status) { wait_count(&bars.finished, d.piece, bars, status); }
+__device__ __forceinline__ void end_turn(const Deposit& d, Bars& bars, int lane) { set_count(&bars.finished, d.piece + 1, lane); }
+template <int NT>
+__device__ __forceinline__ float sum_of(const Deposit& d, int slots, int row, int token) {
+    const float* at = d.scratch + ((d.piece & 1) * kConsumers * NT + (token >> 3)) * 128 + ((row >> 3) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
     float s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kConsumers; ++w) s += at[w * 2 * NT * 128];
+    for (int w = 0; w < slots; ++w) s += at[w * NT * 128];
     return s;
 }
 
