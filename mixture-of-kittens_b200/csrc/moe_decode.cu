@@ -6,8 +6,8 @@
 //              the same 8 up rows, so that hidden = silu(gate) * up is formed where the sums end up.
 //   down:      every SM owns a slice of the output's columns and walks all experts, so a token's sum over its experts happens in
 //              one place, in shared memory, in a fixed order: shared expert, then experts by number.  No atomics on values, no
-//              partial rows.  The warp that completes an expert's sum adds it while the others are at the next experts: when the
-//              whole block met for every expert, 2000 of 2500 clocks an expert were latency (hidden 2048, intermediate 768).
+//              partial rows.  One warp adds the experts' parts while the others are at the next experts: when the whole block met for
+//              every expert, 2000 of 2500 clocks an expert were latency (hidden 2048, intermediate 768).
 //
 // The second kernel is launched while the first runs, next to it on each SM, fills its ring with down weights and waits for the
 // hidden rows in hardware (programmatic dependent launch): no spinning, and nothing has to be co-resident for it to finish.
@@ -71,11 +71,66 @@ __device__ __forceinline__ Routing carve_routing(uint8_t* smem, int experts, int
     return r;
 }
 
+// Up to 32 routes: one warp, in registers (the general form costs a single token 4 us, mostly instruction misses).
+__device__ __forceinline__ void find_experts_of_few(const Decode& p, const Routing& r, int lane) {
+    const int routes = p.tokens * p.topk, token = lane / p.topk;
+    uint32_t e = kNobody;
+    float w = 0.0f;
+    if (lane < routes) {
+        const uint32_t local = static_cast<uint32_t>(__ldcg(p.routes + lane)) - static_cast<uint32_t>(p.first_expert);
+        if (local < static_cast<uint32_t>(p.experts)) e = local;
+        w = __ldcg(p.route_weights + lane);
+    }
+    const uint32_t same = __match_any_sync(0xffffffffu, e == kNobody ? 0x80000000u | lane : e << 8 | token);   // token and expert
+    const bool first = e != kNobody && (same & ((1u << lane) - 1u)) == 0;
+    if (__any_sync(0xffffffffu, (same & (same - 1u)) != 0)) {
+        float sum = 0.0f;
+        for (int l = 0; l < routes; ++l) {
+            const float other = __shfl_sync(0xffffffffu, w, l);
+            if (same >> l & 1u) sum += other;
+        }
+        w = sum;
+    }
+    const uint32_t mates = __match_any_sync(0xffffffffu, first ? e : 0x80000000u | lane);
+    const int mine = __popc(mates) | (__popc(mates) + p.token_cap - 1) / p.token_cap << 16;
+    int rank = 0, before = 0, total = 0;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, first && (mates & ((1u << lane) - 1u)) == 0);
+    for (uint32_t left = leaders; left != 0; left &= left - 1u) {
+        const int l = __ffs(left) - 1;
+        const uint32_t other = __shfl_sync(0xffffffffu, e, l);
+        const int its = __shfl_sync(0xffffffffu, mine, l);
+        total += its;
+        if (other < e) {
+            ++rank;
+            before += its;
+        }
+    }
+    if (first) {
+        const int at = (before & 0xFFFF) + __popc(mates & ((1u << lane) - 1u));
+        r.list[at] = static_cast<uint16_t>(lane);
+        r.token[at] = static_cast<uint8_t>(token);
+        r.weights[at] = w;
+        r.active[rank] = static_cast<uint16_t>(e);   // by every route of the expert, alike
+        r.begin[rank] = static_cast<uint16_t>(before & 0xFFFF);
+        r.passes[rank] = static_cast<uint16_t>(before >> 16);
+    }
+    if (lane == 0) {
+        r.begin[__popc(leaders)] = static_cast<uint16_t>(total & 0xFFFF);
+        r.passes[__popc(leaders)] = static_cast<uint16_t>(total >> 16);
+        *r.num_active = __popc(leaders);
+    }
+}
+
 // The consumer threads of the block.
 __device__ __forceinline__ void find_experts(const Decode& p, const Routing& r) {
     const int routes = p.tokens * p.topk;
+    if (routes <= 32) {
+        if (threadIdx.x < 32) find_experts_of_few(p, r, threadIdx.x);
+        consumer_barrier();
+        return;
+    }
     for (int i = threadIdx.x; i < routes; i += kConsumerThreads) {
-        const uint32_t e = static_cast<uint32_t>(p.routes[i]) - static_cast<uint32_t>(p.first_expert);
+        const uint32_t e = static_cast<uint32_t>(__ldcg(p.routes + i)) - static_cast<uint32_t>(p.first_expert);
         r.expert[i] = static_cast<uint16_t>(e < static_cast<uint32_t>(p.experts) ? e : kNobody);
     }
     for (int e = threadIdx.x; e < p.experts; e += kConsumerThreads) r.next[e] = 0;
@@ -124,9 +179,9 @@ __device__ __forceinline__ void find_experts(const Decode& p, const Routing& r) 
     for (int i = threadIdx.x; i < routes; i += kConsumerThreads) {
         const int token = i / p.topk;
         if (!counts(i, token)) continue;
-        float w = p.route_weights[i];
+        float w = __ldcg(p.route_weights + i);
         for (int j = i + 1; j < (token + 1) * p.topk; ++j)
-            if (r.expert[j] == r.expert[i]) w += p.route_weights[j];
+            if (r.expert[j] == r.expert[i]) w += __ldcg(p.route_weights + j);
         const int at = atomicAdd(&r.next[r.expert[i]], 1);   // any order: a column's sums do not depend on its place
         r.list[at] = static_cast<uint16_t>(i);
         r.token[at] = static_cast<uint8_t>(token);
@@ -196,13 +251,36 @@ __global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    allow_next_kernel();
     Ring ring = set_up_ring(bars, smem, p.stage_bytes, p.stages, kConsumerThreads);
+    wait_previous_kernel();
+    allow_next_kernel();   // not before: the down kernel reads weights and routes that earlier kernels may have written
     Deposit sums;
     sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
     const Routing r = carve_routing(reinterpret_cast<uint8_t*>(sums.scratch + deposit_floats<NT>()), p.experts, p.tokens * p.topk);
     const int chunks = Form<false, false>::chunks(p.hidden_size), chunks8 = Form<true, false>::chunks(p.hidden_size);
-    if (warp >= kConsumers) {
+    auto slots_of = [&](const Piece& q) { return min(W8 && q.expert >= 0 ? chunks8 : chunks, kConsumers); };
+    if (warp == kFinisher) {
+        auto run = [&](const Piece& q) {
+            const int slots = slots_of(q);
+            collect(sums, bars, p.status, slots);
+            for (int i = lane; i < kPairs * q.tokens; i += 32) {
+                const int pair = i & (kPairs - 1), c = i / kPairs;
+                if (pair >= q.count) continue;
+                float g = sum_of<NT>(sums, slots, pair, c), u = sum_of<NT>(sums, slots, pair + 8, c);
+                if (p.clamp) {   // comparisons that let a NaN through
+                    g = g > p.limit ? p.limit : g;
+                    u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+                }
+                const bf16 h = __float2bfloat16(g * sigmoid_fast(g) * u);
+                if (q.expert < 0) p.hidden_shared[static_cast<long long>(q.from + c) * p.shared_intermediate + q.row + pair] = h;
+                else p.hidden[static_cast<long long>(r.list[q.from + c]) * p.intermediate + q.row + pair] = h;
+            }
+            collected(sums, bars, lane);
+            return true;
+        };
+        for_shared_pieces(p, run);
+        if (mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) for_routed_pieces(p, r, run);
+    } else if (warp >= kConsumers) {
         int turn = warp - kConsumers;   // this producer's next chunk, counted from the piece's first
         auto run = [&](const Piece& q) {
             const bool shared = q.expert < 0, w8 = W8 && !shared;
@@ -232,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p
         int turn = warp;   // this warp's next chunk, counted from the piece's first
         auto run = [&](const Piece& q) {
             const bool shared = q.expert < 0, w8 = W8 && !shared;
-            const int n = w8 ? chunks8 : chunks, tiles = (q.tokens + 7) >> 3, slots = min(n, kConsumers);
+            const int n = w8 ? chunks8 : chunks, tiles = (q.tokens + 7) >> 3;
             const int slot = turn;
             if (slot < n) {
                 float acc[NT][4];
@@ -251,21 +329,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p
                     for (int c = slot; c < n; c += kConsumers)
                         consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, s, lane, acc);
                 }
-                if (deposit<NT>(sums, bars, p.status, acc, slot, slots, tiles, lane)) {
-                    for (int i = lane; i < kPairs * q.tokens; i += 32) {
-                        const int pair = i & (kPairs - 1), c = i / kPairs;
-                        if (pair >= q.count) continue;
-                        float g = sum_of<NT>(sums, slots, pair, c), u = sum_of<NT>(sums, slots, pair + 8, c);
-                        if (p.clamp) {   // comparisons that let a NaN through
-                            g = g > p.limit ? p.limit : g;
-                            u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
-                        }
-                        const bf16 h = __float2bfloat16(g * sigmoid_fast(g) * u);
-                        if (shared) p.hidden_shared[static_cast<long long>(q.from + c) * p.shared_intermediate + q.row + pair] = h;
-                        else p.hidden[static_cast<long long>(r.list[q.from + c]) * p.intermediate + q.row + pair] = h;
-                    }
-                    release(sums, bars, lane);
-                }
+                deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
             }
             ++sums.piece;
             ring.next_piece(n);
@@ -394,124 +458,130 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const Decode p) {
     float* out = sums.scratch + deposit_floats<NT>();   // [token][row of the piece]
     const int values = p.tokens * kRows;
     const Routing r = carve_routing(reinterpret_cast<uint8_t*>(out + values), p.experts, p.tokens * p.topk);
-    if (warp >= kConsumers) {
+    if (warp >= kConsumers && warp != kFinisher) {
         produce_down<W8, NT>(p, r, slice, ring, bars, warp - kConsumers, lane);
         return;
     }
-    find_experts(p, r);
-    mbar_arrive(smem_u32(&bars.routed));
+    auto depth_of = [&](const Piece& q) { return q.expert < 0 ? p.shared_intermediate : p.intermediate; };
+    auto chunks_of = [&](const Piece& q) {
+        return W8 && q.expert >= 0 ? Form<W8, false>::chunks(depth_of(q)) : Form<false, false>::chunks(depth_of(q));
+    };
+    const bool finisher = warp == kFinisher;
+    const int worker = finisher ? kConsumerThreads + lane : threadIdx.x;   // of the consumers and the finisher
+    if (!finisher) {
+        find_experts(p, r);
+        mbar_arrive(smem_u32(&bars.routed));
+    }
     int turn = warp;
     for (int i = 0; i < slice.pieces; ++i) {
-        for (int k = threadIdx.x; k < values; k += kConsumerThreads) out[k] = 0.0f;
-        consumer_barrier();
+        for (int k = worker; k < values; k += kConsumerThreads + 32) out[k] = 0.0f;
+        asm volatile("bar.sync 2, %0;" ::"n"(kConsumerThreads + 32) : "memory");
         const int row0 = slice.row(i), count = slice.row(i + 1) - row0;
-        for_experts(p, r, row0, count, false, [&](const Piece& q) {
-            const bool shared = q.expert < 0, w8 = W8 && !shared;
-            const int depth = shared ? p.shared_intermediate : p.intermediate, tiles = (q.tokens + 7) >> 3;
-            const int n = w8 ? Form<W8, false>::chunks(depth) : Form<false, false>::chunks(depth), slots = min(n, kConsumers);
-            const int slot = turn;
-            if (slot < n) {
-                float acc[NT][4];
-                clear(acc);
-                Scales<false, NT> s;
-                if (w8) {
-                    const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
-                    const int lo = min(q.row + (lane >> 2), p.hidden_size - 1), hi = min(lo + 8, p.hidden_size - 1);
-                    const long long at = static_cast<long long>(q.expert) * row_blocks;
-                    s.lo = p.down_scales + (at + lo / 128) * blocks;
-                    s.hi = p.down_scales + (at + hi / 128) * blocks;
-                    s.row_block = 1;
-                    for (int c = slot; c < n; c += kConsumers)
-                        consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
-                } else {
-                    for (int c = slot; c < n; c += kConsumers)
-                        consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
+        if (finisher) {
+            for_experts(p, r, row0, count, false, [&](const Piece& q) {
+                const int slots = min(chunks_of(q), kConsumers);
+                collect(sums, bars, p.status, slots);
+                for (int k = lane; k < kRows * q.tokens; k += 32) {   // a token is listed once
+                    const int row = k & (kRows - 1), c = k / kRows;
+                    float* at = out + (q.expert < 0 ? q.from + c : r.token[q.from + c]) * kRows + row;
+                    *at = fmaf(q.expert < 0 ? 1.0f : r.weights[q.from + c], sum_of<NT>(sums, slots, row, c), *at);
                 }
-                if (deposit<NT>(sums, bars, p.status, acc, slot, slots, tiles, lane)) {
-                    wait_turn(sums, bars, p.status);
-                    for (int k = lane; k < kRows * q.tokens; k += 32) {   // a token is listed once
-                        const int row = k & (kRows - 1), c = k / kRows;
-                        float* at = out + (shared ? q.from + c : r.token[q.from + c]) * kRows + row;
-                        *at = fmaf(shared ? 1.0f : r.weights[q.from + c], sum_of<NT>(sums, slots, row, c), *at);
+                collected(sums, bars, lane);
+                return true;
+            });
+        } else {
+            for_experts(p, r, row0, count, false, [&](const Piece& q) {
+                const bool w8 = W8 && q.expert >= 0;
+                const int depth = depth_of(q), n = chunks_of(q), tiles = (q.tokens + 7) >> 3, slot = turn;
+                if (slot < n) {
+                    float acc[NT][4];
+                    clear(acc);
+                    Scales<false, NT> s;
+                    if (w8) {
+                        const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
+                        const int lo = min(q.row + (lane >> 2), p.hidden_size - 1), hi = min(lo + 8, p.hidden_size - 1);
+                        const long long at = static_cast<long long>(q.expert) * row_blocks;
+                        s.lo = p.down_scales + (at + lo / 128) * blocks;
+                        s.hi = p.down_scales + (at + hi / 128) * blocks;
+                        s.row_block = 1;
+                        for (int c = slot; c < n; c += kConsumers)
+                            consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
+                    } else {
+                        for (int c = slot; c < n; c += kConsumers)
+                            consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
                     }
-                    end_turn(sums, bars, lane);
-                    release(sums, bars, lane);
+                    deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
                 }
-            }
-            ++sums.piece;
-            ring.next_piece(n);
-            turn = (turn - n) & (kConsumers - 1);
-            return true;
-        });
-        consumer_barrier();
+                ++sums.piece;
+                ring.next_piece(n);
+                turn = (turn - n) & (kConsumers - 1);
+                return true;
+            });
+        }
+        asm volatile("bar.sync 2, %0;" ::"n"(kConsumerThreads + 32) : "memory");
         wait_previous_kernel();   // its word on how it went
         const bool bad = p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0;
-        for (int k = threadIdx.x; k < values; k += kConsumerThreads) {
+        for (int k = worker; k < values; k += kConsumerThreads + 32) {
             const int row = k & (kRows - 1), token = k / kRows;
             if (row < count)
                 p.out[static_cast<long long>(token) * p.hidden_size + row0 + row] = __float2bfloat16(bad ? __uint_as_float(0x7FC00000u) : out[k]);
         }
-        consumer_barrier();
+        asm volatile("bar.sync 2, %0;" ::"n"(kConsumerThreads + 32) : "memory");
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kStatic = 1024 + 512;   // reserved per block + barriers
+constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kStatic = 1024 + 384;   // reserved per block + barriers
+static_assert(sizeof(Bars) <= 384, "");
+// The two kernels share the SMs when the first takes a little more than half of the shared memory (two of its blocks on one SM, while
+// another SM has none, cost 40 us of 250) and the second what is left.
+constexpr int kGateUpBytes = kSmemPerSm / 2 - kStatic + 128, kDownBytes = kSmemPerSm - kGateUpBytes - 2 * kStatic;
 
-// Ring of a kernel whose other shared memory is `other` bytes: 8 or 16 stages, so that every consumer keeps its stages, with room for
-// the second kernel's block next to it on the SM, or else 8 that take what they need.  0: does not fit.
-int ring_stages(int stage, int other) {
-    const int half = (kSmemPerSm / 2 - kStatic - other) / stage;
-    if (half >= kConsumers) return half >= 2 * kConsumers ? 2 * kConsumers : kConsumers;
-    return (kSmemPerBlock - kStatic - other) / stage >= kConsumers ? kConsumers : 0;
+int stage_bytes(int tokens, bool w8) {   // the shared expert is bf16 in either case
+    const int a = Form<false, false>::stage_bytes(tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
+    return a > b ? a : b;
+}
+// Shared memory beside the ring.
+int gate_up_rest(const Decode& p, int nt) { return kDeposits * kConsumers * nt * 128 * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
+int down_rest(const Decode& p, int nt) { return gate_up_rest(p, nt) + p.tokens * kRows * 4; }
+
+// Tokens of a stage; 0: nothing fits.  The ring has 8 stages, so that every consumer keeps its own.  An expert that more tokens chose
+// is read more than once (from L2 after the first time), so few suffice where experts see few tokens, and then both kernels fit an SM;
+// with more tokens the stages take what they need.
+int token_cap(const Decode& p, bool w8) {
+    const int most = p.tokens < (w8 ? 4 : 6) ? p.tokens : w8 ? 4 : 6;
+    if (p.tokens <= (w8 ? 4 : 32))
+        for (int cap = most; cap >= (most < 4 ? most : 4); --cap)
+            if (kConsumers * stage_bytes(cap, w8) + gate_up_rest(p, 1) <= kGateUpBytes && kConsumers * stage_bytes(cap, w8) + down_rest(p, 1) <= kDownBytes) return cap;
+    for (int cap = w8 ? 8 : 16; cap >= 4; cap -= 4)
+        if (kConsumers * stage_bytes(cap, w8) + down_rest(p, cap > 8 ? 2 : 1) <= kSmemPerBlock - kStatic) return cap;
+    return 0;
 }
 
-// Tokens of a stage.  An expert that more tokens chose is read more than once (from L2 after the first time), so few suffice where
-// experts see few tokens, and eight stages of them fit an SM twice; with more tokens the second block's room goes to the stages.
-int token_cap(int tokens, bool w8) {
-    if (w8) return tokens <= 4 ? tokens : 8;
-    return tokens <= 6 ? tokens : tokens <= 32 ? 6 : 16;
-}
-
-template <bool W8, int NT, typename Kernel>
-int launch_decode(Kernel kernel, const char* name, int (&ready)[16], Decode p, int other, bool early, cudaStream_t stream) {
+template <typename Kernel>
+int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decode& p, int smem, cudaStream_t stream) {
     int dev = 0;
     MOK_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 16) return MOK_ERR_UNSUPPORTED;
     if (ready[dev] == 0) {
         MOK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock - kStatic));
+        // all of it as shared memory: a partition that just fits one kernel keeps the other off the SM
+        MOK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
         ready[dev] = 1;
     }
-    // the shared expert is bf16 in either case; the rows of a stage's last n tile that no token has are read as what follows in memory
-    const int a = Form<false, false>::stage_bytes(p.token_cap), b = W8 ? Form<true, false>::stage_bytes(p.token_cap) : 0;
-    p.stage_bytes = a > b ? a : b;
-    p.stages = ring_stages(p.stage_bytes, other);
-    if (p.stages == 0) return MOK_ERR_TOO_LARGE;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sm_count());
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = other + p.stages * p.stage_bytes;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = early ? 1 : 0;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
-    if (err != cudaSuccess) return fail_cuda(name, err);
-    MOK_LAUNCH_CHECK(name);
-    return MOK_OK;
+    return launch_early(kernel, name, dim3(sm_count()), kThreads, smem, stream, p);
 }
 
 template <bool W8, int NT>
-int run_decode(const Decode& p, cudaStream_t stream) {
+int run_decode(Decode p, cudaStream_t stream) {
     static int gate_up_ready[16] = {0}, down_ready[16] = {0};
-    const int routing = routing_bytes(p.experts, p.tokens * p.topk);
-    MOK_TRY((launch_decode<W8, NT>(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, deposit_floats<NT>() * 4 + routing, false, stream)));
-    return launch_decode<W8, NT>(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, p, (deposit_floats<NT>() + p.tokens * kRows) * 4 + routing, true,
-                                 stream);
+    p.stages = kConsumers;
+    p.stage_bytes = stage_bytes(p.token_cap, W8);
+    const int ring = p.stages * p.stage_bytes, gate_up = ring + gate_up_rest(p, NT);
+    MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, gate_up > kGateUpBytes ? gate_up : kGateUpBytes, stream));
+    return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, p, ring + down_rest(p, NT), stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -570,7 +640,8 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.clamp = has_limit;
     p.limit = limit;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    p.token_cap = token_cap(num_tokens, w8);
+    p.token_cap = token_cap(p, w8);
+    if (p.token_cap == 0) return MOK_ERR_TOO_LARGE;
     if (w8) return run_decode<true, 1>(p, s);
     return p.token_cap <= 8 ? run_decode<false, 1>(p, s) : run_decode<false, 2>(p, s);
 }

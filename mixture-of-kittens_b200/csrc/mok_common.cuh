@@ -113,6 +113,32 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // ---------------------------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel launched with launch_early() may begin while the one before it in the stream still runs.
+// It has to wait_previous_kernel() before it touches anything that one may write; allow_next_kernel() lets the next one begin.
+// Both do nothing in other launches.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename Kernel, typename... Args>
+int launch_early(Kernel kernel, const char* name, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (err != cudaSuccess) return fail_cuda(name, err);
+    MOK_LAUNCH_CHECK(name);
+    return MOK_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
 // TMA (bulk tensor copies, global -> shared; the loads themselves are with the CTA-pair helpers below)
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {

@@ -27,6 +27,8 @@ __global__ void __launch_bounds__(256) topk_softmax_kernel(const float* __restri
                                                             int32_t* __restrict__ routes, float* __restrict__ weights) {
     const int lane = threadIdx.x & 31;
     const int warps = (gridDim.x * blockDim.x) >> 5;
+    wait_previous_kernel();
+    allow_next_kernel();
     for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < tokens; t += warps) {
         float v[PER_LANE];
 #pragma unroll
@@ -111,6 +113,7 @@ template <int EXPERTS, int TOKENS, bool W32>
 __global__ void __launch_bounds__(256) few_logits_kernel(const bf16* __restrict__ x, long long x_stride, const void* __restrict__ w, int tokens,
                                                          int hidden, int experts, float* __restrict__ logits) {
     __shared__ float part[8][EXPERTS * TOKENS];
+    allow_next_kernel();
     const int e0 = blockIdx.x * EXPERTS, t0 = blockIdx.y * TOKENS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float acc[EXPERTS][TOKENS];
@@ -182,12 +185,18 @@ int warp_grid(int tokens) {
     return static_cast<int>(blocks < cap ? blocks : cap);
 }
 
+// `early`: launched while the kernel that writes the logits runs.
 int launch_topk(const float* logits, const float* bias, int T, int num_experts, int ld, int topk, int32_t* top_experts, float* router_weights,
-                cudaStream_t s) {
-    const int grid = warp_grid(T);
+                bool early, cudaStream_t s) {
+    const int grid = early ? T : warp_grid(T), threads = early ? 32 : 256;   // few tokens: one warp a block
     const int per_lane = (num_experts + 31) / 32;
-#define MOK_TOPK_CASE(N)                                                                                                   \
-    topk_softmax_kernel<N><<<grid, 256, 0, s>>>(logits, bias, T, num_experts, ld, topk, top_experts, router_weights)
+#define MOK_TOPK_CASE(N)                                                                                                                 \
+    do {                                                                                                                                 \
+        if (early)                                                                                                                       \
+            return launch_early(topk_softmax_kernel<N>, "topk_softmax_kernel", dim3(grid), threads, 0, s, logits, bias, T, num_experts,  \
+                                ld, topk, top_experts, router_weights);                                                                  \
+        topk_softmax_kernel<N><<<grid, threads, 0, s>>>(logits, bias, T, num_experts, ld, topk, top_experts, router_weights);            \
+    } while (0)
     if (per_lane <= 1) MOK_TOPK_CASE(1);
     else if (per_lane <= 2) MOK_TOPK_CASE(2);
     else if (per_lane <= 4) MOK_TOPK_CASE(4);
@@ -224,7 +233,7 @@ extern "C" int mok_router_forward(const void* x, const void* w_hi, const void* w
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int T = static_cast<int>(num_tokens);
     MOK_TRY(launch_rows_gemm_f32(dense_problem(T, status), x, hidden, w_hi, w_lo, logits, padded_experts, s));
-    return launch_topk(logits, bias, T, num_experts, padded_experts, topk, top_experts, router_weights, s);
+    return launch_topk(logits, bias, T, num_experts, padded_experts, topk, top_experts, router_weights, false, s);
 }
 
 extern "C" int mok_router_backward(const void* x, const void* w_hi, const int32_t* top_experts, const float* router_weights,
@@ -268,5 +277,5 @@ extern "C" int mok_router_decode(const void* x, int64_t x_stride, const void* w,
     const bf16* xb = static_cast<const bf16*>(x);
     MOK_TRY(w_is_f32 ? launch_few_logits<true>(xb, x_stride, w, num_tokens, hidden, num_experts, logits, s)
                      : launch_few_logits<false>(xb, x_stride, w, num_tokens, hidden, num_experts, logits, s));
-    return launch_topk(logits, bias, num_tokens, num_experts, num_experts, topk, top_experts, router_weights, s);
+    return launch_topk(logits, bias, num_tokens, num_experts, num_experts, topk, top_experts, router_weights, true, s);
 }

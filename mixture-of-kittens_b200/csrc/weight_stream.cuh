@@ -4,16 +4,18 @@
 // A block has four producer warps and eight consumer warps around a ring of stages.  A stage is a chunk of a piece: 16 weight rows
 // and the rows of the tokens concerned, kChunk elements of k.  One producer warp fills it with cp.async (32 x 16 bytes lie in one
 // row: any row count, stride and gather), one consumer warp multiplies it with mma.sync (weights on the M side, tokens on the N
-// side of 8); chunks go round the producers and round the consumers in turn.  Producers run ahead as far as the ring reaches: about
-// 64 KB of weights in flight per block is what HBM needs.  tcgen05 would need 128 rows a tile, which leaves SMs idle at these
-// sizes; the tensor work here is a few percent of the time.
+// side of 8); chunks go round the producers and round the consumers in turn.  A last warp, the finisher, adds up the chunks' sums of
+// a piece and does with them what the kernel is for, while the consumers are at the next piece.  Producers run ahead as far as the
+// ring reaches: about 64 KB of weights in flight per block is what HBM needs.  tcgen05 would need 128 rows a tile, which leaves SMs
+// idle at these sizes; the tensor work here is a few percent of the time.
 //
 // The barriers of a stage tell rounds apart by one bit, so nobody may be two rounds ahead of a barrier: the number of stages is a
 // multiple of eight, so that a stage has one producer and one consumer, which have seen every round of it.
 //
 // What did not do: bulk copies, one per row (an SM issues one in about 60 clocks: 1.4 - 1.8 TB/s with rows of 512 bytes, 2.2 - 3.4
 // with 1024); every consumer taking an eighth of every chunk (all eight pay the waits and addresses of each chunk, 350 instructions
-// a warp for 21 KB of weights: 2.1 - 3.7 TB/s with experts of 768 rows).
+// a warp for 21 KB of weights: 2.1 - 3.7 TB/s with experts of 768 rows); the last consumer of a piece as its finisher (178 instead of
+// 147 us for the blocks whose experts have five tokens or more).
 //
 // The order of k within a slice of 32 is free as long as both operands use the same one: lane (g, t) of an mma takes elements 8 t ..
 // 8 t + 7 of rows g and g + 8, one 16-byte (8-byte in e4m3) shared-memory load per row, for two mma of K = 16.  Row pitches of 64
@@ -30,7 +32,8 @@ namespace stream {
 constexpr int kConsumers = 8;                       // warps
 constexpr int kConsumerThreads = kConsumers * 32;
 constexpr int kProducers = 4;
-constexpr int kThreads = kConsumerThreads + kProducers * 32;
+constexpr int kFinisher = kConsumers + kProducers;  // warp
+constexpr int kThreads = kConsumerThreads + kProducers * 32 + 32;
 constexpr int kRows = 16;                           // weight rows of a piece
 constexpr int kMaxStages = 16;
 constexpr int kDeposits = 2;
@@ -59,13 +62,9 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory"); }
-// The other kernels of a stream: let the next one begin, and wait for the one before to be done and visible.
-__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages], routed;
-    int count[kDeposits], done[kDeposits], finished;   // deposits of the piece so far; pieces that left the deposit; pieces in order
+    int count[kDeposits], done[kDeposits];   // deposits so far, pieces that were finished
     int abort_flag;
 };
 
@@ -110,7 +109,6 @@ __device__ __forceinline__ Ring set_up_ring(Bars& bars, const uint8_t* smem, int
             bars.count[d] = bars.done[d] = 0;
         }
         mbar_init(smem_u32(&bars.routed), routed_arrivals);
-        bars.finished = 0;
         bars.abort_flag = 0;
         mbar_fence_init();
     }
@@ -329,20 +327,21 @@ __device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages,
 }
 
 // ---- sums of a piece over the consumers -----------------------------------------------------------------------------
-// Chunk c's sums go to slot c % 8 (whichever warp computed them), so the order of the final addition is that of k.  The warp that
-// deposits last adds the slots and goes on to what becomes of them; the others are at the next piece by then (two deposits in turn).
+// Chunk c's sums go to slot c % 8 (whichever warp computed them), so the order of the final addition is that of k.  Two deposits in
+// turn: consumers are at most two pieces ahead of the finisher.
 template <int NT>
 constexpr int deposit_floats() { return kDeposits * kConsumers * NT * 128; }
 
 struct Deposit {
     float* scratch;
-    int piece = 0;      // pieces so far
+    int piece = 0;                     // pieces so far
+    int expected[kDeposits] = {0, 0};  // finisher: deposits that make the pieces so far complete
 };
-// Waits, with the limit of all pipeline waits, until a counter in shared memory has a value.  Not a barrier of one bit: a warp may
-// have no part in many pieces and be far ahead.
+// Waits, with the limit of all pipeline waits, until a counter in shared memory has reached a value.  Not a barrier of one bit: a
+// warp may have no part in many pieces and be far ahead.
 __device__ __forceinline__ void wait_count(int* counter, int value, Bars& bars, uint32_t* status) {
     const long long start = clock64();
-    while (*static_cast<volatile int*>(counter) != value && !*static_cast<volatile int*>(&bars.abort_flag)) {
+    while (*static_cast<volatile int*>(counter) < value && !*static_cast<volatile int*>(&bars.abort_flag)) {
         if (clock64() - start > kPipelineWaitCycles) {
             *static_cast<volatile int*>(&bars.abort_flag) = 1;
             if (status != nullptr) atomicOr(status, (uint32_t)MOK_STATUS_PIPELINE_TIMEOUT);
@@ -351,14 +350,8 @@ __device__ __forceinline__ void wait_count(int* counter, int value, Bars& bars, 
     __threadfence_block();
     __syncwarp();
 }
-__device__ __forceinline__ void set_count(int* counter, int value, int lane) {
-    __threadfence_block();
-    __syncwarp();
-    if (lane == 0) *static_cast<volatile int*>(counter) = value;
-}
-// True for the warp that has to finish the piece; `slots` of them were filled.  It calls release() afterwards.
 template <int NT>
-__device__ __forceinline__ bool deposit(const Deposit& d, Bars& bars, uint32_t* status, const float (&acc)[NT][4], int slot, int slots, int tiles, int lane) {
+__device__ __forceinline__ void deposit(const Deposit& d, Bars& bars, uint32_t* status, const float (&acc)[NT][4], int slot, int tiles, int lane) {
     const int which = d.piece & 1;
     wait_count(&bars.done[which], d.piece >> 1, bars, status);
     float* at = d.scratch + (which * kConsumers + slot) * NT * 128 + lane;
@@ -369,24 +362,28 @@ __device__ __forceinline__ bool deposit(const Deposit& d, Bars& bars, uint32_t* 
             for (int r = 0; r < 4; ++r) at[n * 128 + r * 32] = acc[n][r];
     __threadfence_block();
     __syncwarp();
-    int last = 0;
-    if (lane == 0) {
-        last = atomicAdd(&bars.count[which], 1) == slots - 1;
-        if (last) bars.count[which] = 0;
-    }
-    last = __shfl_sync(0xffffffffu, last, 0);
-    if (last) __threadfence_block();
-    return last != 0;
+    if (lane == 0) atomicAdd(&bars.count[which], 1);
 }
-__device__ __forceinline__ void release(const Deposit& d, Bars& bars, int lane) { set_count(&bars.done[d.piece & 1], (d.piece >> 1) + 1, lane); }
-// Lets the finishing warps through in the order of their pieces.
-__device__ __forceinline__ void wait_turn(const Deposit& d, Bars& bars, uint32_t* status) { wait_count(&bars.finished, d.piece, bars, status); }
-__device__ __forceinline__ void end_turn(const Deposit& d, Bars& bars, int lane) { set_count(&bars.finished, d.piece + 1, lane); }
+// The finisher's side: every piece in order, `slots` deposits each.
+__device__ __forceinline__ void collect(Deposit& d, Bars& bars, uint32_t* status, int slots) {
+    const int which = d.piece & 1;
+    d.expected[which] += slots;
+    wait_count(&bars.count[which], d.expected[which], bars, status);
+}
+__device__ __forceinline__ void collected(Deposit& d, Bars& bars, int lane) {
+    __threadfence_block();
+    __syncwarp();
+    if (lane == 0) *static_cast<volatile int*>(&bars.done[d.piece & 1]) = (d.piece >> 1) + 1;
+    ++d.piece;
+}
 template <int NT>
 __device__ __forceinline__ float sum_of(const Deposit& d, int slots, int row, int token) {
     const float* at = d.scratch + ((d.piece & 1) * kConsumers * NT + (token >> 3)) * 128 + ((row >> 3) * 2 + (token & 1)) * 32 + (row & 7) * 4 + ((token & 7) >> 1);
-    float s = 0.0f;
-    for (int w = 0; w < slots; ++w) s += at[w * NT * 128];
+    float v[kConsumers], s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kConsumers; ++w) v[w] = w < slots ? at[w * NT * 128] : 0.0f;
+#pragma unroll
+    for (int w = 0; w < kConsumers; ++w) s += v[w];
     return s;
 }
 

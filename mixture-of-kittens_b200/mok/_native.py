@@ -157,6 +157,17 @@ def stream_ptr(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_ENTRIES: dict[str, ctypes._CFuncPtr] = {}
+
+
+def entry(name: str):
+    """The library's function of that name."""
+    function = _ENTRIES.get(name)
+    if function is None:
+        function = _ENTRIES[name] = getattr(lib(), name)
+    return function
+
+
 def launch(what: str, function, device: torch.device, *args) -> None:
     """Calls an entry point whose last argument is the stream, on `device` (made current for the call) and its current stream.
     Tensors are passed as addresses (`Tensor.data_ptr()`, None = NULL): small operators are bound by this path."""

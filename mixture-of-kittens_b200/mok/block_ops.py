@@ -14,7 +14,8 @@ from __future__ import annotations
 
 import torch
 
-from ._native import launch, lib, status_word
+from ._native import entry as _entry
+from ._native import launch, status_word
 from .ops import _require
 
 E4M3 = torch.float8_e4m3fn
@@ -22,9 +23,14 @@ _BF16, _F32 = torch.bfloat16, torch.float32
 BLOCK = 128
 
 
+_traced_impl = None
+
+
 def _traced() -> bool:
-    from .functional import _traced as traced
-    return traced()
+    global _traced_impl
+    if _traced_impl is None:
+        from .functional import _traced as _traced_impl
+    return _traced_impl()
 
 
 def _round_up(n: int, m: int) -> int:
@@ -39,7 +45,8 @@ def _check_matrix(name: str, x: torch.Tensor, multiple: int) -> None:
     _require(x.ndim == 2, name + " must be two-dimensional")
     _require(x.is_cuda, name + " must be a CUDA tensor")
     _require(x.dtype is _BF16, name + " must be bfloat16", TypeError)
-    _require(x.shape[1] > 0 and x.shape[1] % multiple == 0, f"{name}'s last dimension must be a positive multiple of {multiple}")
+    if x.shape[1] <= 0 or x.shape[1] % multiple:
+        raise ValueError(f"{name}'s last dimension must be a positive multiple of {multiple}")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -94,7 +101,7 @@ def _norm_forward(x, weight, residual, eps, want_y, want_codes, want_rms):
     scales = _new_scales(x, T, H, 1) if want_codes else None
     rms = x.new_empty((T,), dtype=_F32) if want_rms else None
     if T:
-        launch("rms_norm", lib().mok_rms_norm_forward, x.device, x.data_ptr(), x.stride(0), _address(residual),
+        launch("rms_norm", _entry("mok_rms_norm_forward"), x.device, x.data_ptr(), x.stride(0), _address(residual),
                0 if residual is None else residual.stride(0), weight.data_ptr(), weight.dtype is _F32, T, H, eps, _address(hidden),
                _address(y), _address(codes), codes.stride(0) if want_codes else 0, _address(scales),
                scales.stride(0) if want_codes else 0, scales.stride(1) if want_codes else 0, _address(rms))
@@ -143,8 +150,8 @@ def _norm_backward(d_y, d_hidden, z, weight, rms):
         weight = weight.clone()
     d_y = _rows(d_y.contiguous())
     d_hidden = None if d_hidden is None else _rows(d_hidden.contiguous())
-    scratch = z.new_empty((lib().mok_rms_norm_scratch_bytes(T, H) // 4,), dtype=_F32)
-    launch("rms_norm backward", lib().mok_rms_norm_backward, z.device, d_y.data_ptr(), _address(d_hidden), z.data_ptr(), z.stride(0),
+    scratch = z.new_empty((_entry("mok_rms_norm_scratch_bytes")(T, H) // 4,), dtype=_F32)
+    launch("rms_norm backward", _entry("mok_rms_norm_backward"), z.device, d_y.data_ptr(), _address(d_hidden), z.data_ptr(), z.stride(0),
            weight.data_ptr(), weight.dtype is _F32, rms.data_ptr(), T, H, d_x.data_ptr(), d_weight.data_ptr(), scratch.data_ptr())
     return d_x, d_weight
 
@@ -201,8 +208,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
     if _traced():
         codes, scales, hidden = rms_norm_fp8_fwd(x, weight, residual, eps)
         return (codes, scales), hidden if residual is not None else None
-    with torch.no_grad():
-        _, codes, scales, hidden, _ = _norm_forward(x, weight, residual, eps, False, True, False)
+    _, codes, scales, hidden, _ = _norm_forward(x, weight, residual, eps, False, True, False)
     return (codes, scales), hidden
 
 
@@ -221,7 +227,7 @@ def _quantize(x, tile_rows, normal, transpose):
     if transpose:
         qt, st = _new_codes(x, N, M), _new_scales(x, N, M, tile_rows)
     if M:
-        launch("block_quantize", lib().mok_block_quantize, x.device, x.data_ptr(), x.stride(0), M, N, tile_rows,
+        launch("block_quantize", _entry("mok_block_quantize"), x.device, x.data_ptr(), x.stride(0), M, N, tile_rows,
                _address(q), q.stride(0) if normal else 0, _address(s), s.stride(0) if normal else 0, s.stride(1) if normal else 0,
                _address(qt), qt.stride(0) if transpose else 0, _address(st), st.stride(0) if transpose else 0,
                st.stride(1) if transpose else 0)
@@ -255,8 +261,7 @@ def quantize_blocks(x: torch.Tensor, *, tile_rows: int = 1, transpose: bool = Fa
     if _traced():
         q, s, qt, st = block_quantize(x, tile_rows, transpose)
     else:
-        with torch.no_grad():
-            q, s, qt, st = _quantize(x, tile_rows, True, transpose)
+        q, s, qt, st = _quantize(x, tile_rows, True, transpose)
     return ((q, s), (qt, st)) if transpose else (q, s)
 
 
@@ -287,9 +292,9 @@ def _matmul(a, a_scales, b, b_scales):
     _require(a.device == b.device == a_scales.device == b_scales.device, "a, b and their scales must be on one device")
     out = a.new_empty((M, N), dtype=_BF16)
     if M:
-        size = lib().mok_block_matmul_scratch_bytes(M, N, K)
+        size = _entry("mok_block_matmul_scratch_bytes")(M, N, K)
         scratch = a.new_empty((size // 4,), dtype=_F32) if size else None
-        launch("block_matmul", lib().mok_block_matmul, a.device, a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0),
+        launch("block_matmul", _entry("mok_block_matmul"), a.device, a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0),
                a_scales.stride(1), b.data_ptr(), b.stride(0), b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), tile_rows,
                M, N, K, out.data_ptr(), N, _address(scratch), status_word(a.device).data_ptr())
     return out

@@ -8,7 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from ._native import launch, lib, status_word
+from ._native import entry as _entry
+from ._native import launch, status_word
 from .block_ops import BLOCK, E4M3, _address, _rows, _traced
 from .ops import _require
 
@@ -16,10 +17,13 @@ MAX_TOKENS, MAX_TOPK, MAX_ROUTES, MAX_EXPERTS = 256, 32, 4096, 1024
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
+# A step of one token takes 40 us on the GPU: the checks below build their messages only where they fail.
 def _check_tokens(x: torch.Tensor, multiple: int) -> None:
     _require(x.ndim == 2, "x must have shape (num_tokens, hidden_size)")
-    _require(x.shape[0] <= MAX_TOKENS, "num_tokens must be at most 256 (mok.functional.forward takes 512 and more)")
-    _require(x.shape[1] > 0 and x.shape[1] % multiple == 0, f"hidden_size must be a positive multiple of {multiple}")
+    T, H = x.shape
+    _require(T <= MAX_TOKENS, "num_tokens must be at most 256 (mok.functional.forward takes 512 and more)")
+    if H <= 0 or H % multiple:
+        raise ValueError(f"hidden_size must be a positive multiple of {multiple}")
     _require(x.is_cuda, "x must be a CUDA tensor")
     _require(x.dtype is _BF16, "x must be bfloat16", TypeError)
 
@@ -47,7 +51,7 @@ def _route(x, w_router, bias, topk):
         if w_router.data_ptr() % 16:
             w_router = w_router.clone()
         logits = x.new_empty((T, E), dtype=_F32)
-        launch("router_decode", lib().mok_router_decode, x.device, x.data_ptr(), x.stride(0), w_router.data_ptr(), w_router.dtype is _F32,
+        launch("router_decode", _entry("mok_router_decode"), x.device, x.data_ptr(), x.stride(0), w_router.data_ptr(), w_router.dtype is _F32,
                _address(bias), T, H, E, topk, logits.data_ptr(), routes.data_ptr(), weights.data_ptr())
     return routes, weights
 
@@ -66,18 +70,22 @@ def route_decode(x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor | N
     """`mok.route` for a few tokens: (top_experts int32 [T, topk], router_weights fp32 [T, topk]).  Not differentiable."""
     if _traced():
         return router_decode(x, w_router, bias, topk)
-    with torch.no_grad():
-        return _route(x, w_router, bias, topk)
+    return _route(x, w_router, bias, topk)
 
 
 # ------------------------------------------------------------------------------------------------------------
 # layer
 # ------------------------------------------------------------------------------------------------------------
-def _weight(name: str, w: torch.Tensor, shape, device, dtype) -> torch.Tensor:
-    _require(w.shape == shape, f"{name} must have shape {tuple(shape)}")
-    _require(w.device == device, name + " must be on the device of x")
-    _require(w.dtype is dtype and w.is_contiguous() and w.data_ptr() % 16 == 0, f"{name} must be contiguous {dtype}, 16-byte aligned", TypeError)
-    return w
+def _weight(name: str, w: torch.Tensor, shape, device, dtype) -> int:
+    """The weight's address."""
+    address = w.data_ptr()
+    if w.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    if w.device != device:
+        raise ValueError(f"{name} must be on the device of x")
+    if w.dtype is not dtype or address % 16 or not w.is_contiguous():
+        raise TypeError(f"{name} must be contiguous {dtype}, 16-byte aligned")
+    return address
 
 
 def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert, swiglu_limit):
@@ -101,22 +109,24 @@ def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert
     w8 = scales[0] is not None
     _require(all((s is not None) == w8 for s in scales), "the routed weights must be all bfloat16 or all (codes, scales)", TypeError)
     dtype = E4M3 if w8 else _BF16
-    _weight("w_routed_gate", gate, (E, I, H), dev, dtype)
-    _weight("w_routed_up", up, (E, I, H), dev, dtype)
-    _weight("w_routed_down", down, (E, H, I), dev, dtype)
+    up_shape, down_shape = (E, I, H), (E, H, I)
+    weights = (_weight("w_routed_gate", gate, up_shape, dev, dtype), _weight("w_routed_up", up, up_shape, dev, dtype),
+               _weight("w_routed_down", down, down_shape, dev, dtype))
     if w8:
         h, i = -(-H // BLOCK), -(-I // BLOCK)
-        for name, s, shape in (("gate", scales[0], (E, i, h)), ("up", scales[1], (E, i, h)), ("down", scales[2], (E, h, i))):
-            _weight(f"scales of w_routed_{name}", s, shape, dev, _F32)
-    _require(all(w is None for w in shared) or all(w is not None for w in shared), "the three shared weights must be given together")
-    shared_i = 0
-    if shared[0] is not None:
-        _require(shared[0].ndim == 2, "w_shared_gate must have shape (shared_intermediate_size, hidden_size)")
-        shared_i = shared[0].shape[0]
+        weights += (_weight("scales of w_routed_gate", scales[0], (E, i, h), dev, _F32), _weight("scales of w_routed_up", scales[1], (E, i, h), dev, _F32),
+                    _weight("scales of w_routed_down", scales[2], (E, h, i), dev, _F32))
+    else:
+        weights += (None, None, None)
+    sg, su, sd = shared
+    _require((sg is None) == (su is None) == (sd is None), "the three shared weights must be given together")
+    shared_i, shared_weights = 0, (None, None, None)
+    if sg is not None:
+        _require(sg.ndim == 2, "w_shared_gate must have shape (shared_intermediate_size, hidden_size)")
+        shared_i = sg.shape[0]
         _require(shared_i > 0 and shared_i % 64 == 0, "shared_intermediate_size must be a positive multiple of 64")
-        _weight("w_shared_gate", shared[0], (shared_i, H), dev, _BF16)
-        _weight("w_shared_up", shared[1], (shared_i, H), dev, _BF16)
-        _weight("w_shared_down", shared[2], (H, shared_i), dev, _BF16)
+        shared_weights = (_weight("w_shared_gate", sg, (shared_i, H), dev, _BF16), _weight("w_shared_up", su, (shared_i, H), dev, _BF16),
+                          _weight("w_shared_down", sd, (H, shared_i), dev, _BF16))
     out = x.new_empty((T, H))
     if T == 0:
         return out
@@ -125,9 +135,8 @@ def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert
         top_experts = top_experts.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     top_experts, router_weights = top_experts.contiguous(), router_weights.contiguous()
     scratch = x.new_empty((T * K * I + T * shared_i,))
-    launch("moe_decode", lib().mok_moe_decode, dev, x.data_ptr(), x.stride(0), top_experts.data_ptr(), router_weights.data_ptr(), T, K, H,
-           _address(shared[0]), _address(shared[1]), _address(shared[2]), shared_i, gate.data_ptr(), up.data_ptr(), down.data_ptr(),
-           _address(scales[0]), _address(scales[1]), _address(scales[2]), I, E, first_expert, swiglu_limit is not None,
+    launch("moe_decode", _entry("mok_moe_decode"), dev, x.data_ptr(), x.stride(0), top_experts.data_ptr(), router_weights.data_ptr(), T, K, H,
+           *shared_weights, shared_i, *weights, I, E, first_expert, swiglu_limit is not None,
            0.0 if swiglu_limit is None else float(swiglu_limit), out.data_ptr(), scratch.data_ptr(), status_word(dev).data_ptr())
     return out
 
@@ -166,6 +175,5 @@ def moe_decode(x: torch.Tensor, top_experts: torch.Tensor, router_weights: torch
     if _traced():
         return _moe_decode_op(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, g, gs, u, us, d, ds, first_expert,
                               swiglu_limit)
-    with torch.no_grad():
-        return _decode(x, top_experts, router_weights, (w_shared_gate, w_shared_up, w_shared_down), (g, u, d), (gs, us, ds), first_expert,
-                       swiglu_limit)
+    return _decode(x, top_experts, router_weights, (w_shared_gate, w_shared_up, w_shared_down), (g, u, d), (gs, us, ds), first_expert,
+                   swiglu_limit)
