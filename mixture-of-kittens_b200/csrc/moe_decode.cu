@@ -40,7 +40,7 @@ struct Decode {
     int tokens, hidden_size, intermediate, shared_intermediate, experts, first_expert, topk;
     int clamp;
     float limit;
-    int stages, stage_bytes, token_cap;   // the ring; tokens of a stage
+    int stages, stage_bytes, token_cap, shared_cap;   // the ring; tokens of a stage, of routed experts and the shared one
 };
 
 // Which experts are in use: active[i], and the range [begin[i], begin[i + 1]) of its routes in list (with their tokens and weights
@@ -206,8 +206,8 @@ __device__ __forceinline__ bool for_shared_pieces(const Decode& p, F&& f) {
     q.expert = -1;
     for (q.row = static_cast<int>(static_cast<long long>(p.shared_intermediate) * blockIdx.x / gridDim.x); q.row < end; q.row += kPairs) {
         q.count = min(kPairs, end - q.row);
-        for (q.from = 0; q.from < p.tokens; q.from += p.token_cap) {
-            q.tokens = min(p.token_cap, p.tokens - q.from);
+        for (q.from = 0; q.from < p.tokens; q.from += p.shared_cap) {
+            q.tokens = min(p.shared_cap, p.tokens - q.from);
             if (!f(q)) return false;
         }
     }
@@ -247,7 +247,7 @@ __device__ __forceinline__ void for_routed_pieces(const Decode& p, const Routing
 
 // ---- gate / up --------------------------------------------------------------------------------------------------------
 template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -359,9 +359,9 @@ __device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, i
     q.count = count;
     for (int a = p.shared_gate != nullptr ? -1 : 0; a < active; ++a) {
         q.expert = a < 0 ? -1 : r.active[a];
-        const int to = a < 0 ? p.tokens : r.begin[a + 1];
-        for (q.from = a < 0 ? 0 : r.begin[a]; q.from < to; q.from += p.token_cap) {
-            q.tokens = min(p.token_cap, to - q.from);
+        const int to = a < 0 ? p.tokens : r.begin[a + 1], cap = a < 0 ? p.shared_cap : p.token_cap;
+        for (q.from = a < 0 ? 0 : r.begin[a]; q.from < to; q.from += cap) {
+            q.tokens = min(cap, to - q.from);
             if (!f(q)) return false;
         }
     }
@@ -447,7 +447,7 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
 }
 
 template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const Decode p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -539,25 +539,34 @@ static_assert(sizeof(Bars) <= 384, "");
 // another SM has none, cost 40 us of 250) and the second what is left.
 constexpr int kGateUpBytes = kSmemPerSm / 2 - kStatic + 128, kDownBytes = kSmemPerSm - kGateUpBytes - 2 * kStatic;
 
-int stage_bytes(int tokens, bool w8) {   // the shared expert is bf16 in either case
-    const int a = Form<false, false>::stage_bytes(tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
+int stage_bytes(int tokens, int shared_tokens, bool w8) {   // the shared expert is bf16 in either case
+    const int a = Form<false, false>::stage_bytes(shared_tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
     return a > b ? a : b;
 }
 // Shared memory beside the ring.
 int gate_up_rest(const Decode& p, int nt) { return kDeposits * kConsumers * nt * 128 * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
 int down_rest(const Decode& p, int nt) { return gate_up_rest(p, nt) + p.tokens * kRows * 4; }
 
-// Tokens of a stage; 0: nothing fits.  The ring has 8 stages, so that every consumer keeps its own.  An expert that more tokens chose
-// is read more than once (from L2 after the first time), so few suffice where experts see few tokens, and then both kernels fit an SM;
-// with more tokens the stages take what they need.
-int token_cap(const Decode& p, bool w8) {
-    const int most = p.tokens < (w8 ? 4 : 6) ? p.tokens : w8 ? 4 : 6;
+// Tokens of a stage, and the bytes that follow from it; false: nothing fits.  The ring has 8 stages, so that every consumer keeps its
+// own.  An expert that more tokens chose is read more than once (from L2 after the first time), so few suffice where experts see few
+// tokens, and then both kernels fit an SM.  Beyond that the stages take what they need: the shared expert, which sees all tokens, has
+// 24 of them in one pass, and so have bf16 experts.
+bool plan(Decode& p, bool w8) {
+    p.stages = kConsumers;
+    const int few = w8 ? 4 : 6, most = p.tokens < few ? p.tokens : few;
     if (p.tokens <= (w8 ? 4 : 32))
-        for (int cap = most; cap >= (most < 4 ? most : 4); --cap)
-            if (kConsumers * stage_bytes(cap, w8) + gate_up_rest(p, 1) <= kGateUpBytes && kConsumers * stage_bytes(cap, w8) + down_rest(p, 1) <= kDownBytes) return cap;
-    for (int cap = w8 ? 8 : 16; cap >= 4; cap -= 4)
-        if (kConsumers * stage_bytes(cap, w8) + down_rest(p, cap > 8 ? 2 : 1) <= kSmemPerBlock - kStatic) return cap;
-    return 0;
+        for (int cap = most; cap >= (most < 4 ? most : 4); --cap) {
+            p.token_cap = p.shared_cap = cap;
+            p.stage_bytes = stage_bytes(cap, cap, w8);
+            if (kConsumers * p.stage_bytes + gate_up_rest(p, 1) <= kGateUpBytes && kConsumers * p.stage_bytes + down_rest(p, 1) <= kDownBytes) return true;
+        }
+    for (int cap = 24; cap >= 4; cap -= 4) {
+        p.shared_cap = cap;
+        p.token_cap = w8 ? (cap + 1) / 2 : cap;   // their tokens take twice the bytes of the weights
+        p.stage_bytes = stage_bytes(p.token_cap, cap, w8);
+        if (kConsumers * p.stage_bytes + down_rest(p, (cap + 7) / 8) <= kSmemPerBlock - kStatic) return true;
+    }
+    return false;
 }
 
 template <typename Kernel>
@@ -575,10 +584,8 @@ int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decod
 }
 
 template <bool W8, int NT>
-int run_decode(Decode p, cudaStream_t stream) {
+int run_decode(const Decode& p, cudaStream_t stream) {
     static int gate_up_ready[16] = {0}, down_ready[16] = {0};
-    p.stages = kConsumers;
-    p.stage_bytes = stage_bytes(p.token_cap, W8);
     const int ring = p.stages * p.stage_bytes, gate_up = ring + gate_up_rest(p, NT);
     MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, gate_up > kGateUpBytes ? gate_up : kGateUpBytes, stream));
     return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, p, ring + down_rest(p, NT), stream);
@@ -640,8 +647,8 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.clamp = has_limit;
     p.limit = limit;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    p.token_cap = token_cap(p, w8);
-    if (p.token_cap == 0) return MOK_ERR_TOO_LARGE;
-    if (w8) return run_decode<true, 1>(p, s);
-    return p.token_cap <= 8 ? run_decode<false, 1>(p, s) : run_decode<false, 2>(p, s);
+    if (!plan(p, w8)) return MOK_ERR_TOO_LARGE;
+    const int nt = (p.shared_cap + 7) / 8;
+    if (w8) return nt == 1 ? run_decode<true, 1>(p, s) : nt == 2 ? run_decode<true, 2>(p, s) : run_decode<true, 3>(p, s);
+    return nt == 1 ? run_decode<false, 1>(p, s) : nt == 2 ? run_decode<false, 2>(p, s) : run_decode<false, 3>(p, s);
 }
