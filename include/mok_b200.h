@@ -446,7 +446,7 @@ int mok_router_decode(const void* x, int64_t x_stride, const void* w, int w_is_f
  * num_experts) contribute nothing; an expert that a token names twice counts with both weights.  scratch:
  * mok_moe_decode_scratch_bytes().  `out` is NaN while the status word is not zero (see mok_fwd_epilogue).
  */
-int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int intermediate, int shared_intermediate);
+int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int hidden, int intermediate, int shared_intermediate, int fp8);
 int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* top_experts, const float* router_weights, int num_tokens, int topk,
                    int hidden, const void* w_shared_gate, const void* w_shared_up, const void* w_shared_down, int shared_intermediate,
                    const void* w_gate, const void* w_up, const void* w_down, const float* gate_scales, const float* up_scales,

@@ -13,6 +13,8 @@
 // hidden rows in hardware (programmatic dependent launch): no spinning, and nothing has to be co-resident for it to finish.
 // Every block finds out by itself which experts are in use and by whom, while its producers already copy the shared expert's
 // weights; hidden rows are kept by route number, so the order in which that happens does not matter.
+#include <cstdlib>
+
 #include "swiglu_math.cuh"
 #include "weight_stream.cuh"
 
@@ -36,10 +38,13 @@ struct Decode {
     const uint8_t *gate, *up, *down;
     const float *gate_scales, *up_scales, *down_scales;   // W8: [E, ceil(I / 128), ceil(H / 128)] and [E, ceil(H / 128), ceil(I / 128)]
     bf16 *hidden, *hidden_shared, *out;
+    __half* x_half;                       // W8: tokens and, in place, hidden rows as f16 with a power of two per row
+    float *x_scale, *hidden_scale;        // [tokens], [routes]
     uint32_t* status;
     int tokens, hidden_size, intermediate, shared_intermediate, experts, first_expert, topk;
     int clamp;
     float limit;
+    int blocks;   // per SM
     int stages, stage_bytes, token_cap, shared_cap;   // the ring; tokens of a stage, of routed experts and the shared one
 };
 
@@ -245,6 +250,57 @@ __device__ __forceinline__ void for_routed_pieces(const Decode& p, const Routing
     }
 }
 
+// ---- tokens for 8-bit weights -------------------------------------------------------------------------------------------
+// bf16 rows as f16 with a power of two per row that brings its largest finite value to [2^14, 2^15): eight bits of significand fit
+// eleven, values from 2^-28 of the largest on are exact and smaller ones are off by 2^-40 of it at most, far below the sums' fp32.
+// One block per row; `out` may be `rows` itself.  HIDDEN: rows of routes to other ranks' experts hold nothing and are passed over,
+// and the rows are the previous kernel's, which may still run.
+template <bool HIDDEN>
+__global__ void __launch_bounds__(256) to_half_kernel(const Decode p) {
+    __shared__ uint32_t part[8];
+    const int row = blockIdx.x, cols = HIDDEN ? p.intermediate : p.hidden_size;
+    const bf16* in = HIDDEN ? p.hidden + static_cast<long long>(row) * cols : p.x + row * p.x_stride;
+    uint4* out = HIDDEN ? reinterpret_cast<uint4*>(p.hidden + static_cast<long long>(row) * cols)
+                        : reinterpret_cast<uint4*>(p.x_half + static_cast<long long>(row) * cols);
+    if (HIDDEN) allow_next_kernel();   // the down kernel: it has weights to fetch meanwhile, and waits for this one
+    wait_previous_kernel();            // every block: who waits for this kernel has waited for the one before
+    if (HIDDEN) {
+        const uint32_t e = static_cast<uint32_t>(__ldcg(p.routes + row)) - static_cast<uint32_t>(p.first_expert);
+        if (e >= static_cast<uint32_t>(p.experts)) return;
+    } else {
+        allow_next_kernel();
+    }
+    uint32_t big = 0;
+    auto finite = [](uint32_t v) { return v < 0x7F80u ? v : 0u; };
+    for (int i = threadIdx.x; i < cols / 8; i += 256) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(in) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = max(big, max(finite(w[j] & 0x7FFFu), finite(w[j] >> 16 & 0x7FFFu)));
+    }
+    big = __reduce_max_sync(0xffffffffu, big);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = big;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) big = max(big, part[i]);
+    // biased exponent of the scale's reciprocal, 2^(14 - exponent); 1 .. 253 keeps both normal
+    const int k = min(max(127 + 14 - (static_cast<int>(big >> 7) - 127), 1), 253);
+    const float factor = __uint_as_float(static_cast<uint32_t>(k) << 23);
+    if (threadIdx.x == 0) (HIDDEN ? p.hidden_scale : p.x_scale)[row] = __uint_as_float(static_cast<uint32_t>(254 - k) << 23);
+    for (int i = threadIdx.x; i < cols / 8; i += 256) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(in) + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(w[j]);
+            const __half2 r = __floats2half2_rn(f.x * factor, f.y * factor);
+            h[j] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+        out[i] = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+}
+
 // ---- gate / up --------------------------------------------------------------------------------------------------------
 template <bool W8, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(const Decode p) {
@@ -267,6 +323,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
                 const int pair = i & (kPairs - 1), c = i / kPairs;
                 if (pair >= q.count) continue;
                 float g = sum_of<NT>(sums, slots, pair, c), u = sum_of<NT>(sums, slots, pair + 8, c);
+                if (W8 && q.expert >= 0) {
+                    const float scale = __ldcg(p.x_scale + r.token[q.from + c]);
+                    g *= scale;
+                    u *= scale;
+                }
                 if (p.clamp) {   // comparisons that let a NaN through
                     g = g > p.limit ? p.limit : g;
                     u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
@@ -293,10 +354,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
 #pragma unroll
             for (int j = 0; j < 8 * NT; ++j) {
                 f.token[j] = nullptr;
-                if (j < q.tokens) f.token[j] = reinterpret_cast<const uint8_t*>(p.x + (shared ? q.from + j : r.token[q.from + j]) * p.x_stride) + lane * 16;
+                if (j < q.tokens) {
+                    const int token = shared ? q.from + j : r.token[q.from + j];
+                    f.token[j] = (w8 ? reinterpret_cast<const uint8_t*>(p.x_half + static_cast<long long>(token) * p.hidden_size)
+                                     : reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride)) + lane * 16;
+                }
             }
-            const bool ok = w8 ? produce<Form<W8, false>>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, lane)
-                               : produce<Form<false, false>>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, lane);
+            f.scale = nullptr;
+            if (w8 && lane < kRows && (lane & 7) < q.count) {
+                const int blocks = (p.hidden_size + 127) / 128, row_blocks = (p.intermediate + 127) / 128;
+                f.scale = (lane < 8 ? p.gate_scales : p.up_scales) +
+                          (static_cast<long long>(q.expert) * row_blocks + (q.row + (lane & 7)) / 128) * blocks;
+                f.scale_stride = 1;
+            }
+            const bool ok = w8 ? produce<Form<W8, false>, false>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, p.token_cap, lane)
+                               : produce<Form<false, false>, false>(ring, &bars.abort_flag, p.status, f, turn, p.hidden_size, p.token_cap, lane);
             const int n = w8 ? chunks8 : chunks;
             turn = (turn - n) & (kProducers - 1);
             ring.next_piece(n);
@@ -315,19 +387,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
             if (slot < n) {
                 float acc[NT][4];
                 clear(acc);
-                Scales<false, NT> s;
-                if (w8) {
-                    const int blocks = (p.hidden_size + 127) / 128, row_blocks = (p.intermediate + 127) / 128;
-                    const int row = min(q.row + (lane >> 2), p.intermediate - 1);   // rows g and g + 8: gate and up of one pair
-                    const long long at = (static_cast<long long>(q.expert) * row_blocks + row / 128) * blocks;
-                    s.lo = p.gate_scales + at;
-                    s.hi = p.up_scales + at;
-                    s.row_block = 1;
-                    for (int c = slot; c < n; c += kConsumers)
-                        consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, s, lane, acc);
-                } else {
-                    for (int c = slot; c < n; c += kConsumers)
-                        consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, s, lane, acc);
+                for (int c = slot; c < n; c += kConsumers) {
+                    if (w8) consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
+                    else consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
                 }
                 deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
             }
@@ -381,6 +443,12 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
         f.low = (shared ? reinterpret_cast<const uint8_t*>(p.shared_down) : p.down) +
                 ((shared ? 0 : static_cast<long long>(q.expert) * p.hidden_size) + q.row) * f.row_bytes + lane * 16;
         f.high = f.low + 8 * f.row_bytes;
+        f.scale = nullptr;
+        if (W8 && !shared && lane < q.count) {
+            const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
+            f.scale = p.down_scales + (static_cast<long long>(q.expert) * row_blocks + (q.row + lane) / 128) * blocks;
+            f.scale_stride = 1;
+        }
     };
     auto tokens_of = [&](const Piece& q, Feed<CAP>& f) {
         const bool shared = q.expert < 0;
@@ -400,8 +468,11 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
         Feed<CAP> f;
         weights_of(q, f);
         for (int c = 0; c * F::kChunk < depth && met < start.stages; ++c, ++met)
-            if (met >= done && (met & (kProducers - 1)) == producer)
-                copy_weights<F>(start.base + met * start.stage_bytes, f, c * F::kChunk, min(F::kChunk, depth - c * F::kChunk), lane);
+            if (met >= done && (met & (kProducers - 1)) == producer) {
+                const int len = min(F::kChunk, depth - c * F::kChunk);
+                copy_weights<F>(start.base + met * start.stage_bytes, f, c * F::kChunk, len, lane);
+                if (F::kScales) copy_scales<F, false>(start.base + met * start.stage_bytes, f, c * F::kChunk, len, p.token_cap, lane);
+            }
         return met < start.stages;
     };
     auto early_pieces = [&](bool shared_only, int done) {
@@ -433,7 +504,7 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
             copy_tokens<F>(ring.base + (ring.at + c) * ring.stage_bytes, f, c * F::kChunk, min(F::kChunk, depth - c * F::kChunk), lane);
             arrive_when_copied(ring.full + 8 * (ring.at + c));
         }
-        const bool ok = produce<F>(ring, &bars.abort_flag, p.status, f, c, depth, lane);
+        const bool ok = produce<F, false>(ring, &bars.abort_flag, p.status, f, c, depth, p.token_cap, lane);
         turn = (turn - n) & (kProducers - 1);
         ring.next_piece(n);
         return ok;
@@ -484,7 +555,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
                 for (int k = lane; k < kRows * q.tokens; k += 32) {   // a token is listed once
                     const int row = k & (kRows - 1), c = k / kRows;
                     float* at = out + (q.expert < 0 ? q.from + c : r.token[q.from + c]) * kRows + row;
-                    *at = fmaf(q.expert < 0 ? 1.0f : r.weights[q.from + c], sum_of<NT>(sums, slots, row, c), *at);
+                    float v = sum_of<NT>(sums, slots, row, c);
+                    if (W8 && q.expert >= 0) v *= __ldcg(p.hidden_scale + r.list[q.from + c]);
+                    *at = fmaf(q.expert < 0 ? 1.0f : r.weights[q.from + c], v, *at);
                 }
                 collected(sums, bars, lane);
                 return true;
@@ -496,19 +569,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
                 if (slot < n) {
                     float acc[NT][4];
                     clear(acc);
-                    Scales<false, NT> s;
-                    if (w8) {
-                        const int blocks = (p.intermediate + 127) / 128, row_blocks = (p.hidden_size + 127) / 128;
-                        const int lo = min(q.row + (lane >> 2), p.hidden_size - 1), hi = min(lo + 8, p.hidden_size - 1);
-                        const long long at = static_cast<long long>(q.expert) * row_blocks;
-                        s.lo = p.down_scales + (at + lo / 128) * blocks;
-                        s.hi = p.down_scales + (at + hi / 128) * blocks;
-                        s.row_block = 1;
-                        for (int c = slot; c < n; c += kConsumers)
-                            consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
-                    } else {
-                        for (int c = slot; c < n; c += kConsumers)
-                            consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, s, lane, acc);
+                    for (int c = slot; c < n; c += kConsumers) {
+                        if (w8) consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
+                        else consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
                     }
                     deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
                 }
@@ -535,9 +598,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kStatic = 1024 + 384;   // reserved per block + barriers
 static_assert(sizeof(Bars) <= 384, "");
-// The two kernels share the SMs when the first takes a little more than half of the shared memory (two of its blocks on one SM, while
-// another SM has none, cost 40 us of 250) and the second what is left.
-constexpr int kGateUpBytes = kSmemPerSm / 2 - kStatic + 128, kDownBytes = kSmemPerSm - kGateUpBytes - 2 * kStatic;
+// Two blocks of a kernel share an SM when each takes half of the shared memory.
+constexpr int kHalf = kSmemPerSm / 2 - kStatic;
 
 int stage_bytes(int tokens, int shared_tokens, bool w8) {   // the shared expert is bf16 in either case
     const int a = Form<false, false>::stage_bytes(shared_tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
@@ -547,30 +609,29 @@ int stage_bytes(int tokens, int shared_tokens, bool w8) {   // the shared expert
 int gate_up_rest(const Decode& p, int nt) { return kDeposits * kConsumers * nt * 128 * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
 int down_rest(const Decode& p, int nt) { return gate_up_rest(p, nt) + p.tokens * kRows * 4; }
 
-// Tokens of a stage, and the bytes that follow from it; false: nothing fits.  The ring has 8 stages, so that every consumer keeps its
-// own.  An expert that more tokens chose is read more than once (from L2 after the first time), so few suffice where experts see few
-// tokens, and then both kernels fit an SM.  Beyond that the stages take what they need: the shared expert, which sees all tokens, has
-// 24 of them in one pass, and so have bf16 experts.
 bool plan(Decode& p, bool w8) {
     p.stages = kConsumers;
-    const int few = w8 ? 4 : 6, most = p.tokens < few ? p.tokens : few;
-    if (p.tokens <= (w8 ? 4 : 32))
-        for (int cap = most; cap >= (most < 4 ? most : 4); --cap) {
+    const char* pe = std::getenv("MOK_PAIR"), *ce = std::getenv("MOK_CAP");
+    const int few = ce ? std::atoi(ce) : w8 ? 3 : 6, most = p.tokens < few ? p.tokens : few;
+    if (pe ? std::atoi(pe) : p.tokens <= (w8 ? 16 : 32))
+        for (int cap = most; cap >= (most < 3 ? most : 3); --cap) {
             p.token_cap = p.shared_cap = cap;
             p.stage_bytes = stage_bytes(cap, cap, w8);
-            if (kConsumers * p.stage_bytes + gate_up_rest(p, 1) <= kGateUpBytes && kConsumers * p.stage_bytes + down_rest(p, 1) <= kDownBytes) return true;
+            p.blocks = 2;
+            if (kConsumers * p.stage_bytes + gate_up_rest(p, 1) <= kHalf && kConsumers * p.stage_bytes + down_rest(p, 1) <= kHalf) return true;
         }
     for (int cap = 24; cap >= 4; cap -= 4) {
         p.shared_cap = cap;
         p.token_cap = w8 ? (cap + 1) / 2 : cap;   // their tokens take twice the bytes of the weights
         p.stage_bytes = stage_bytes(p.token_cap, cap, w8);
+        p.blocks = 1;
         if (kConsumers * p.stage_bytes + down_rest(p, (cap + 7) / 8) <= kSmemPerBlock - kStatic) return true;
     }
     return false;
 }
 
 template <typename Kernel>
-int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decode& p, int smem, cudaStream_t stream) {
+int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decode& p, int blocks, int smem, cudaStream_t stream) {
     int dev = 0;
     MOK_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 16) return MOK_ERR_UNSUPPORTED;
@@ -580,15 +641,21 @@ int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decod
         MOK_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
         ready[dev] = 1;
     }
-    return launch_early(kernel, name, dim3(sm_count()), kThreads, smem, stream, p);
+    return launch_early(kernel, name, dim3(blocks * sm_count()), kThreads, smem, stream, p);
 }
 
 template <bool W8, int NT>
 int run_decode(const Decode& p, cudaStream_t stream) {
     static int gate_up_ready[16] = {0}, down_ready[16] = {0};
-    const int ring = p.stages * p.stage_bytes, gate_up = ring + gate_up_rest(p, NT);
-    MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, gate_up > kGateUpBytes ? gate_up : kGateUpBytes, stream));
-    return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, p, ring + down_rest(p, NT), stream);
+    const char* de = std::getenv("MOK_DOWN");
+    const int ring = p.stages * p.stage_bytes;
+    if (W8) MOK_TRY(launch_early(to_half_kernel<false>, "to_half_kernel", dim3(p.tokens), 256, 0, stream, p));
+    MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, p.blocks, ring + gate_up_rest(p, NT), stream));
+    if (W8) MOK_TRY(launch_early(to_half_kernel<true>, "to_half_kernel", dim3(p.tokens * p.topk), 256, 0, stream, p));
+    const int blocks = de ? std::atoi(de) : p.hidden_size >= 12 * 2 * sm_count() ? p.blocks : 1;
+    Decode q = p;
+    if (blocks == 1 && 16 * p.stage_bytes + down_rest(p, NT) <= kSmemPerBlock - kStatic && !std::getenv("MOK_S8")) q.stages = 16;
+    return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, q, blocks, q.stages * p.stage_bytes + down_rest(p, NT), stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -596,9 +663,11 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 }  // namespace mok
 
-extern "C" int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int intermediate, int shared_intermediate) {
-    if (num_tokens <= 0 || topk <= 0 || intermediate <= 0 || shared_intermediate < 0) return 0;
-    return 2 * (static_cast<int64_t>(num_tokens) * topk * intermediate + static_cast<int64_t>(num_tokens) * shared_intermediate);
+// hidden rows of the routes, of the shared expert; 8-bit experts: tokens in f16 and the scales
+extern "C" int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int hidden, int intermediate, int shared_intermediate, int fp8) {
+    if (num_tokens <= 0 || topk <= 0 || hidden <= 0 || intermediate <= 0 || shared_intermediate < 0) return 0;
+    const int64_t tokens = num_tokens, routes = tokens * topk;
+    return 2 * (routes * intermediate + tokens * shared_intermediate) + (fp8 ? 2 * tokens * hidden + 4 * (tokens + routes) : 0);
 }
 
 extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* top_experts, const float* router_weights, int num_tokens,
@@ -635,6 +704,9 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.down_scales = down_scales;
     p.hidden = static_cast<bf16*>(scratch);
     p.hidden_shared = p.hidden + static_cast<long long>(num_tokens) * topk * intermediate;
+    p.x_half = reinterpret_cast<__half*>(p.hidden_shared + static_cast<long long>(num_tokens) * shared_intermediate);
+    p.x_scale = reinterpret_cast<float*>(p.x_half + static_cast<long long>(num_tokens) * hidden);
+    p.hidden_scale = p.x_scale + num_tokens;
     p.out = static_cast<bf16*>(out);
     p.status = status;
     p.tokens = num_tokens;

@@ -38,7 +38,9 @@ constexpr int kRows = 16;                           // weight rows of a piece
 constexpr int kMaxStages = 16;
 constexpr int kDeposits = 2;
 
-// W8 / X8: weights / tokens in e4m3 instead of bf16.
+// W8: weights in e4m3 instead of bf16, and tokens in f16 (every code is an f16 number, one conversion per pair; as bf16 it takes
+// five operations a pair, all on the pipes of 64 lanes a clock, and 22 experts of 44 MB took 384 us instead of NEWTIME), or, X8, in
+// e4m3 too.
 template <bool W8, bool X8>
 struct Form {
     static constexpr int kChunk = W8 ? 512 : 256;               // elements of k per stage
@@ -46,12 +48,19 @@ struct Form {
     static constexpr int kRowPitch = kRowBytes + (W8 ? 32 : 64);
     static constexpr int kTokenBytes = kChunk * (X8 ? 1 : 2);
     static constexpr int kTokenPitch = kTokenBytes + (X8 ? 32 : 64);
-    static constexpr int stage_bytes(int tokens) { return kRows * kRowPitch + tokens * kTokenPitch; }
+    static constexpr int kBlocks = kChunk / 128;
+    static constexpr int kScales = W8 ? 4 * kBlocks * kRows : 0;   // bytes; one per row and 128 of k, then X8 one per token
+    // weight rows, their scales, token rows, their scales
+    static constexpr int stage_bytes(int tokens) { return kRows * kRowPitch + kScales + tokens * (kTokenPitch + (X8 ? 4 * kBlocks : 0)); }
+    static constexpr int kTokens = kRows * kRowPitch + kScales;
     __device__ static __forceinline__ int chunks(int k_total) { return (k_total + kChunk - 1) / kChunk; }
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // One arrival once every copy that this thread has issued so far is done.
 __device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
@@ -125,7 +134,22 @@ struct Feed {
     const uint8_t *low, *high, *token[CAP];
     long long row_bytes;
     int rows_low, rows_high;
+    // scales of this lane's row (lanes 0 .. 15; nullptr: none) and token, and the distance between blocks of k
+    const float *scale, *token_scale;
+    long long scale_stride, token_scale_stride;
 };
+// Consumers that fetched the scales themselves waited for them, some 600 clocks in every block of 128.
+template <typename F, bool X8, int CAP>
+__device__ __forceinline__ void copy_scales(uint32_t stage, const Feed<CAP>& f, int k0, int len, int token_cap, int lane) {
+    const int block0 = k0 / 128, blocks = (len + 127) / 128;
+#pragma unroll
+    for (int b = 0; b < F::kBlocks; ++b) {
+        if (b >= blocks) break;
+        if (f.scale != nullptr) copy4(stage + kRows * F::kRowPitch + (lane * F::kBlocks + b) * 4, f.scale + (block0 + b) * f.scale_stride);
+        if (X8 && f.token_scale != nullptr)
+            copy4(stage + F::kTokens + token_cap * F::kTokenPitch + (lane * F::kBlocks + b) * 4, f.token_scale + (block0 + b) * f.token_scale_stride);
+    }
+}
 template <typename F, int CAP>
 __device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kRowBytes / F::kChunk;
@@ -146,7 +170,7 @@ template <typename F, int CAP>
 __device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kTokenBytes / F::kChunk;
     const long long at = static_cast<long long>(k0) * kBytes;
-    const uint32_t dst = stage + kRows * F::kRowPitch + lane * 16;
+    const uint32_t dst = stage + F::kTokens + lane * 16;
 #pragma unroll
     for (int part = 0; part < F::kTokenBytes; part += 512)
         if (part + lane * 16 < len * kBytes) {
@@ -159,9 +183,9 @@ __device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<CAP>& f, 
 }
 // A producer's chunks of a piece, from chunk `first` on: those whose number in the whole sequence is `producer` modulo kProducers.
 // False: a wait ran out.
-template <typename F, int CAP>
+template <typename F, bool X8, int CAP>
 __device__ __forceinline__ bool produce(const Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed<CAP>& f, int first, int k_total,
-                                        int lane) {
+                                        int token_cap, int lane) {
     for (int c = first; c * F::kChunk < k_total; c += kProducers) {
         uint32_t parity;
         const int s = ring.stage(c, parity);
@@ -169,6 +193,7 @@ __device__ __forceinline__ bool produce(const Ring& ring, volatile int* abort_fl
         const int k0 = c * F::kChunk, len = min(F::kChunk, k_total - k0);
         const uint32_t stage = ring.base + s * ring.stage_bytes;
         copy_weights<F>(stage, f, k0, len, lane);
+        if (F::kScales) copy_scales<F, X8>(stage, f, k0, len, token_cap, lane);
         copy_tokens<F>(stage, f, k0, len, lane);
         arrive_when_copied(ring.full + 8 * s);
     }
@@ -191,14 +216,6 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_codes) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two_codes)));
     return h;
 }
-// Two e4m3 codes as bf16 (exact, NaN stays NaN) by way of f16 and fp32.  Moving the bits into place and multiplying by 2^120 was
-// measured too: 560 instead of 355 us for 22 experts of 44 MB.
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t two_codes) {
-    const uint32_t h = e4m3x2_to_f16x2(two_codes);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    return pack_bf16x2(f.x, f.y);
-}
-
 // The first `count` (may be <= 0) of eight codes, the others zero.
 __device__ __forceinline__ uint2 keep_codes(uint2 v, int count) {
     if (count < 8) v.y = count > 4 ? v.y & (0xFFFFFFFFu >> (8 * (8 - count))) : 0u;
@@ -215,25 +232,20 @@ __device__ __forceinline__ void clear(float (&acc)[NT][4]) {
 }
 
 // acc += 32 elements of k from element `k` of a stage on (of this lane: k + 8 t .. k + 8 t + 7).  `left`: valid elements from k on
-// (X8; the others hold multiples of 32).  `tiles`: n tiles in use.
-template <bool W8, bool X8, int NT>
-__device__ __forceinline__ void multiply_slice(const uint8_t* weights, const uint8_t* tokens, int k, int left, int tiles, int t, float (&acc)[NT][4]) {
+// (X8; the others hold multiples of 32).
+template <bool W8, bool X8, int TILES, int NT>
+__device__ __forceinline__ void multiply_slice(const uint8_t* weights, const uint8_t* tokens, int k, int left, int t, float (&acc)[NT][4]) {
     typedef Form<W8, X8> F;
     uint32_t lo[4], hi[4];
     if (W8) {
         uint2 l = *reinterpret_cast<const uint2*>(weights + k);
         uint2 h = *reinterpret_cast<const uint2*>(weights + 8 * F::kRowPitch + k);
-        if (X8) {
-            if (left < 32) {
-                l = keep_codes(l, left - 8 * t);
-                h = keep_codes(h, left - 8 * t);
-            }
-            lo[0] = e4m3x2_to_f16x2(l.x); lo[1] = e4m3x2_to_f16x2(l.x >> 16); lo[2] = e4m3x2_to_f16x2(l.y); lo[3] = e4m3x2_to_f16x2(l.y >> 16);
-            hi[0] = e4m3x2_to_f16x2(h.x); hi[1] = e4m3x2_to_f16x2(h.x >> 16); hi[2] = e4m3x2_to_f16x2(h.y); hi[3] = e4m3x2_to_f16x2(h.y >> 16);
-        } else {
-            lo[0] = e4m3x2_to_bf16x2(l.x); lo[1] = e4m3x2_to_bf16x2(l.x >> 16); lo[2] = e4m3x2_to_bf16x2(l.y); lo[3] = e4m3x2_to_bf16x2(l.y >> 16);
-            hi[0] = e4m3x2_to_bf16x2(h.x); hi[1] = e4m3x2_to_bf16x2(h.x >> 16); hi[2] = e4m3x2_to_bf16x2(h.y); hi[3] = e4m3x2_to_bf16x2(h.y >> 16);
+        if (X8 && left < 32) {
+            l = keep_codes(l, left - 8 * t);
+            h = keep_codes(h, left - 8 * t);
         }
+        lo[0] = e4m3x2_to_f16x2(l.x); lo[1] = e4m3x2_to_f16x2(l.x >> 16); lo[2] = e4m3x2_to_f16x2(l.y); lo[3] = e4m3x2_to_f16x2(l.y >> 16);
+        hi[0] = e4m3x2_to_f16x2(h.x); hi[1] = e4m3x2_to_f16x2(h.x >> 16); hi[2] = e4m3x2_to_f16x2(h.y); hi[3] = e4m3x2_to_f16x2(h.y >> 16);
     } else {
         const uint4 l = *reinterpret_cast<const uint4*>(weights + k * 2);
         const uint4 h = *reinterpret_cast<const uint4*>(weights + 8 * F::kRowPitch + k * 2);
@@ -241,8 +253,7 @@ __device__ __forceinline__ void multiply_slice(const uint8_t* weights, const uin
         hi[0] = h.x; hi[1] = h.y; hi[2] = h.z; hi[3] = h.w;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        if (n >= tiles) break;
+    for (int n = 0; n < TILES; ++n) {
         uint32_t b[4];
         if (X8) {
             uint2 v = *reinterpret_cast<const uint2*>(tokens + n * 8 * F::kTokenPitch + k);
@@ -252,48 +263,23 @@ __device__ __forceinline__ void multiply_slice(const uint8_t* weights, const uin
             mma_f16(acc[n], lo[2], hi[2], lo[3], hi[3], b[2], b[3]);
         } else {
             const uint4 v = *reinterpret_cast<const uint4*>(tokens + n * 8 * F::kTokenPitch + k * 2);
-            mma_bf16(acc[n], lo[0], hi[0], lo[1], hi[1], v.x, v.y);
-            mma_bf16(acc[n], lo[2], hi[2], lo[3], hi[3], v.z, v.w);
+            if (W8) {
+                mma_f16(acc[n], lo[0], hi[0], lo[1], hi[1], v.x, v.y);
+                mma_f16(acc[n], lo[2], hi[2], lo[3], hi[3], v.z, v.w);
+            } else {
+                mma_bf16(acc[n], lo[0], hi[0], lo[1], hi[1], v.x, v.y);
+                mma_bf16(acc[n], lo[2], hi[2], lo[3], hi[3], v.z, v.w);
+            }
         }
     }
 }
 
-// Scales of a lane's rows (g and g + 8) and, X8, of its tokens (2 t and 2 t + 1 of each n tile), one per 128 of k.
-template <bool X8, int NT>
-struct Scales {
-    const float *lo, *hi, *x[X8 ? NT : 1][2];
-    long long row_block, x_block;   // elements from one block of k to the next
-};
-
-// Waits for a chunk and adds its products to acc.  A wait that runs out is reported in the status word and the warp goes on with what
-// is there, so that every warp still meets the same barriers.
-template <bool W8, bool X8, int NT>
-__device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages, volatile int* abort_flag, uint32_t* status, int c, int k_total, int tiles,
-                                        const Scales<X8, NT>& scales, int lane, float (&acc)[NT][4]) {
+// acc += a chunk, block of 128 by block.  Whole blocks are one run of code for a number of n tiles known to the compiler: with a
+// condition on it in every slice nothing overlapped, 200 clocks a slice.
+template <bool W8, bool X8, int TILES, int NT>
+__device__ __forceinline__ void multiply_chunk(const uint8_t* weights, const uint8_t* tokens, const float* scales, const float* token_scales, int len,
+                                               int t, float (&acc)[NT][4]) {
     typedef Form<W8, X8> F;
-    const int g = lane >> 2, t = lane & 3;
-    const int len = min(F::kChunk, k_total - c * F::kChunk);
-    const int block0 = c * (F::kChunk / 128);
-    float lo = 0.0f, hi = 0.0f, x[X8 ? NT : 1][2];
-    auto fetch = [&](int b) {
-        lo = __ldg(scales.lo + (block0 + b) * scales.row_block);
-        hi = __ldg(scales.hi + (block0 + b) * scales.row_block);
-        if (X8) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                if (n < tiles) {
-                    x[n][0] = __ldg(scales.x[n][0] + (block0 + b) * scales.x_block);
-                    x[n][1] = __ldg(scales.x[n][1] + (block0 + b) * scales.x_block);
-                }
-        }
-    };
-    if (W8) fetch(0);
-    uint32_t parity;
-    const int s = ring.stage(c, parity);
-    mbar_wait(ring.full + 8 * s, parity, abort_flag, status);
-    const uint8_t* weights = stages + s * ring.stage_bytes + g * F::kRowPitch;
-    const uint8_t* tokens = stages + s * ring.stage_bytes + kRows * F::kRowPitch + g * F::kTokenPitch;
-    // blocks of 128: whole ones without a condition in between, so that their loads and conversions overlap
 #pragma unroll 1
     for (int b = 0; b * 128 < len; ++b) {
         float part[NT][4];
@@ -302,30 +288,44 @@ __device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages,
         const int left = len - b * 128, k0 = b * 128 + 8 * t;
         if (left >= 128) {
 #pragma unroll
-            for (int k = 0; k < 128; k += 32) multiply_slice<W8, X8, NT>(weights, tokens, k0 + k, 32, tiles, t, to);
+            for (int k = 0; k < 128; k += 32) multiply_slice<W8, X8, TILES, NT>(weights, tokens, k0 + k, 32, t, to);
         } else {
 #pragma unroll 1
-            for (int k = 0; k < left; k += 32) multiply_slice<W8, X8, NT>(weights, tokens, k0 + k, left - k, tiles, t, to);
+            for (int k = 0; k < left; k += 32) multiply_slice<W8, X8, TILES, NT>(weights, tokens, k0 + k, left - k, t, to);
         }
         if (W8) {
-            const float lo0 = lo, hi0 = hi;
-            float x0[X8 ? NT : 1][2];
-            if (X8) {
+            const float lo = scales[b], hi = scales[8 * F::kBlocks + b];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) x0[n][0] = x[n][0], x0[n][1] = x[n][1];
-            }
-            if (left > 128) fetch(b + 1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (n >= tiles) break;
-                const int m = X8 ? n : 0;
-                acc[n][0] = fmaf(part[n][0], X8 ? lo0 * x0[m][0] : lo0, acc[n][0]);
-                acc[n][1] = fmaf(part[n][1], X8 ? lo0 * x0[m][1] : lo0, acc[n][1]);
-                acc[n][2] = fmaf(part[n][2], X8 ? hi0 * x0[m][0] : hi0, acc[n][2]);
-                acc[n][3] = fmaf(part[n][3], X8 ? hi0 * x0[m][1] : hi0, acc[n][3]);
+            for (int n = 0; n < TILES; ++n) {
+                const float x0 = X8 ? token_scales[n * 8 * F::kBlocks + b] : 1.0f, x1 = X8 ? token_scales[(n * 8 + 1) * F::kBlocks + b] : 1.0f;
+                acc[n][0] = fmaf(part[n][0], X8 ? lo * x0 : lo, acc[n][0]);
+                acc[n][1] = fmaf(part[n][1], X8 ? lo * x1 : lo, acc[n][1]);
+                acc[n][2] = fmaf(part[n][2], X8 ? hi * x0 : hi, acc[n][2]);
+                acc[n][3] = fmaf(part[n][3], X8 ? hi * x1 : hi, acc[n][3]);
             }
         }
     }
+}
+
+// Waits for a chunk and adds its products to acc.  A wait that runs out is reported in the status word and the warp goes on with what
+// is there, so that every warp still meets the same barriers.
+template <bool W8, bool X8, int NT>
+__device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages, volatile int* abort_flag, uint32_t* status, int c, int k_total, int tiles,
+                                        int token_cap, int lane, float (&acc)[NT][4]) {
+    typedef Form<W8, X8> F;
+    const int g = lane >> 2, t = lane & 3;
+    const int len = min(F::kChunk, k_total - c * F::kChunk);
+    uint32_t parity;
+    const int s = ring.stage(c, parity);
+    mbar_wait(ring.full + 8 * s, parity, abort_flag, status);
+    const uint8_t* stage = stages + s * ring.stage_bytes;
+    const uint8_t* weights = stage + g * F::kRowPitch;
+    const uint8_t* tokens = stage + F::kTokens + g * F::kTokenPitch;
+    const float* scales = reinterpret_cast<const float*>(stage + kRows * F::kRowPitch) + g * F::kBlocks;
+    const float* token_scales = reinterpret_cast<const float*>(stage + F::kTokens + token_cap * F::kTokenPitch) + 2 * t * F::kBlocks;
+    if (NT == 1 || tiles == 1) multiply_chunk<W8, X8, 1, NT>(weights, tokens, scales, token_scales, len, t, acc);
+    else if (NT == 2 || tiles == 2) multiply_chunk<W8, X8, NT < 2 ? NT : 2, NT>(weights, tokens, scales, token_scales, len, t, acc);
+    else multiply_chunk<W8, X8, NT, NT>(weights, tokens, scales, token_scales, len, t, acc);
     __syncwarp();
     if (lane == 0) mbar_arrive(ring.empty + 8 * s);
 }

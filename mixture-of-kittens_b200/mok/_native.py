@@ -128,7 +128,7 @@ def lib() -> ctypes.CDLL:
                                        c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
         L.mok_router_decode.argtypes = [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                         c_void_p, c_void_p]
-        L.mok_moe_decode_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int]
+        L.mok_moe_decode_scratch_bytes.argtypes = [c_int] * 6
         L.mok_moe_decode.argtypes = ([c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int]
                                      + [c_void_p] * 6 + [c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
         for name in ("mok_rms_norm_scratch_bytes", "mok_block_matmul_scratch_bytes", "mok_moe_decode_scratch_bytes"):

@@ -21,7 +21,9 @@ def test_layer_entry_point_refuses():
         assert call(**bad) == -1, bad
     for large in (dict(T=257), dict(K=33), dict(T=256, K=17), dict(E=1025)):
         assert call(**large) == -4, large
-    assert L.mok_moe_decode_scratch_bytes(4, 2, 128, 64) == 2 * (4 * 2 * 128 + 4 * 64) and L.mok_moe_decode_scratch_bytes(0, 2, 128, 64) == 0
+    assert L.mok_moe_decode_scratch_bytes(4, 2, 256, 128, 64, 0) == 2 * (4 * 2 * 128 + 4 * 64)
+    assert L.mok_moe_decode_scratch_bytes(4, 2, 256, 128, 64, 1) == 2 * (4 * 2 * 128 + 4 * 64) + 2 * 4 * 256 + 4 * (4 + 8)
+    assert L.mok_moe_decode_scratch_bytes(0, 2, 256, 128, 64, 0) == 0
 
 
 def test_router_entry_point_refuses():
