@@ -9,12 +9,11 @@
 //              partial rows.  One warp adds the experts' parts while the others are at the next experts: when the whole block met for
 //              every expert, 2000 of 2500 clocks an expert were latency (hidden 2048, intermediate 768).
 //
-// The second kernel is launched while the first runs, next to it on each SM, fills its ring with down weights and waits for the
-// hidden rows in hardware (programmatic dependent launch): no spinning, and nothing has to be co-resident for it to finish.
+// The second kernel is launched while the first runs, takes an SM's place as soon as there is room, fills its ring with down weights
+// and waits for the hidden rows in hardware (programmatic dependent launch): no spinning, and nothing has to be co-resident for it to
+// finish.
 // Every block finds out by itself which experts are in use and by whom, while its producers already copy the shared expert's
 // weights; hidden rows are kept by route number, so the order in which that happens does not matter.
-#include <cstdlib>
-
 #include "swiglu_math.cuh"
 #include "weight_stream.cuh"
 
@@ -345,21 +344,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
         int turn = warp - kConsumers;   // this producer's next chunk, counted from the piece's first
         auto run = [&](const Piece& q) {
             const bool shared = q.expert < 0, w8 = W8 && !shared;
-            Feed<8 * NT> f;
+            Feed f;
             f.row_bytes = p.hidden_size * (w8 ? 1 : 2);
             f.rows_low = f.rows_high = q.count;
             const long long at = ((shared ? 0 : static_cast<long long>(q.expert) * p.intermediate) + q.row) * f.row_bytes + lane * 16;
             f.low = (shared ? reinterpret_cast<const uint8_t*>(p.shared_gate) : p.gate) + at;
             f.high = (shared ? reinterpret_cast<const uint8_t*>(p.shared_up) : p.up) + at;
-#pragma unroll
-            for (int j = 0; j < 8 * NT; ++j) {
-                f.token[j] = nullptr;
-                if (j < q.tokens) {
-                    const int token = shared ? q.from + j : r.token[q.from + j];
-                    f.token[j] = (w8 ? reinterpret_cast<const uint8_t*>(p.x_half + static_cast<long long>(token) * p.hidden_size)
-                                     : reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride)) + lane * 16;
-                }
-            }
+            f.tokens = q.tokens;
+            const int token = shared ? q.from + lane : lane < q.tokens ? r.token[q.from + lane] : 0;
+            f.token = w8 ? reinterpret_cast<const uint8_t*>(p.x_half + static_cast<long long>(token) * p.hidden_size)
+                         : reinterpret_cast<const uint8_t*>(p.x + token * p.x_stride);
             f.scale = nullptr;
             if (w8 && lane < kRows && (lane & 7) < q.count) {
                 const int blocks = (p.hidden_size + 127) / 128, row_blocks = (p.intermediate + 127) / 128;
@@ -431,11 +425,10 @@ __device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, i
 }
 
 // The producers.  Until the gate / up kernel is done the stages of the empty ring get their weights only; the hidden rows follow.
-template <bool W8, int NT>
+template <bool W8>
 __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, const Slice& slice, const Ring& start, Bars& bars, int producer, int lane) {
-    constexpr int CAP = 8 * NT;
     auto depth_of = [&](const Piece& q) { return q.expert < 0 ? p.shared_intermediate : p.intermediate; };
-    auto weights_of = [&](const Piece& q, Feed<CAP>& f) {
+    auto weights_of = [&](const Piece& q, Feed& f) {
         const bool shared = q.expert < 0;
         f.row_bytes = depth_of(q) * (W8 && !shared ? 1 : 2);
         f.rows_low = q.count;
@@ -450,22 +443,18 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
             f.scale_stride = 1;
         }
     };
-    auto tokens_of = [&](const Piece& q, Feed<CAP>& f) {
+    auto tokens_of = [&](const Piece& q, Feed& f) {
         const bool shared = q.expert < 0;
-        const bf16* h = shared ? p.hidden_shared : p.hidden;
-#pragma unroll
-        for (int j = 0; j < CAP; ++j) {
-            f.token[j] = nullptr;
-            if (j < q.tokens)
-                f.token[j] = reinterpret_cast<const uint8_t*>(h + static_cast<long long>(shared ? q.from + j : r.list[q.from + j]) * depth_of(q)) + lane * 16;
-        }
+        const int row = shared ? q.from + lane : lane < q.tokens ? r.list[q.from + lane] : 0;
+        f.tokens = q.tokens;
+        f.token = reinterpret_cast<const uint8_t*>((shared ? p.hidden_shared : p.hidden) + static_cast<long long>(row) * depth_of(q));
     };
     // this producer's chunks among the first `stages` of the sequence, from chunk number `done` on
     int met = 0;
     auto early = [&](const Piece& q, int done, auto form) {
         typedef decltype(form) F;
         const int depth = depth_of(q);
-        Feed<CAP> f;
+        Feed f;
         weights_of(q, f);
         for (int c = 0; c * F::kChunk < depth && met < start.stages; ++c, ++met)
             if (met >= done && (met & (kProducers - 1)) == producer) {
@@ -496,7 +485,7 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
     auto rest = [&](const Piece& q, auto form) {
         typedef decltype(form) F;
         const int depth = depth_of(q), n = F::chunks(depth);
-        Feed<CAP> f;
+        Feed f;
         weights_of(q, f);
         tokens_of(q, f);
         int c = turn;
@@ -530,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
     const int values = p.tokens * kRows;
     const Routing r = carve_routing(reinterpret_cast<uint8_t*>(out + values), p.experts, p.tokens * p.topk);
     if (warp >= kConsumers && warp != kFinisher) {
-        produce_down<W8, NT>(p, r, slice, ring, bars, warp - kConsumers, lane);
+        produce_down<W8>(p, r, slice, ring, bars, warp - kConsumers, lane);
         return;
     }
     auto depth_of = [&](const Piece& q) { return q.expert < 0 ? p.shared_intermediate : p.intermediate; };
@@ -609,17 +598,26 @@ int stage_bytes(int tokens, int shared_tokens, bool w8) {   // the shared expert
 int gate_up_rest(const Decode& p, int nt) { return kDeposits * kConsumers * nt * 128 * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
 int down_rest(const Decode& p, int nt) { return gate_up_rest(p, nt) + p.tokens * kRows * 4; }
 
+// Blocks per SM, tokens of a stage, and the bytes that follow from it; false: nothing fits.  The ring has 8 stages, so that every
+// consumer keeps its own.  Two blocks of few tokens an SM hide each other's latency: hidden 4096, 8 experts of 14336, 4 tokens 370 ->
+// 327 us.  But an expert that more tokens chose is read more than once (from L2 after the first time), and the shared one sees
+// them all; one block has room for 24 tokens (bf16, shared) or 12.  bf16, two blocks against one, us:
+//                         4        8       16       32       64 tokens
+//   128 experts, K 8   73/95  112/142  165/210  222/275  288/349    (hidden 2048, experts of 768)
+//   32 of 256, K 8    95/116  108/120  169/187  380/419  536/560    (hidden 7168, experts of 2048)
+//   8 experts, K 2   327/370  462/489  593/605  949/771  1500/1240
+// 8-bit: 8 tokens 98/102, 100/106, 344/366; 16 tokens 141/147, 156/153, 622/449.
 bool plan(Decode& p, bool w8) {
     p.stages = kConsumers;
-    const char* pe = std::getenv("MOK_PAIR"), *ce = std::getenv("MOK_CAP");
-    const int few = ce ? std::atoi(ce) : w8 ? 3 : 6, most = p.tokens < few ? p.tokens : few;
-    if (pe ? std::atoi(pe) : p.tokens <= (w8 ? 16 : 32))
-        for (int cap = most; cap >= (most < 3 ? most : 3); --cap) {
-            p.token_cap = p.shared_cap = cap;
-            p.stage_bytes = stage_bytes(cap, cap, w8);
-            p.blocks = 2;
-            if (kConsumers * p.stage_bytes + gate_up_rest(p, 1) <= kHalf && kConsumers * p.stage_bytes + down_rest(p, 1) <= kHalf) return true;
-        }
+    const int few = w8 ? 3 : 6;
+    const bool pair = w8 ? p.tokens <= 8 : p.tokens <= 16 || (p.tokens <= 64 && p.experts >= 32);
+    for (int cap = p.tokens < few ? p.tokens : few; pair && cap > 0; --cap) {
+        p.token_cap = p.shared_cap = cap;
+        p.stage_bytes = stage_bytes(cap, cap, w8);
+        p.blocks = 2;
+        if (kConsumers * p.stage_bytes + down_rest(p, 1) <= kHalf) return true;
+        if (cap <= few / 2) break;   // large routing tables
+    }
     for (int cap = 24; cap >= 4; cap -= 4) {
         p.shared_cap = cap;
         p.token_cap = w8 ? (cap + 1) / 2 : cap;   // their tokens take twice the bytes of the weights
@@ -647,14 +645,15 @@ int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decod
 template <bool W8, int NT>
 int run_decode(const Decode& p, cudaStream_t stream) {
     static int gate_up_ready[16] = {0}, down_ready[16] = {0};
-    const char* de = std::getenv("MOK_DOWN");
     const int ring = p.stages * p.stage_bytes;
     if (W8) MOK_TRY(launch_early(to_half_kernel<false>, "to_half_kernel", dim3(p.tokens), 256, 0, stream, p));
     MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, p.blocks, ring + gate_up_rest(p, NT), stream));
     if (W8) MOK_TRY(launch_early(to_half_kernel<true>, "to_half_kernel", dim3(p.tokens * p.topk), 256, 0, stream, p));
-    const int blocks = de ? std::atoi(de) : p.hidden_size >= 12 * 2 * sm_count() ? p.blocks : 1;
+    // Two blocks an SM where each has 12 of the output's columns or more, else one with twice the stages if they fit: hidden 2048, 32
+    // tokens of 128 experts 222 instead of 255 us; hidden 7168, 32 of 256 experts, 380 instead of 411 us.
+    const int blocks = p.hidden_size >= 12 * 2 * sm_count() ? p.blocks : 1;
     Decode q = p;
-    if (blocks == 1 && 16 * p.stage_bytes + down_rest(p, NT) <= kSmemPerBlock - kStatic && !std::getenv("MOK_S8")) q.stages = 16;
+    if (blocks == 1 && 2 * kConsumers * p.stage_bytes + down_rest(p, NT) <= kSmemPerBlock - kStatic) q.stages = 2 * kConsumers;
     return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, q, blocks, q.stages * p.stage_bytes + down_rest(p, NT), stream);
 }
 

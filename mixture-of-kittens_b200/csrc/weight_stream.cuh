@@ -39,7 +39,7 @@ constexpr int kMaxStages = 16;
 constexpr int kDeposits = 2;
 
 // W8: weights in e4m3 instead of bf16, and tokens in f16 (every code is an f16 number, one conversion per pair; as bf16 it takes
-// five operations a pair, all on the pipes of 64 lanes a clock, and 22 experts of 44 MB took 384 us instead of NEWTIME), or, X8, in
+// five operations a pair, all on the pipes of 64 lanes a clock, and 22 experts of 44 MB took 384 us instead of 351), or, X8, in
 // e4m3 too.
 template <bool W8, bool X8>
 struct Form {
@@ -126,21 +126,21 @@ __device__ __forceinline__ Ring set_up_ring(Bars& bars, const uint8_t* smem, int
 }
 
 // ---- producer -----------------------------------------------------------------------------------------------------
-// Rows of a piece as a producer copies them, this lane's 16 bytes of each at k = 0.  Weights: rows 0 .. 7 from low and rows 8 .. 15
-// from high, row_bytes apart, `rows_low` and `rows_high` of them (the others stay as they are and are not used).  Found once per
-// piece: with addresses worked out chunk by chunk the producers were the bottleneck (1500 clocks a chunk, 2.2 TB/s).
-template <int CAP>
+// Rows of a piece as a producer copies them.  Weights: rows 0 .. 7 from low and rows 8 .. 15 from high (this lane's 16 bytes at k = 0),
+// row_bytes apart, `rows_low` and `rows_high` of them (the others stay as they are and are not used).  Tokens: lane j holds the address
+// of row j.  Found once per piece: with addresses worked out chunk by chunk the producers were the bottleneck (1500 clocks a chunk,
+// 2.2 TB/s), and with every lane holding all token addresses they were at 24 tokens.
 struct Feed {
-    const uint8_t *low, *high, *token[CAP];
+    const uint8_t *low, *high, *token;
     long long row_bytes;
-    int rows_low, rows_high;
+    int rows_low, rows_high, tokens;
     // scales of this lane's row (lanes 0 .. 15; nullptr: none) and token, and the distance between blocks of k
     const float *scale, *token_scale;
     long long scale_stride, token_scale_stride;
 };
 // Consumers that fetched the scales themselves waited for them, some 600 clocks in every block of 128.
-template <typename F, bool X8, int CAP>
-__device__ __forceinline__ void copy_scales(uint32_t stage, const Feed<CAP>& f, int k0, int len, int token_cap, int lane) {
+template <typename F, bool X8>
+__device__ __forceinline__ void copy_scales(uint32_t stage, const Feed& f, int k0, int len, int token_cap, int lane) {
     const int block0 = k0 / 128, blocks = (len + 127) / 128;
 #pragma unroll
     for (int b = 0; b < F::kBlocks; ++b) {
@@ -150,8 +150,8 @@ __device__ __forceinline__ void copy_scales(uint32_t stage, const Feed<CAP>& f, 
             copy4(stage + F::kTokens + token_cap * F::kTokenPitch + (lane * F::kBlocks + b) * 4, f.token_scale + (block0 + b) * f.token_scale_stride);
     }
 }
-template <typename F, int CAP>
-__device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
+template <typename F>
+__device__ __forceinline__ void copy_weights(uint32_t stage, const Feed& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kRowBytes / F::kChunk;
     static_assert(F::kRowBytes == 512, "");
     if (lane * 16 >= len * kBytes) return;
@@ -166,25 +166,25 @@ __device__ __forceinline__ void copy_weights(uint32_t stage, const Feed<CAP>& f,
         high += f.row_bytes;
     }
 }
-template <typename F, int CAP>
-__device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed<CAP>& f, int k0, int len, int lane) {
+template <typename F>
+__device__ __forceinline__ void copy_tokens(uint32_t stage, const Feed& f, int k0, int len, int lane) {
     constexpr int kBytes = F::kTokenBytes / F::kChunk;
-    const long long at = static_cast<long long>(k0) * kBytes;
-    const uint32_t dst = stage + F::kTokens + lane * 16;
+    const int bytes = len * kBytes;
+    uint32_t dst = stage + F::kTokens + lane * 16;
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(f.token) + static_cast<long long>(k0) * kBytes;
+#pragma unroll 2
+    for (int j = 0; j < f.tokens; ++j) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, mine, j)) + lane * 16;
 #pragma unroll
-    for (int part = 0; part < F::kTokenBytes; part += 512)
-        if (part + lane * 16 < len * kBytes) {
-#pragma unroll
-            for (int j = 0; j < CAP; ++j) {
-                if (f.token[j] == nullptr) break;   // tokens come without gaps
-                copy16(dst + j * F::kTokenPitch + part, f.token[j] + at + part);
-            }
-        }
+        for (int part = 0; part < F::kTokenBytes; part += 512)
+            if (part + lane * 16 < bytes) copy16(dst + part, row + part);
+        dst += F::kTokenPitch;
+    }
 }
 // A producer's chunks of a piece, from chunk `first` on: those whose number in the whole sequence is `producer` modulo kProducers.
 // False: a wait ran out.
-template <typename F, bool X8, int CAP>
-__device__ __forceinline__ bool produce(const Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed<CAP>& f, int first, int k_total,
+template <typename F, bool X8>
+__device__ __forceinline__ bool produce(const Ring& ring, volatile int* abort_flag, uint32_t* status, const Feed& f, int first, int k_total,
                                         int token_cap, int lane) {
     for (int c = first; c * F::kChunk < k_total; c += kProducers) {
         uint32_t parity;
