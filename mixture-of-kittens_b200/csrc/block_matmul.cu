@@ -9,6 +9,7 @@
 //
 // Few tiles (a short grid and a long K): the blocks along K are cut into `splits` shares, every share writes its fp32 sums, and
 // a second kernel adds them in order.
+#include "block_matmul.cuh"
 #include "block_scale.cuh"
 #include "gemm_tiles.cuh"
 
@@ -392,6 +393,7 @@ int shares(int tiles, int k_blocks) {
 }
 
 int plan_splits(long long rows, int cols, int depth) {
+    if (rows <= kFewRows) return 1;
     return shares(div_up(rows, BM) * div_up(cols, BN), div_up(depth, BK));
 }
 
@@ -416,6 +418,13 @@ extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_
     if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) != 0 || a_stride % 16 != 0 || b_stride % 16 != 0 ||
         a_stride < depth || b_stride < depth || out_stride < cols)
         return MOK_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (rows <= kFewRows) {
+        const BlockProduct few{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), a_stride, b_stride, a_scales, b_scales,
+                               a_scale_row_stride, a_scale_block_stride, b_scale_row_stride, b_scale_block_stride, b_tile_rows,
+                               static_cast<int>(rows), cols, depth, static_cast<bf16*>(out), out_stride, status};
+        return launch_block_matmul_few(few, s);
+    }
     Product p{};
     p.sa = a_scales;
     p.sa_row = a_scale_row_stride;
@@ -438,7 +447,6 @@ extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_
     CUtensorMap map_a, map_b;
     MOK_TRY(code_map(&map_a, a, a_stride, rows, depth));
     MOK_TRY(code_map(&map_b, b, b_stride, cols, depth));
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int tiles = p.m_tiles * p.n_tiles * p.splits;
     if (b_tile_rows == 1) {
         static int resident[16] = {0};

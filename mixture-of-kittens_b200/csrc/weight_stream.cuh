@@ -325,6 +325,7 @@ __device__ __forceinline__ void consume(const Ring& ring, const uint8_t* stages,
     const float* token_scales = reinterpret_cast<const float*>(stage + F::kTokens + token_cap * F::kTokenPitch) + 2 * t * F::kBlocks;
     if (NT == 1 || tiles == 1) multiply_chunk<W8, X8, 1, NT>(weights, tokens, scales, token_scales, len, t, acc);
     else if (NT == 2 || tiles == 2) multiply_chunk<W8, X8, NT < 2 ? NT : 2, NT>(weights, tokens, scales, token_scales, len, t, acc);
+    else if (NT == 3 || tiles == 3) multiply_chunk<W8, X8, NT < 3 ? NT : 3, NT>(weights, tokens, scales, token_scales, len, t, acc);
     else multiply_chunk<W8, X8, NT, NT>(weights, tokens, scales, token_scales, len, t, acc);
     __syncwarp();
     if (lane == 0) mbar_arrive(ring.empty + 8 * s);
