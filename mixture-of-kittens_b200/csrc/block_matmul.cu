@@ -66,15 +66,6 @@ __device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-// 32 lanes x 16 consecutive fp32 columns as eight pairs.
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
 // Two fp32 operations per instruction (sm_100).
 __device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) {
     unsigned long long d;
@@ -94,6 +85,37 @@ __device__ __forceinline__ unsigned long long pair_mul(unsigned long long a, uns
 }
 __device__ __forceinline__ void pair_split(unsigned long long d, uint32_t& lo, uint32_t& hi) {
     asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(d));
+}
+
+// mbar_wait that polls instead of suspending the thread: the accumulators change hands once per block of K.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* status) {
+    long long start = 0;
+    for (uint32_t spin = 0;; ++spin) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((spin & 0x3FF) == 0x3FF) {
+            if (*abort_flag) return false;
+            if (start == 0) start = clock64();
+            if (clock64() - start > kPipelineWaitCycles) {
+                *abort_flag = 1;
+                if (status != nullptr) atomicOr(status, (uint32_t)MOK_STATUS_PIPELINE_TIMEOUT);
+                return false;
+            }
+        }
+    }
+}
+
+// Arrival at the leader CTA's barrier that orders nothing but the tensor-memory loads before it (they are complete and fenced).  The
+// usual release at cluster scope also waits for the scales on their way from L2: 1100 clocks a block of K, where all else takes 550.
+__device__ __forceinline__ void arrive_leader_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar & kPairLeaderMask) : "memory");
 }
 
 struct Work {
@@ -185,7 +207,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     const Work w = decode(p, t);
                     for (int kb = w.kb0; kb < w.kb1; ++kb, ++block) {
                         const uint32_t buf = block & 1u;
-                        ok = mbar_wait(bar_acc_empty + 8 * buf, ((block >> 1) & 1u) ^ 1u, abort_flag, p.status) &&
+                        ok = mbar_poll(bar_acc_empty + 8 * buf, ((block >> 1) & 1u) ^ 1u, abort_flag, p.status) &&
                              mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status);
                         if (!ok) break;
                         tc_fence_after_sync();
@@ -243,30 +265,31 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
                     for (int j = 0; j < (COLUMN_SCALES ? 4 : 1); ++j) next_b[j] = sb[j][(kb + 1) * p.sb_block];
                 }
-                ok = mbar_wait(bar_acc_full + 8 * buf, (block >> 1) & 1u, abort_flag, p.status);
+                ok = mbar_poll(bar_acc_full + 8 * buf, (block >> 1) & 1u, abort_flag, p.status);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
                 const unsigned long long s2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
-                uint32_t v[2][16];
-                tmem_ld_32x16(taddr, v[0]);
+                // 64 columns at a time, two loads in flight; the loads of the second half follow the sums of the first
+                uint32_t v[2][32];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld_32x32(taddr + h * 64, v[0]);
+                    tmem_ld_32x32(taddr + h * 64 + 32, v[1]);
                     tmem_ld_wait();
-                    if (c + 1 < 8) tmem_ld_32x16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
-                    if (c == 7) {
+                    if (h == 1) {
                         tc_fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_leader(bar_acc_empty + 8 * buf);
+                        if (lane == 0) arrive_leader_relaxed(bar_acc_empty + 8 * buf);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const unsigned long long d = pair_of(v[c & 1][2 * i], v[c & 1][2 * i + 1]);
+                    for (int i = 0; i < 32; ++i) {
+                        const unsigned long long d = pair_of(v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]);
                         if (COLUMN_SCALES) {
-                            const unsigned long long cs = *reinterpret_cast<const unsigned long long*>(cols + c * 16 + 2 * i);
-                            acc[c * 8 + i] = pair_fma(d, pair_mul(cs, s2), acc[c * 8 + i]);
+                            const unsigned long long cs = *reinterpret_cast<const unsigned long long*>(cols + h * 64 + 2 * i);
+                            acc[h * 32 + i] = pair_fma(d, pair_mul(cs, s2), acc[h * 32 + i]);
                         } else {
-                            acc[c * 8 + i] = pair_fma(d, s2, acc[c * 8 + i]);
+                            acc[h * 32 + i] = pair_fma(d, s2, acc[h * 32 + i]);
                         }
                     }
                 }
