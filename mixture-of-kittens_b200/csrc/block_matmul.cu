@@ -176,6 +176,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    allow_next_kernel();   // the kernel that adds the shares, if there is one, waits for this one
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
@@ -270,28 +271,35 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 tc_fence_after_sync();
                 const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
                 const unsigned long long s2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
-                // 64 columns at a time, two loads in flight; the loads of the second half follow the sums of the first
+                // 32 columns at a time: the next load runs while the columns before are added, and the accumulator goes back to the
+                // MMAs before its last columns are
                 uint32_t v[2][32];
+                tmem_ld_32x32(taddr, v[0]);
+                tmem_ld_32x32(taddr + 32, v[1]);
+                tmem_ld_wait();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    tmem_ld_32x32(taddr + h * 64, v[0]);
-                    tmem_ld_32x32(taddr + h * 64 + 32, v[1]);
-                    tmem_ld_wait();
-                    if (h == 1) {
+                for (int q = 0; q < 4; ++q) {
+                    if (q >= 2) tmem_ld_wait();
+                    if (q == 3) {
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) arrive_leader_relaxed(bar_acc_empty + 8 * buf);
                     }
+                    if (q == 2) tmem_ld_32x32(taddr + 96, v[1]);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const unsigned long long d = pair_of(v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]);
+                    for (int i = 0; i < 8; ++i) {
+                        const unsigned long long d0 = pair_of(v[q & 1][4 * i], v[q & 1][4 * i + 1]);
+                        const unsigned long long d1 = pair_of(v[q & 1][4 * i + 2], v[q & 1][4 * i + 3]);
+                        unsigned long long f0 = s2, f1 = s2;
                         if (COLUMN_SCALES) {
-                            const unsigned long long cs = *reinterpret_cast<const unsigned long long*>(cols + h * 64 + 2 * i);
-                            acc[h * 32 + i] = pair_fma(d, pair_mul(cs, s2), acc[h * 32 + i]);
-                        } else {
-                            acc[h * 32 + i] = pair_fma(d, s2, acc[h * 32 + i]);
+                            const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(cols + q * 32 + 4 * i);
+                            f0 = pair_mul(cs.x, s2);
+                            f1 = pair_mul(cs.y, s2);
                         }
+                        acc[q * 16 + 2 * i] = pair_fma(d0, f0, acc[q * 16 + 2 * i]);
+                        acc[q * 16 + 2 * i + 1] = pair_fma(d1, f1, acc[q * 16 + 2 * i + 1]);
                     }
+                    if (q == 0) tmem_ld_32x32(taddr + 64, v[0]);
                 }
             }
             if (!ok) {   // a wait ran out (reported in the status word): this tile and the ones that follow are NaN
@@ -371,6 +379,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 __global__ void __launch_bounds__(256) sum_shares_kernel(const float* __restrict__ partial, int splits, long long count, int cols,
                                                          bf16* __restrict__ out, long long out_stride) {
     const long long i = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+    wait_previous_kernel();
     if (i >= count) return;
     if ((cols & 3) == 0) {
         float4 s = *reinterpret_cast<const float4*>(partial + i);
@@ -406,13 +415,14 @@ int code_map(CUtensorMap* map, const void* base, long long stride, long long row
 
 int div_up(long long a, int b) { return static_cast<int>((a + b - 1) / b); }
 
-// Shares of K: enough to give every CTA pair a tile, each at least four blocks long (shorter shares pay more for their sums in
-// memory than they save).
+// Shares of K: enough to give every CTA pair a tile, each at least four blocks long, where that takes 16 blocks or more (0.4 us each)
+// off the longest chain: writing, reading and adding the shares costs 6 us.  1000 x 1544 x 1808 (28 tiles, 15 blocks) takes 20.5 us in
+// one share and 24.5 in two.
 int shares(int tiles, int k_blocks) {
     const int pairs = sm_count() / 2;
     int s = pairs / tiles;
     if (s > k_blocks / 4) s = k_blocks / 4;
-    return s < 1 ? 1 : s;
+    return s < 2 || k_blocks - k_blocks / s < 16 ? 1 : s;
 }
 
 int plan_splits(long long rows, int cols, int depth) {
@@ -480,8 +490,8 @@ extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_
     }
     if (p.splits > 1) {
         const long long count = rows * cols;
-        sum_shares_kernel<<<static_cast<unsigned>((count + 1023) / 1024), 256, 0, s>>>(p.partial, p.splits, count, cols, p.out, out_stride);
-        MOK_LAUNCH_CHECK("sum_shares_kernel");
+        MOK_TRY(launch_early(sum_shares_kernel, "sum_shares_kernel", dim3(static_cast<unsigned>((count + 1023) / 1024)), 256, 0, s,
+                             static_cast<const float*>(p.partial), p.splits, count, cols, p.out, static_cast<long long>(out_stride)));
     }
     return MOK_OK;
 }
