@@ -112,6 +112,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// 16 bytes to shared memory, asynchronously, past L1.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------
 // Programmatic dependent launch: a kernel launched with launch_early() may begin while the one before it in the stream still runs.
 // It has to wait_previous_kernel() before it touches anything that one may write; allow_next_kernel() lets the next one begin.

@@ -2,8 +2,9 @@
 // and / or as e4m3 with a scale per 128 columns; hidden = bf16(z) is the next residual stream.  The norm is taken of z before
 // it is rounded.  Backward, with z read back from `hidden`:
 //   g = dy w,  dx = dr = rho (g - z rho^2 mean(g z)) + dhidden,  dw = sum over rows of dy z rho.
-// Both are bound by HBM (by launch and latency for a few rows): every input is read once, into registers, and all sums are
-// fp32.
+// Both are bound by HBM (by launch and latency for a few rows): every input is read once and all sums are fp32.  16384 x 7168 with
+// a residual: forward 172 us, 5.5 TB/s; with 8-bit output instead 176 us; backward with d_hidden 172 us, 5.5 TB/s.  2048 columns:
+// 47, 51 and 64 us.  One row: 4 us, which is the launch.
 #include "block_scale.cuh"
 
 namespace mok {
@@ -48,9 +49,10 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < warps; ++i) s += part[i];
-    return s;
+    v = (threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
 }
 
 // One row per block; a thread holds V vectors of 8 columns, so 16 adjacent lanes hold one block of 128.
@@ -124,6 +126,23 @@ __global__ void __launch_bounds__(V < 4 ? 256 : 512) rms_norm_forward_kernel(con
     }
 }
 
+// Eight weights of a thread's columns, as they are stored.
+template <bool W32>
+struct Weight8 {
+    uint4 raw[W32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* weight, int i, int vectors) {
+#pragma unroll
+        for (int k = 0; k < (W32 ? 2 : 1); ++k)
+            raw[k] = i < vectors ? reinterpret_cast<const uint4*>(weight)[i * (W32 ? 2 : 1) + k] : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ float at(int j) const {
+        const uint4& q = raw[W32 ? j >> 2 : 0];
+        const int k = W32 ? j & 3 : j >> 1;
+        const uint32_t u = k == 0 ? q.x : k == 1 ? q.y : k == 2 ? q.z : q.w;
+        return __uint_as_float(W32 ? u : (j & 1) ? (u & 0xFFFF0000u) : (u << 16));
+    }
+};
+
 struct NormBackward {
     const bf16 *d_y, *d_hidden, *z;
     const void* weight;
@@ -131,37 +150,66 @@ struct NormBackward {
     bf16* d_x;
     float* partials;   // [gridDim.x, cols]
     long long z_stride, rows;
-    int cols;
+    int cols, stages;
 };
 
-// A block takes every gridDim.x-th row and keeps its share of the weight gradient in registers.
-template <int V, bool W32>
-__global__ void __launch_bounds__(V == 1 ? 256 : 512) rms_norm_backward_kernel(const NormBackward p) {
+// A block takes every gridDim.x-th row and keeps its share of the weight gradient in registers.  The rows to come are on their way to
+// shared memory meanwhile (each thread copies, waits for and reads its own columns, so a row costs one barrier, that of its sum): with
+// loads to registers, those of d_hidden behind the sum, a row was two trips to memory and 16384 x 7168 took 408 us.  Two blocks an SM
+// fill each other's barriers (one of them with a ring of four rows 299 us, two with two rows 192 us, now 172 us).
+template <int V, int THREADS, int BLOCKS, bool W32>
+__global__ void __launch_bounds__(THREADS, BLOCKS) rms_norm_backward_kernel(const NormBackward p) {
+    extern __shared__ __align__(16) uint8_t ring[];   // [stage][z, d_y, d_hidden][cols]
     __shared__ float part[2][32];
     const int vectors = p.cols >> 3;
+    const long long row_bytes = p.cols * 2;
+    const int inputs = p.d_hidden != nullptr ? 3 : 2;
     float dw[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[v][j] = 0.0f;
-    int flip = 0;
+    allow_next_kernel();
+    auto slot = [&](int stage, int input, int i) { return ring + (stage * inputs + input) * row_bytes + i * 16; };
+    auto fetch = [&](long long row, int stage) {
+        if (row < p.rows) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int i = v * blockDim.x + threadIdx.x;
+                if (i < vectors) {
+                    copy16(smem_u32(slot(stage, 0, i)), p.z + row * p.z_stride + i * 8);
+                    copy16(smem_u32(slot(stage, 1, i)), p.d_y + row * p.cols + i * 8);
+                    if (inputs == 3) copy16(smem_u32(slot(stage, 2, i)), p.d_hidden + row * p.cols + i * 8);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int s = 0; s < p.stages - 1; ++s) fetch(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    Weight8<W32> w[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) w[v].load(p.weight, v * blockDim.x + threadIdx.x, vectors);
+    int flip = 0, stage = 0;
+    float rho = p.inv_rms[blockIdx.x];
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, flip ^= 1) {
-        const float rho = p.inv_rms[row];
-        float z[V][8], g[V][8];
+        const float next_rho = row + gridDim.x < p.rows ? p.inv_rms[row + gridDim.x] : 0.0f;
+        const int behind = stage == 0 ? p.stages - 1 : stage - 1;   // the stage of the row before, which this thread has read
+        fetch(row + static_cast<long long>(p.stages - 1) * gridDim.x, behind);
+        if (p.stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else if (p.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else asm volatile("cp.async.wait_group 3;" ::: "memory");
         float dot = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int i = v * blockDim.x + threadIdx.x;
             if (i < vectors) {
-                float w[8];
-                unpack8(*reinterpret_cast<const uint4*>(p.z + row * p.z_stride + i * 8), z[v]);
-                unpack8(*reinterpret_cast<const uint4*>(p.d_y + row * p.cols + i * 8), g[v]);
-                load_weight<W32>(p.weight, i * 8, w);
+                float z[8], g[8];
+                unpack8(*reinterpret_cast<const uint4*>(slot(stage, 0, i)), z);
+                unpack8(*reinterpret_cast<const uint4*>(slot(stage, 1, i)), g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    dw[v][j] = fmaf(g[v][j], z[v][j] * rho, dw[v][j]);
-                    g[v][j] *= w[j];
-                    dot = fmaf(g[v][j], z[v][j], dot);
+                    dw[v][j] = fmaf(g[j], z[j] * rho, dw[v][j]);
+                    dot = fmaf(g[j] * w[v].at(j), z[j], dot);
                 }
             }
         }
@@ -169,18 +217,23 @@ __global__ void __launch_bounds__(V == 1 ? 256 : 512) rms_norm_backward_kernel(c
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int i = v * blockDim.x + threadIdx.x;
-            if (i < vectors) {
-                float d[8];
-                if (p.d_hidden != nullptr) unpack8(*reinterpret_cast<const uint4*>(p.d_hidden + row * p.cols + i * 8), d);
+            if (i < vectors) {   // read again: kept in registers they would leave room for half the threads
+                float z[8], g[8], d[8];
+                unpack8(*reinterpret_cast<const uint4*>(slot(stage, 0, i)), z);
+                unpack8(*reinterpret_cast<const uint4*>(slot(stage, 1, i)), g);
+                if (inputs == 3) unpack8(*reinterpret_cast<const uint4*>(slot(stage, 2, i)), d);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float dx = rho * (g[v][j] - z[v][j] * c);
-                    d[j] = p.d_hidden != nullptr ? dx + d[j] : dx;
+                    const float dx = rho * (g[j] * w[v].at(j) - z[j] * c);
+                    d[j] = inputs == 3 ? dx + d[j] : dx;
                 }
                 *reinterpret_cast<uint4*>(p.d_x + row * p.cols + i * 8) = pack8(d);
             }
         }
+        rho = next_rho;
+        if (++stage == p.stages) stage = 0;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int i = v * blockDim.x + threadIdx.x;
@@ -192,37 +245,59 @@ __global__ void __launch_bounds__(V == 1 ? 256 : 512) rms_norm_backward_kernel(c
     }
 }
 
-// dw = sum of the blocks' shares, in block order: 32 columns x 8 phases a block.
+// dw = sum of the blocks' shares in a fixed order: 32 columns x 32 phases a block.
 template <bool W32>
-__global__ void __launch_bounds__(256) rms_norm_weight_grad_kernel(const float* __restrict__ partials, int blocks, int cols, void* d_weight) {
-    __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) rms_norm_weight_grad_kernel(const float* __restrict__ partials, int blocks, int cols, void* d_weight) {
+    __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, phase = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
     float s = 0.0f;
-    if (col < cols)
-        for (int b = phase; b < blocks; b += 8) s += partials[static_cast<long long>(b) * cols + col];
-    part[phase][lane] = s;
+    wait_previous_kernel();
+    if (col < cols) {
+#pragma unroll 8
+        for (int b = phase; b < blocks; b += 32) s += partials[static_cast<long long>(b) * cols + col];
+    }
+    part[lane][phase] = s;
     __syncthreads();
-    if (phase == 0 && col < cols) {
-        s = 0.0f;
+    s = part[phase][lane];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += part[i][lane];
-        if (W32) static_cast<float*>(d_weight)[col] = s;
-        else static_cast<bf16*>(d_weight)[col] = __float2bfloat16(s);
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    const int out = blockIdx.x * 32 + phase;
+    if (lane == 0 && out < cols) {
+        if (W32) static_cast<float*>(d_weight)[out] = s;
+        else static_cast<bf16*>(d_weight)[out] = __float2bfloat16(s);
     }
 }
 
-int backward_blocks(long long rows) {
-    const long long most = 2LL * sm_count();
+// Blocks of the backward: as many an SM as registers and rings of two rows leave room for.  16384 x 4096: two an SM 125 us, four 102 us.
+int backward_blocks_per_sm(int cols) { return cols <= 4096 ? 4 : cols <= 8192 ? 2 : 1; }
+int backward_blocks(long long rows, int cols) {
+    const long long most = static_cast<long long>(backward_blocks_per_sm(cols)) * sm_count();
     return static_cast<int>(rows < most ? rows : most);
 }
 
-// Vectors of 8 columns per thread (1, 2 or 4) and threads for a row: vectors are added while the block is wider than `wide`.
-void row_shape(int cols, int wide, int& v, int& threads) {
+// Vectors of 8 columns per thread and threads for a row of the forward: vectors are added while the block is wider than 256.
+void row_shape(int cols, int& v, int& threads) {
     const int vectors = cols / 8;
     v = 1;
-    while (v < 4 && (vectors + v - 1) / v > (v == 1 ? 256 : wide)) v *= 2;
+    while (v < 4 && (vectors + v - 1) / v > 256) v *= 2;
     threads = ((vectors + v - 1) / v + 31) / 32 * 32;
+}
+
+template <int V, int THREADS, int BLOCKS, bool W32>
+int launch_backward(const NormBackward& p, int grid, int threads, int smem, cudaStream_t stream) {
+    static int ready[16] = {0};
+    int dev = 0;
+    MOK_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 16) return MOK_ERR_UNSUPPORTED;
+    const auto rms_norm_backward = rms_norm_backward_kernel<V, THREADS, BLOCKS, W32>;
+    if (ready[dev] == 0) {
+        MOK_CUDA_CHECK(cudaFuncSetAttribute(rms_norm_backward, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+        ready[dev] = 1;
+    }
+    rms_norm_backward<<<grid, threads, smem, stream>>>(p);
+    MOK_LAUNCH_CHECK("rms_norm_backward_kernel");
+    return MOK_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -232,7 +307,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 extern "C" int64_t mok_rms_norm_scratch_bytes(int64_t rows, int hidden) {
     if (rows <= 0 || hidden <= 0) return 0;
-    return static_cast<int64_t>(mok::backward_blocks(rows)) * hidden * 4;
+    return static_cast<int64_t>(mok::backward_blocks(rows, hidden)) * hidden * 4;
 }
 
 extern "C" int mok_rms_norm_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
@@ -268,7 +343,7 @@ extern "C" int mok_rms_norm_forward(const void* x, int64_t x_stride, const void*
     p.cols = hidden;
     p.eps = eps;
     int v, threads;
-    row_shape(hidden, 256, v, threads);
+    row_shape(hidden, v, threads);
     const int grid = static_cast<int>(rows);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
 #define MOK_NORM(V)                                                                      \
@@ -305,22 +380,20 @@ extern "C" int mok_rms_norm_backward(const void* d_y, const void* d_hidden, cons
     p.z_stride = z_stride;
     p.rows = rows;
     p.cols = hidden;
-    int v, threads;
-    row_shape(hidden, 512, v, threads);
-    const int grid = backward_blocks(rows);
+    const int vectors = hidden / 8, v = vectors <= 256 ? 1 : 2, threads = ((vectors + v - 1) / v + 31) / 32 * 32;
+    const int row_bytes = (d_hidden != nullptr ? 3 : 2) * hidden * 2, room = (224 * 1024) / backward_blocks_per_sm(hidden) - 1024;
+    p.stages = room / row_bytes > 4 ? 4 : room / row_bytes;   // 2 at 16384 columns
+    const int grid = backward_blocks(rows, hidden), smem = p.stages * row_bytes;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define MOK_NORM(V)                                                                       \
-    do {                                                                                  \
-        if (weight_is_f32) rms_norm_backward_kernel<V, true><<<grid, threads, 0, s>>>(p); \
-        else rms_norm_backward_kernel<V, false><<<grid, threads, 0, s>>>(p);              \
-    } while (0)
-    if (v == 1) MOK_NORM(1);
-    else if (v == 2) MOK_NORM(2);
-    else MOK_NORM(4);
-#undef MOK_NORM
-    MOK_LAUNCH_CHECK("rms_norm_backward_kernel");
-    if (weight_is_f32) rms_norm_weight_grad_kernel<true><<<(hidden + 31) / 32, 256, 0, s>>>(scratch, grid, hidden, d_weight);
-    else rms_norm_weight_grad_kernel<false><<<(hidden + 31) / 32, 256, 0, s>>>(scratch, grid, hidden, d_weight);
-    MOK_LAUNCH_CHECK("rms_norm_weight_grad_kernel");
-    return MOK_OK;
+    using Launch = int (*)(const NormBackward&, int, int, int, cudaStream_t);
+    Launch launch;
+    if (v == 1) launch = weight_is_f32 ? launch_backward<1, 256, 4, true> : launch_backward<1, 256, 4, false>;
+    else if (threads <= 256) launch = weight_is_f32 ? launch_backward<2, 256, 4, true> : launch_backward<2, 256, 4, false>;
+    else if (threads <= 512) launch = weight_is_f32 ? launch_backward<2, 512, 2, true> : launch_backward<2, 512, 2, false>;
+    else launch = weight_is_f32 ? launch_backward<2, 1024, 1, true> : launch_backward<2, 1024, 1, false>;
+    MOK_TRY(launch(p, grid, threads, smem, s));
+    const dim3 columns((hidden + 31) / 32);
+    const float* shares = scratch;
+    if (weight_is_f32) return launch_early(rms_norm_weight_grad_kernel<true>, "rms_norm_weight_grad_kernel", columns, 1024, 0, s, shares, grid, hidden, d_weight);
+    return launch_early(rms_norm_weight_grad_kernel<false>, "rms_norm_weight_grad_kernel", columns, 1024, 0, s, shares, grid, hidden, d_weight);
 }

@@ -56,9 +56,6 @@ struct Form {
     __device__ static __forceinline__ int chunks(int k_total) { return (k_total + kChunk - 1) / kChunk; }
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
