@@ -13,9 +13,6 @@ constexpr int kScaleBlock = 128;
 // Largest magnitude of a block as the bits of an fp32 value: integer order is that of magnitudes, infinities come above the
 // finite values and NaNs above those, where fmaxf would drop them.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t abs_bits_bf16x2(uint32_t v) {
-    return max((v << 16) & 0x7FFF0000u, v & 0x7FFF0000u);
-}
 
 // Scale of a block and its reciprocal, both exact.  448 = 1.75 * 2^8: 2^k with k = exponent - 8, one more where the mantissa is
 // above 1.75; at least 2^-126 (blocks of zeros too).  A block that holds an infinity or a NaN gets scale and reciprocal NaN, so
