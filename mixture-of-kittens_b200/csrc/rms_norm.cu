@@ -3,8 +3,8 @@
 // it is rounded.  Backward, with z read back from `hidden`:
 //   g = dy w,  dx = dr = rho (g - z rho^2 mean(g z)) + dhidden,  dw = sum over rows of dy z rho.
 // Both are bound by HBM (by launch and latency for a few rows): every input is read once and all sums are fp32.  16384 x 7168 with
-// a residual: forward 172 us, 5.5 TB/s; with 8-bit output instead 176 us; backward with d_hidden 172 us, 5.5 TB/s.  2048 columns:
-// 47, 51 and 64 us.  One row: 4 us, which is the launch.
+// a residual: forward 158 us, 5.9 TB/s; with 8-bit output instead 195 us; backward with d_hidden 172 us, 5.5 TB/s.  2048 columns:
+// 45, 53 and 62 us.  One row: 4 us, which is the launch.
 #include "block_scale.cuh"
 
 namespace mok {
@@ -21,6 +21,7 @@ struct NormForward {
     long long x_stride, residual_stride, codes_stride, scale_row_stride, scale_block_stride, rows;
     int cols;
     float eps;
+    double inv_cols;
 };
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -41,23 +42,33 @@ __device__ __forceinline__ void load_weight(const void* w, int col, float (&f)[8
     }
 }
 
-// Sum over the block, the same value in every thread, in a fixed order.  `part` holds one float per warp; the caller alternates
+// Sum over the block, the same value in every thread, in a fixed order.  `part` holds one value per warp; the caller alternates
 // between two of them, so that one barrier per sum is enough.
-__device__ __forceinline__ float block_sum(float v, float* part) {
+template <class T = float>   // of the last step, over the warps
+__device__ __forceinline__ T block_sum(float v, float* part) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : 0.0f;
+    T s = (threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : 0.0f;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return s;
 }
 
-// One row per block; a thread holds V vectors of 8 columns, so 16 adjacent lanes hold one block of 128.
-template <int V, bool W32>
-__global__ void __launch_bounds__(V < 4 ? 256 : 512) rms_norm_forward_kernel(const NormForward p) {
+// y / scale in fp32 is a few units off in its last place, which decides the code only where it comes that close to the middle
+// between two codes: with 20 bits below e4m3's mantissa, one value in 130 000.  Those are made from 64 bits, so that a code is off
+// its neighbour's side about ten times as rarely.  (Codes below 2^-6 have their middles elsewhere; half a step there is 2^-18 of the
+// largest value.)
+__device__ __forceinline__ uint32_t from_middle(float v) { return (__float_as_uint(v) - 0x7FFFCu) & 0xFFFFFu; }
+constexpr uint32_t kNearMiddle = 8;
+// One row per block; a thread holds V vectors of 8 columns, so 16 adjacent lanes hold one block of 128.  With codes the bounds
+// below ask for more blocks an SM than registers allow without spills, which all lie on the rare path: 16384 x 7168 in 195 us, 207
+// with four blocks.  z kept in shared memory (225 us) and the rare values listed there for the block's end (221 us) took longer.
+template <int V, int THREADS, bool W32, bool CODES>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : !CODES ? 1 : V == 4 ? 5 : V == 2 ? 6 : 7)
+    rms_norm_forward_kernel(const NormForward p) {
     __shared__ float part[32];
     const long long row = blockIdx.x;
     const int vectors = p.cols >> 3;
@@ -92,7 +103,14 @@ __global__ void __launch_bounds__(V < 4 ? 256 : 512) rms_norm_forward_kernel(con
     for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(z[v][j], z[v][j], sum);
-    const float rho = __frsqrt_rn(__fdiv_rn(block_sum(sum, part), static_cast<float>(p.cols)) + p.eps);
+    float rho;
+    double mean = 0.0;
+    if (CODES) {
+        mean = block_sum<double>(sum, part) * p.inv_cols + p.eps;
+        rho = __frsqrt_rn(static_cast<float>(mean));
+    } else {
+        rho = __frsqrt_rn(__fdiv_rn(block_sum(sum, part), static_cast<float>(p.cols)) + p.eps);
+    }
     if (p.inv_rms != nullptr && threadIdx.x == 0) p.inv_rms[row] = rho;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -103,9 +121,9 @@ __global__ void __launch_bounds__(V < 4 ? 256 : 512) rms_norm_forward_kernel(con
             load_weight<W32>(p.weight, i * 8, y);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = z[v][j] * rho * y[j];
-            if (p.y != nullptr) *reinterpret_cast<uint4*>(p.y + row * p.cols + i * 8) = pack8(y);
+            if (!CODES || p.y != nullptr) *reinterpret_cast<uint4*>(p.y + row * p.cols + i * 8) = pack8(y);
         }
-        if (p.codes != nullptr) {
+        if (CODES) {
             uint32_t big = 0;
             if (mine) {
 #pragma unroll
@@ -116,10 +134,22 @@ __global__ void __launch_bounds__(V < 4 ? 256 : 512) rms_norm_forward_kernel(con
             float inv;
             const float scale = block_scale(big, inv);
             if (mine) {
-                uint2 q;
-                q.x = mxfp8_convert4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-                q.y = mxfp8_convert4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
-                *reinterpret_cast<uint2*>(p.codes + row * p.codes_stride + i * 8) = q;
+                uint32_t nearest = kNearMiddle;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] *= inv;
+                    nearest = min(nearest, from_middle(y[j]));
+                }
+                if (nearest < kNearMiddle) {
+                    float w[8];
+                    load_weight<W32>(p.weight, i * 8, w);
+                    const double r0 = rho, better = fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0);   // a Newton step
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (from_middle(y[j]) < kNearMiddle) y[j] = static_cast<float>(better * z[v][j] * w[j] * inv);
+                }
+                *reinterpret_cast<uint2*>(p.codes + row * p.codes_stride + i * 8) =
+                    make_uint2(mxfp8_convert4(y[0], y[1], y[2], y[3]), mxfp8_convert4(y[4], y[5], y[6], y[7]));
                 if ((i & 15) == 0) p.scales[row * p.scale_row_stride + (i >> 4) * p.scale_block_stride] = scale;
             }
         }
@@ -342,19 +372,22 @@ extern "C" int mok_rms_norm_forward(const void* x, int64_t x_stride, const void*
     p.rows = rows;
     p.cols = hidden;
     p.eps = eps;
+    p.inv_cols = 1.0 / hidden;
     int v, threads;
     row_shape(hidden, v, threads);
     const int grid = static_cast<int>(rows);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define MOK_NORM(V)                                                                      \
-    do {                                                                                 \
-        if (weight_is_f32) rms_norm_forward_kernel<V, true><<<grid, threads, 0, s>>>(p); \
-        else rms_norm_forward_kernel<V, false><<<grid, threads, 0, s>>>(p);              \
-    } while (0)
-    if (v == 1) MOK_NORM(1);
-    else if (v == 2) MOK_NORM(2);
-    else MOK_NORM(4);
+    const bool w32 = weight_is_f32 != 0, with_codes = codes != nullptr;
+    void (*kernel)(NormForward);
+#define MOK_NORM(V, THREADS)                                                                                                     \
+    kernel = with_codes ? w32 ? rms_norm_forward_kernel<V, THREADS, true, true> : rms_norm_forward_kernel<V, THREADS, false, true> \
+                        : w32 ? rms_norm_forward_kernel<V, THREADS, true, false> : rms_norm_forward_kernel<V, THREADS, false, false>
+    if (v == 1) MOK_NORM(1, 256);
+    else if (v == 2) MOK_NORM(2, 256);
+    else if (threads <= 256) MOK_NORM(4, 256);
+    else MOK_NORM(4, 512);
 #undef MOK_NORM
+    kernel<<<grid, threads, 0, s>>>(p);
     MOK_LAUNCH_CHECK("rms_norm_forward_kernel");
     return MOK_OK;
 }
