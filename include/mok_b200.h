@@ -442,7 +442,7 @@ int mok_router_decode(const void* x, int64_t x_stride, const void* w, int w_is_f
  * The layer for 1 to 256 tokens (num_tokens * topk <= 4096), without workspace or schedule: out bf16 [num_tokens, hidden] =
  * shared(x) + sum over k of router_weights[t, k] * expert(top_experts[t, k])(x).  Routed weights are bf16 (the three scale arrays
  * NULL) or e4m3 with an fp32 scale per 128 x 128 of every expert ([num_experts, ceil(rows / 128), ceil(columns / 128)]); the shared
- * ones are bf16, or NULL with shared_intermediate 0.  Sizes are multiples of 64.  Routes outside [first_expert, first_expert +
+ * ones are bf16, or NULL with shared_intermediate 0.  Sizes are multiples of 64, addresses of 16 bytes.  Routes outside [first_expert, first_expert +
  * num_experts) contribute nothing; an expert that a token names twice counts with both weights.  scratch:
  * mok_moe_decode_scratch_bytes().  `out` is NaN while the status word is not zero (see mok_fwd_epilogue).
  */

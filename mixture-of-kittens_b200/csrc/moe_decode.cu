@@ -39,12 +39,12 @@ struct Decode {
     bf16 *hidden, *hidden_shared, *out;
     __half* x_half;                       // W8: tokens and, in place, hidden rows as f16 with a power of two per row
     float *x_scale, *hidden_scale;        // [tokens], [routes]
+    float* parts;                         // wide form: [routes, then tokens for the shared expert][hidden_size]
     uint32_t* status;
     int tokens, hidden_size, intermediate, shared_intermediate, experts, first_expert, topk;
     int clamp;
     float limit;
-    int blocks;   // per SM
-    int stages, stage_bytes, token_cap, shared_cap;   // the ring; tokens of a stage, of routed experts and the shared one
+    int stages, stage_bytes, token_cap;   // the ring; tokens of a stage
 };
 
 // Which experts are in use: active[i], and the range [begin[i], begin[i + 1]) of its routes in list (with their tokens and weights
@@ -210,8 +210,8 @@ __device__ __forceinline__ bool for_shared_pieces(const Decode& p, F&& f) {
     q.expert = -1;
     for (q.row = static_cast<int>(static_cast<long long>(p.shared_intermediate) * blockIdx.x / gridDim.x); q.row < end; q.row += kPairs) {
         q.count = min(kPairs, end - q.row);
-        for (q.from = 0; q.from < p.tokens; q.from += p.shared_cap) {
-            q.tokens = min(p.shared_cap, p.tokens - q.from);
+        for (q.from = 0; q.from < p.tokens; q.from += p.token_cap) {
+            q.tokens = min(p.token_cap, p.tokens - q.from);
             if (!f(q)) return false;
         }
     }
@@ -300,9 +300,17 @@ __global__ void __launch_bounds__(256) to_half_kernel(const Decode p) {
     }
 }
 
+__device__ __forceinline__ bf16 hidden_value(const Decode& p, float g, float u) {
+    if (p.clamp) {   // comparisons that let a NaN through
+        g = g > p.limit ? p.limit : g;
+        u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
+    }
+    return __float2bfloat16(g * sigmoid_fast(g) * u);
+}
+
 // ---- gate / up --------------------------------------------------------------------------------------------------------
-template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(const Decode p) {
+template <bool W8>
+__global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
     allow_next_kernel();   // not before: the down kernel reads weights and routes that earlier kernels may have written
     Deposit sums;
     sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
-    const Routing r = carve_routing(reinterpret_cast<uint8_t*>(sums.scratch + deposit_floats<NT>()), p.experts, p.tokens * p.topk);
+    const Routing r = carve_routing(reinterpret_cast<uint8_t*>(sums.scratch + deposit_floats<1>()), p.experts, p.tokens * p.topk);
     const int chunks = Form<false, false>::chunks(p.hidden_size), chunks8 = Form<true, false>::chunks(p.hidden_size);
     auto slots_of = [&](const Piece& q) { return min(W8 && q.expert >= 0 ? chunks8 : chunks, kConsumers); };
     if (warp == kFinisher) {
@@ -321,17 +329,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
             for (int i = lane; i < kPairs * q.tokens; i += 32) {
                 const int pair = i & (kPairs - 1), c = i / kPairs;
                 if (pair >= q.count) continue;
-                float g = sum_of<NT>(sums, slots, pair, c), u = sum_of<NT>(sums, slots, pair + 8, c);
+                float g = sum_of<1>(sums, slots, pair, c), u = sum_of<1>(sums, slots, pair + 8, c);
                 if (W8 && q.expert >= 0) {
                     const float scale = __ldcg(p.x_scale + r.token[q.from + c]);
                     g *= scale;
                     u *= scale;
                 }
-                if (p.clamp) {   // comparisons that let a NaN through
-                    g = g > p.limit ? p.limit : g;
-                    u = u > p.limit ? p.limit : u < -p.limit ? -p.limit : u;
-                }
-                const bf16 h = __float2bfloat16(g * sigmoid_fast(g) * u);
+                const bf16 h = hidden_value(p, g, u);
                 if (q.expert < 0) p.hidden_shared[static_cast<long long>(q.from + c) * p.shared_intermediate + q.row + pair] = h;
                 else p.hidden[static_cast<long long>(r.list[q.from + c]) * p.intermediate + q.row + pair] = h;
             }
@@ -379,13 +383,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_gate_up_kernel(
             const int n = w8 ? chunks8 : chunks, tiles = (q.tokens + 7) >> 3;
             const int slot = turn;
             if (slot < n) {
-                float acc[NT][4];
+                float acc[1][4];
                 clear(acc);
                 for (int c = slot; c < n; c += kConsumers) {
-                    if (w8) consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
-                    else consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
+                    if (w8) consume<W8, false, 1>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
+                    else consume<false, false, 1>(ring, smem, &bars.abort_flag, p.status, c, p.hidden_size, tiles, p.token_cap, lane, acc);
                 }
-                deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
+                deposit<1>(sums, bars, p.status, acc, slot, tiles, lane);
             }
             ++sums.piece;
             ring.next_piece(n);
@@ -415,9 +419,9 @@ __device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, i
     q.count = count;
     for (int a = p.shared_gate != nullptr ? -1 : 0; a < active; ++a) {
         q.expert = a < 0 ? -1 : r.active[a];
-        const int to = a < 0 ? p.tokens : r.begin[a + 1], cap = a < 0 ? p.shared_cap : p.token_cap;
-        for (q.from = a < 0 ? 0 : r.begin[a]; q.from < to; q.from += cap) {
-            q.tokens = min(cap, to - q.from);
+        const int to = a < 0 ? p.tokens : r.begin[a + 1];
+        for (q.from = a < 0 ? 0 : r.begin[a]; q.from < to; q.from += p.token_cap) {
+            q.tokens = min(p.token_cap, to - q.from);
             if (!f(q)) return false;
         }
     }
@@ -506,8 +510,8 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
     wait_copies();
 }
 
-template <bool W8, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(const Decode p) {
+template <bool W8>
+__global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -515,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
     Ring ring = set_up_ring(bars, smem, p.stage_bytes, p.stages, kConsumerThreads);
     Deposit sums;
     sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
-    float* out = sums.scratch + deposit_floats<NT>();   // [token][row of the piece]
+    float* out = sums.scratch + deposit_floats<1>();   // [token][row of the piece]
     const int values = p.tokens * kRows;
     const Routing r = carve_routing(reinterpret_cast<uint8_t*>(out + values), p.experts, p.tokens * p.topk);
     if (warp >= kConsumers && warp != kFinisher) {
@@ -544,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
                 for (int k = lane; k < kRows * q.tokens; k += 32) {   // a token is listed once
                     const int row = k & (kRows - 1), c = k / kRows;
                     float* at = out + (q.expert < 0 ? q.from + c : r.token[q.from + c]) * kRows + row;
-                    float v = sum_of<NT>(sums, slots, row, c);
+                    float v = sum_of<1>(sums, slots, row, c);
                     if (W8 && q.expert >= 0) v *= __ldcg(p.hidden_scale + r.list[q.from + c]);
                     *at = fmaf(q.expert < 0 ? 1.0f : r.weights[q.from + c], v, *at);
                 }
@@ -556,13 +560,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
                 const bool w8 = W8 && q.expert >= 0;
                 const int depth = depth_of(q), n = chunks_of(q), tiles = (q.tokens + 7) >> 3, slot = turn;
                 if (slot < n) {
-                    float acc[NT][4];
+                    float acc[1][4];
                     clear(acc);
                     for (int c = slot; c < n; c += kConsumers) {
-                        if (w8) consume<W8, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
-                        else consume<false, false, NT>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
+                        if (w8) consume<W8, false, 1>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
+                        else consume<false, false, 1>(ring, smem, &bars.abort_flag, p.status, c, depth, tiles, p.token_cap, lane, acc);
                     }
-                    deposit<NT>(sums, bars, p.status, acc, slot, tiles, lane);
+                    deposit<1>(sums, bars, p.status, acc, slot, tiles, lane);
                 }
                 ++sums.piece;
                 ring.next_piece(n);
@@ -582,6 +586,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) moe_down_kernel(con
     }
 }
 
+}  // namespace
+}  // namespace mok
+
+#include "moe_decode_wide.cuh"
+
+namespace mok {
+namespace {
+
 // ---------------------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------------------
@@ -590,40 +602,34 @@ static_assert(sizeof(Bars) <= 384, "");
 // Two blocks of a kernel share an SM when each takes half of the shared memory.
 constexpr int kHalf = kSmemPerSm / 2 - kStatic;
 
-int stage_bytes(int tokens, int shared_tokens, bool w8) {   // the shared expert is bf16 in either case
-    const int a = Form<false, false>::stage_bytes(shared_tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
+int stage_bytes(int tokens, bool w8) {   // the shared expert is bf16 in either case
+    const int a = Form<false, false>::stage_bytes(tokens), b = w8 ? Form<true, false>::stage_bytes(tokens) : 0;
     return a > b ? a : b;
 }
 // Shared memory beside the ring.
-int gate_up_rest(const Decode& p, int nt) { return kDeposits * kConsumers * nt * 128 * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
-int down_rest(const Decode& p, int nt) { return gate_up_rest(p, nt) + p.tokens * kRows * 4; }
+int gate_up_rest(const Decode& p) { return deposit_floats<1>() * 4 + routing_bytes(p.experts, p.tokens * p.topk); }
+int down_rest(const Decode& p) { return gate_up_rest(p) + p.tokens * kRows * 4; }
 
-// Blocks per SM, tokens of a stage, and the bytes that follow from it; false: nothing fits.  The ring has 8 stages, so that every
-// consumer keeps its own.  Two blocks of few tokens an SM hide each other's latency: hidden 4096, 8 experts of 14336, 4 tokens 370 ->
-// 327 us.  But an expert that more tokens chose is read more than once (from L2 after the first time), and the shared one sees
-// them all; one block has room for 24 tokens (bf16, shared) or 12.  bf16, two blocks against one, us:
-//                         4        8       16       32       64 tokens
-//   128 experts, K 8   73/95  112/142  165/210  222/275  288/349    (hidden 2048, experts of 768)
-//   32 of 256, K 8    95/116  108/120  169/187  380/419  536/560    (hidden 7168, experts of 2048)
-//   8 experts, K 2   327/370  462/489  593/605  949/771  1500/1240
-// 8-bit: 8 tokens 98/102, 100/106, 344/366; 16 tokens 141/147, 156/153, 622/449.
+// Whether tokens that share experts are worth the coarser tiles of the wide form.  Few-token form against wide form, us:
+//   tokens                                                      4         8        16        32        64       256
+//   128 experts, K 8, hidden 2048, experts of 768           69/71   110/105   155/140   204/181   255/210   468/249
+//     8-bit                                                 60/61     87/86   144/117   185/145   242/174   588/238
+//   32 of 256, K 8, hidden 7168, experts of 2048          109/116   123/136   189/192   251/259   414/416   736/474
+//     8-bit                                                 40/49   104/121   156/133   263/209   343/272   568/352
+//   8 experts, K 2, hidden 4096, experts of 14336         316/351   378/380   441/427   568/439   806/470 2581/1105
+//     8-bit                                               143/172   257/305   353/291   401/322   746/391  2298/975
+bool wide_form(int tokens, bool w8) { return tokens >= (w8 ? 9 : 16); }
+
+// Tokens of a stage, and the bytes that follow from it; false: nothing fits (no call that wide_form() leaves).  The ring has 8 stages,
+// so that every consumer keeps its own, and half of the shared memory: two blocks an SM hide each other's latency, hidden 4096, 8
+// experts of 14336, 4 tokens 370 -> 327 us.  An expert that more tokens chose is read more than once (from L2 after the first time).
 bool plan(Decode& p, bool w8) {
     p.stages = kConsumers;
     const int few = w8 ? 3 : 6;
-    const bool pair = w8 ? p.tokens <= 8 : p.tokens <= 16 || (p.tokens <= 64 && p.experts >= 32);
-    for (int cap = p.tokens < few ? p.tokens : few; pair && cap > 0; --cap) {
-        p.token_cap = p.shared_cap = cap;
-        p.stage_bytes = stage_bytes(cap, cap, w8);
-        p.blocks = 2;
-        if (kConsumers * p.stage_bytes + down_rest(p, 1) <= kHalf) return true;
-        if (cap <= few / 2) break;   // large routing tables
-    }
-    for (int cap = 24; cap >= 4; cap -= 4) {
-        p.shared_cap = cap;
-        p.token_cap = w8 ? (cap + 1) / 2 : cap;   // their tokens take twice the bytes of the weights
-        p.stage_bytes = stage_bytes(p.token_cap, cap, w8);
-        p.blocks = 1;
-        if (kConsumers * p.stage_bytes + down_rest(p, (cap + 7) / 8) <= kSmemPerBlock - kStatic) return true;
+    for (int cap = p.tokens < few ? p.tokens : few; cap > 0; --cap) {
+        p.token_cap = cap;
+        p.stage_bytes = stage_bytes(cap, w8);
+        if (kConsumers * p.stage_bytes + down_rest(p) <= kHalf) return true;
     }
     return false;
 }
@@ -642,19 +648,46 @@ int launch_decode(Kernel kernel, const char* name, int (&ready)[16], const Decod
     return launch_early(kernel, name, dim3(blocks * sm_count()), kThreads, smem, stream, p);
 }
 
-template <bool W8, int NT>
-int run_decode(const Decode& p, cudaStream_t stream) {
+template <bool W8>
+int run_few(const Decode& p, cudaStream_t stream) {
     static int gate_up_ready[16] = {0}, down_ready[16] = {0};
     const int ring = p.stages * p.stage_bytes;
     if (W8) MOK_TRY(launch_early(to_half_kernel<false>, "to_half_kernel", dim3(p.tokens), 256, 0, stream, p));
-    MOK_TRY(launch_decode(moe_gate_up_kernel<W8, NT>, "moe_gate_up_kernel", gate_up_ready, p, p.blocks, ring + gate_up_rest(p, NT), stream));
+    MOK_TRY(launch_decode(moe_gate_up_kernel<W8>, "moe_gate_up_kernel", gate_up_ready, p, 2, ring + gate_up_rest(p), stream));
     if (W8) MOK_TRY(launch_early(to_half_kernel<true>, "to_half_kernel", dim3(p.tokens * p.topk), 256, 0, stream, p));
-    // Two blocks an SM where each has 12 of the output's columns or more, else one with twice the stages if they fit: hidden 2048, 32
-    // tokens of 128 experts 222 instead of 255 us; hidden 7168, 32 of 256 experts, 380 instead of 411 us.
-    const int blocks = p.hidden_size >= 12 * 2 * sm_count() ? p.blocks : 1;
+    // Two blocks an SM where each has 12 of the output's columns or more, else one with twice the stages: hidden 2048, 8 tokens of 128
+    // experts 112 instead of 117 us.
+    const int blocks = p.hidden_size >= 12 * 2 * sm_count() ? 2 : 1;
     Decode q = p;
-    if (blocks == 1 && 2 * kConsumers * p.stage_bytes + down_rest(p, NT) <= kSmemPerBlock - kStatic) q.stages = 2 * kConsumers;
-    return launch_decode(moe_down_kernel<W8, NT>, "moe_down_kernel", down_ready, q, blocks, q.stages * p.stage_bytes + down_rest(p, NT), stream);
+    if (blocks == 1) q.stages = 2 * kConsumers;
+    return launch_decode(moe_down_kernel<W8>, "moe_down_kernel", down_ready, q, blocks, q.stages * p.stage_bytes + down_rest(p), stream);
+}
+
+template <bool W8, bool DOWN>
+int launch_wide(const Decode& p, int smem, cudaStream_t stream) {
+    static int ready[16] = {0};
+    int dev = 0;
+    MOK_CUDA_CHECK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 16) return MOK_ERR_UNSUPPORTED;
+    if (ready[dev] == 0) {
+        MOK_CUDA_CHECK(cudaFuncSetAttribute(moe_wide_kernel<W8, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock - kStatic));
+        ready[dev] = 1;
+    }
+    return launch_early(moe_wide_kernel<W8, DOWN>, "moe_wide_kernel", dim3(sm_count()), kWideThreads, smem, stream, p);
+}
+template <bool W8>
+int run_wide(Decode p, cudaStream_t stream) {
+    p.token_cap = kWideTokens;
+    p.stage_bytes = W8 ? WideForm<true>::kStageBytes : WideForm<false>::kStageBytes;   // the shared expert's, in bf16, is the smaller one
+    const int routing = routing_bytes(p.experts, p.tokens * p.topk);
+    p.stages = (kSmemPerBlock - kStatic - routing) / p.stage_bytes;
+    if (p.stages > 8) p.stages = 8;
+    const int smem = p.stages * p.stage_bytes + routing;
+    if (W8) MOK_TRY(launch_early(to_half_kernel<false>, "to_half_kernel", dim3(p.tokens), 256, 0, stream, p));
+    MOK_TRY((launch_wide<W8, false>(p, smem, stream)));
+    if (W8) MOK_TRY(launch_early(to_half_kernel<true>, "to_half_kernel", dim3(p.tokens * p.topk), 256, 0, stream, p));
+    MOK_TRY((launch_wide<W8, true>(p, smem, stream)));
+    return launch_early(moe_wide_sum_kernel, "moe_wide_sum_kernel", dim3((p.hidden_size + 1023) / 1024, p.tokens), 256, 0, stream, p);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -662,11 +695,13 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 }  // namespace
 }  // namespace mok
 
-// hidden rows of the routes, of the shared expert; 8-bit experts: tokens in f16 and the scales
+// hidden rows of the routes, of the shared expert; 8-bit experts: tokens in f16 and the scales; wide form: the experts' parts
 extern "C" int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int hidden, int intermediate, int shared_intermediate, int fp8) {
     if (num_tokens <= 0 || topk <= 0 || hidden <= 0 || intermediate <= 0 || shared_intermediate < 0) return 0;
     const int64_t tokens = num_tokens, routes = tokens * topk;
-    return 2 * (routes * intermediate + tokens * shared_intermediate) + (fp8 ? 2 * tokens * hidden + 4 * (tokens + routes) : 0);
+    const int64_t rows = 2 * (routes * intermediate + tokens * shared_intermediate) + (fp8 ? 2 * tokens * hidden + 4 * (tokens + routes) : 0);
+    if (!mok::wide_form(num_tokens, fp8 != 0)) return rows;
+    return (rows + 15) / 16 * 16 + 4 * hidden * (routes + (shared_intermediate > 0 ? tokens : 0));
 }
 
 extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* top_experts, const float* router_weights, int num_tokens,
@@ -685,7 +720,7 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
         (up_scales != nullptr) != w8 || (down_scales != nullptr) != w8)
         return MOK_ERR_INVALID_ARGUMENT;
     if (!aligned16(x) || !aligned16(w_gate) || !aligned16(w_up) || !aligned16(w_down) || !aligned16(w_shared_gate) || !aligned16(w_shared_up) ||
-        !aligned16(w_shared_down) || !aligned16(scratch) || x_stride % 8 != 0 || x_stride < 0)
+        !aligned16(w_shared_down) || !aligned16(scratch) || !aligned16(out) || x_stride % 8 != 0 || x_stride < 0)
         return MOK_ERR_INVALID_ARGUMENT;
     Decode p{};
     p.x = static_cast<const bf16*>(x);
@@ -718,8 +753,12 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.clamp = has_limit;
     p.limit = limit;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (wide_form(num_tokens, w8)) {
+        p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +
+                                           mok_moe_decode_scratch_bytes(num_tokens, topk, hidden, intermediate, shared_intermediate, w8) -
+                                           4LL * hidden * (static_cast<long long>(num_tokens) * topk + (shared ? num_tokens : 0)));
+        return w8 ? run_wide<true>(p, s) : run_wide<false>(p, s);
+    }
     if (!plan(p, w8)) return MOK_ERR_TOO_LARGE;
-    const int nt = (p.shared_cap + 7) / 8;
-    if (w8) return nt == 1 ? run_decode<true, 1>(p, s) : nt == 2 ? run_decode<true, 2>(p, s) : run_decode<true, 3>(p, s);
-    return nt == 1 ? run_decode<false, 1>(p, s) : nt == 2 ? run_decode<false, 2>(p, s) : run_decode<false, 3>(p, s);
+    return w8 ? run_few<true>(p, s) : run_few<false>(p, s);
 }

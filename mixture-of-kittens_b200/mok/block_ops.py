@@ -66,7 +66,7 @@ def _new_codes(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
 def _new_scales(like: torch.Tensor, rows: int, cols: int, tile_rows: int) -> torch.Tensor:
     blocks = -(-cols // BLOCK)
     if tile_rows == 1:
-        return like.new_empty((blocks, rows), dtype=_F32).t()
+        return torch.empty_strided((rows, blocks), (1, rows), dtype=_F32, device=like.device)
     return like.new_empty((-(-rows // BLOCK), blocks), dtype=_F32)
 
 

@@ -134,7 +134,7 @@ def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert
     if top_experts.dtype is torch.int64:   # a number beyond 32 bits is no expert's; it must not become one
         top_experts = top_experts.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     top_experts, router_weights = top_experts.contiguous(), router_weights.contiguous()
-    scratch = x.new_empty((T * K * I + T * shared_i + (T * H + 2 * (T + T * K) if w8 else 0),))   # mok_moe_decode_scratch_bytes / 2
+    scratch = x.new_empty((_entry("mok_moe_decode_scratch_bytes")(T, K, H, I, shared_i, w8) // 2,))
     launch("moe_decode", _entry("mok_moe_decode"), dev, x.data_ptr(), x.stride(0), top_experts.data_ptr(), router_weights.data_ptr(), T, K, H,
            *shared_weights, shared_i, *weights, I, E, first_expert, swiglu_limit is not None,
            0.0 if swiglu_limit is None else float(swiglu_limit), out.data_ptr(), scratch.data_ptr(), status_word(dev).data_ptr())
