@@ -27,6 +27,11 @@ struct WideForm {
     static constexpr int kChunk = Form<W8, false>::kChunk;
 };
 
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
 struct WideBars {
     uint64_t full[8], empty[8], routed;
     int abort_flag;
@@ -123,9 +128,10 @@ __device__ __forceinline__ int weight_turn(int row) { return W8 ? (row & 3) << 1
 __device__ __forceinline__ int token_turn(int token) { return (token & 1) << 2; }
 
 // The copies of one unit by producer thread (producer, lane), which has rows j + 16 i and tokens j + 16 i, and 16 bytes of each.
-template <bool W8, bool DOWN>
-__device__ __forceinline__ bool produce_unit(const Decode& p, const Routing& r, const Unit& q, WideBars& bars, uint32_t base, int stage_bytes, int stages,
-                                             int& stage, uint32_t& phase, int producer, int lane) {
+// EARLY: weights only, into the empty ring until it is full (false); `early` counts these stages, whose tokens follow.
+template <bool W8, bool DOWN, bool EARLY>
+__device__ __forceinline__ bool produce_unit(const Decode& p, const Routing& r, const Unit& q, WideBars& bars, uint32_t base, int& early, int& stage,
+                                             uint32_t& phase, int producer, int lane) {
     typedef WideForm<W8> W;
     const bool shared = q.expert < 0;
     const int j = producer * 4 + (lane >> 3), u = lane & 7;
@@ -141,7 +147,7 @@ __device__ __forceinline__ bool produce_unit(const Decode& p, const Routing& r, 
     const int pieces = DOWN ? min(8, (rows - q.row) / 16) : 8;   // 64 rows at least; what is missing is not stored
     const uint8_t* token[kWideTokens / 16];
 #pragma unroll
-    for (int i = 0; i < kWideTokens / 16; ++i) {
+    for (int i = 0; i < (EARLY ? 0 : kWideTokens / 16); ++i) {
         const int at = q.from + min(j + 16 * i, q.tokens - 1);
         const void* row;
         if (DOWN) row = shared ? p.hidden_shared + static_cast<long long>(at) * depth : p.hidden + static_cast<long long>(r.list[at]) * depth;
@@ -158,15 +164,25 @@ __device__ __forceinline__ bool produce_unit(const Decode& p, const Routing& r, 
     const uint32_t weight_at = j * 128 + ((u ^ weight_turn<W8>(j)) << 4);
     const uint32_t token_at = kWideTokensAt + j * W::kTokenBytes + ((u ^ token_turn(j)) << 4);
     return walk_depth<W8>(depth, [&](int k, int left) {
-        if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, &bars.abort_flag, p.status)) return false;
-        const uint32_t to = base + stage * stage_bytes;
-        if (!W8 || u * 16 < left) {
+        if (EARLY) {
+            if (early == p.stages) return false;
+        } else if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, &bars.abort_flag, p.status)) {
+            return false;
+        }
+        const uint32_t to = base + (EARLY ? early : stage) * p.stage_bytes;
+        const bool weights = EARLY || early == 0;
+        if (weights && (!W8 || u * 16 < left)) {
             const uint8_t* from = w + static_cast<long long>(k) * (W8 ? 1 : 2);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (i < pieces) copy16(to + weight_at + i * 16 * 128, from);
                 from += step;
             }
+        }
+        if (W8 && weights && scale != nullptr) copy4(to + W::kScales + (producer >> 1) * 4, scale + k / 128);
+        if (EARLY) {
+            ++early;
+            return true;
         }
 #pragma unroll
         for (int i = 0; i < kWideTokens / 16; ++i) {
@@ -175,9 +191,9 @@ __device__ __forceinline__ bool produce_unit(const Decode& p, const Routing& r, 
                 if (W8 && left == 128) copy16(to + token_at + i * 16 * W::kTokenBytes + 128, token[i] + k * 2 + 128);
             }
         }
-        if (W8 && scale != nullptr) copy4(to + W::kScales + (producer >> 1) * 4, scale + k / 128);
         arrive_when_copied(smem_u32(&bars.full[stage]));
-        if (++stage == stages) { stage = 0; phase ^= 1u; }
+        if (!weights) --early;
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         return true;
     }, [] {});
 }
@@ -232,15 +248,15 @@ __device__ __forceinline__ void clear(float (&v)[2][4][4]) {
 
 // The sums of one unit for a warp's M x 16 rows and TILES x 8 tokens.
 template <bool W8, bool DOWN, int M, int TILES>
-__device__ __forceinline__ void consume_unit(const Decode& p, WideBars& bars, const uint8_t* ring, int stage_bytes, int stages, int& stage, uint32_t& phase,
-                                             int depth, int row, int token, int lane, float (&total)[2][4][4]) {
+__device__ __forceinline__ void consume_unit(const Decode& p, WideBars& bars, const uint8_t* ring, int& stage, uint32_t& phase, int depth, int row, int token,
+                                             int lane, float (&total)[2][4][4]) {
     typedef WideForm<W8> W;
     float acc[2][4][4];
     clear(acc);
     walk_depth<W8>(depth, [&](int, int left) {
         // a wait that runs out is reported in the status word, and the warp goes on with what is there
         mbar_wait(smem_u32(&bars.full[stage]), phase, &bars.abort_flag, p.status);
-        const uint8_t* at = ring + stage * stage_bytes;
+        const uint8_t* at = ring + stage * p.stage_bytes;
         if (W8) {
             float part[2][4][4];
             clear(part);
@@ -259,7 +275,7 @@ __device__ __forceinline__ void consume_unit(const Decode& p, WideBars& bars, co
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars.empty[stage]));
-        if (++stage == stages) { stage = 0; phase ^= 1u; }
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         return true;
     }, [&] {
 #pragma unroll
@@ -293,21 +309,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
     const Routing r = carve_routing(smem + p.stages * p.stage_bytes, p.experts, p.tokens * p.topk);
     Units<DOWN> units;
     units.count_shared(p);
-    wait_previous_kernel();
+    // The down kernel has weights to fetch and experts to find while the last blocks before it finish; weights and routes are no
+    // earlier kernel's of this call, and the gate / up kernel has waited for those of earlier ones.
+    if (!DOWN) wait_previous_kernel();
     allow_next_kernel();
     int stage = 0;
     uint32_t phase = 0;
     if (warp >= kConsumers) {
         const int producer = warp - kConsumers;
-        int u = blockIdx.x;
-        bool ok = true;
-        for (; u < units.shared && ok; u += gridDim.x)   // these need no routing
-            ok = produce_unit<false, DOWN>(p, r, units.get(p, r, u), bars, base, p.stage_bytes, p.stages, stage, phase, producer, lane);
-        if (ok && mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) {
+        int early = 0;
+        auto produce = [&](auto when) {
+            constexpr bool kEarly = decltype(when)::value;
+            int u = blockIdx.x;
+            for (; u < units.shared; u += gridDim.x)   // these need no routing
+                if (!produce_unit<false, DOWN, kEarly>(p, r, units.get(p, r, u), bars, base, early, stage, phase, producer, lane)) return;
+            if (!mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) return;
             units.count_routed(r);
-            for (; u < units.total && ok; u += gridDim.x)
-                ok = produce_unit<W8, DOWN>(p, r, units.get(p, r, u), bars, base, p.stage_bytes, p.stages, stage, phase, producer, lane);
+            for (; u < units.total; u += gridDim.x)
+                if (!produce_unit<W8, DOWN, kEarly>(p, r, units.get(p, r, u), bars, base, early, stage, phase, producer, lane)) return;
+        };
+        if (DOWN) {
+            produce(Flag<true>());
+            wait_previous_kernel();
         }
+        produce(Flag<false>());
         wait_copies();
         return;
     }
@@ -315,6 +340,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
     order_lists(p, r);
     mbar_arrive(smem_u32(&bars.routed));
     units.count_routed(r);
+    if (DOWN) wait_previous_kernel();
     const int g = lane >> 2, t = lane & 3;
     for (int u = blockIdx.x; u < units.total; u += gridDim.x) {
         const Unit q = units.get(p, r, u);
@@ -329,8 +355,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
         clear(total);
 #define MOK_CONSUME(M, TILES)                                                                                                               \
     do {                                                                                                                                    \
-        if (w8) consume_unit<W8, DOWN, M, TILES>(p, bars, smem, p.stage_bytes, p.stages, stage, phase, depth, row, token, lane, total);     \
-        else consume_unit<false, DOWN, M, TILES>(p, bars, smem, p.stage_bytes, p.stages, stage, phase, depth, row, token, lane, total);     \
+        if (w8) consume_unit<W8, DOWN, M, TILES>(p, bars, smem, stage, phase, depth, row, token, lane, total);     \
+        else consume_unit<false, DOWN, M, TILES>(p, bars, smem, stage, phase, depth, row, token, lane, total);     \
     } while (0)
         if (tiles == 1) MOK_CONSUME(1, 1);
         else if (tiles == 2) MOK_CONSUME(1, 2);
