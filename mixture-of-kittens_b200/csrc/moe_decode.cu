@@ -1,5 +1,5 @@
 // The whole MoE layer for a few tokens: out[t] = shared(x[t]) + sum over k of w[t, k] * expert(route[t, k])(x[t]), expert(x) =
-// W_down (silu(W_gate x) * (W_up x)), in two kernels.  With a handful of tokens the layer is the reading of its experts' weights
+// W_down (silu(W_gate x) * (W_up x)), in two kernels (kWideFrom tokens and more: moe_decode_wide.cuh).  With a handful of tokens the layer is the reading of its experts' weights
 // (3 H I elements each, once); padding every expert to 256 rows, staging and combining would cost more than that.
 //
 //   gate / up: the rows of all experts in use lie end to end and are cut evenly, to the row, over the SMs; a piece is 8 gate rows and
@@ -611,16 +611,18 @@ int gate_up_rest(const Decode& p) { return deposit_floats<1>() * 4 + routing_byt
 int down_rest(const Decode& p) { return gate_up_rest(p) + p.tokens * kRows * 4; }
 
 // Whether tokens that share experts are worth the coarser tiles of the wide form.  Few-token form against wide form, us:
-//   tokens                                                      4         8        16        32        64       256
-//   128 experts, K 8, hidden 2048, experts of 768           69/71   110/105   155/140   204/181   255/210   468/249
-//     8-bit                                                 60/61     87/86   144/117   185/145   242/174   588/238
-//   32 of 256, K 8, hidden 7168, experts of 2048          109/116   123/136   189/192   251/259   414/416   736/474
-//     8-bit                                                 40/49   104/121   156/133   263/209   343/272   568/352
-//   8 experts, K 2, hidden 4096, experts of 14336         316/351   378/380   441/427   568/439   806/470 2581/1105
-//     8-bit                                               143/172   257/305   353/291   401/322   746/391  2298/975
-bool wide_form(int tokens, bool w8) { return tokens >= (w8 ? 9 : 16); }
+//   tokens                                                      1         4         8        14        64       256
+//   128 experts, K 8, hidden 2048, experts of 768           31/31     68/66    111/98   147/131   255/199   468/232
+//     8-bit                                                 30/32     58/56     85/75   122/105   242/159   588/234
+//   32 of 256, K 8, hidden 7168, experts of 2048            33/45     45/48   121/131   172/180   414/399   736/455
+//     8-bit                                                 39/46     73/83     58/58   127/123   343/234   568/316
+//   8 experts, K 2, hidden 4096, experts of 14336         121/147   225/227   430/420   434/423   806/448  2581/969
+//     8-bit                                                80/114   200/251   258/253   400/288   746/381  2298/857
+//   16 experts, K 4, hidden 4096, experts of 1536           41/42     82/84     90/98   102/108   200/122   662/256
+//     8-bit                                                 34/38     57/62     77/76    101/85   210/110   681/231
+constexpr int kWideFrom = 8;   // tokens
 
-// Tokens of a stage, and the bytes that follow from it; false: nothing fits (no call that wide_form() leaves).  The ring has 8 stages,
+// Tokens of a stage, and the bytes that follow from it; false: nothing fits (no call of fewer than kWideFrom tokens).  The ring has 8 stages,
 // so that every consumer keeps its own, and half of the shared memory: two blocks an SM hide each other's latency, hidden 4096, 8
 // experts of 14336, 4 tokens 370 -> 327 us.  An expert that more tokens chose is read more than once (from L2 after the first time).
 bool plan(Decode& p, bool w8) {
@@ -700,7 +702,7 @@ extern "C" int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int hi
     if (num_tokens <= 0 || topk <= 0 || hidden <= 0 || intermediate <= 0 || shared_intermediate < 0) return 0;
     const int64_t tokens = num_tokens, routes = tokens * topk;
     const int64_t rows = 2 * (routes * intermediate + tokens * shared_intermediate) + (fp8 ? 2 * tokens * hidden + 4 * (tokens + routes) : 0);
-    if (!mok::wide_form(num_tokens, fp8 != 0)) return rows;
+    if (num_tokens < mok::kWideFrom) return rows;
     return (rows + 15) / 16 * 16 + 4 * hidden * (routes + (shared_intermediate > 0 ? tokens : 0));
 }
 
@@ -753,7 +755,7 @@ extern "C" int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* to
     p.clamp = has_limit;
     p.limit = limit;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (wide_form(num_tokens, w8)) {
+    if (num_tokens >= kWideFrom) {
         p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +
                                            mok_moe_decode_scratch_bytes(num_tokens, topk, hidden, intermediate, shared_intermediate, w8) -
                                            4LL * hidden * (static_cast<long long>(num_tokens) * topk + (shared ? num_tokens : 0)));

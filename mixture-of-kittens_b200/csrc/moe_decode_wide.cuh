@@ -1,12 +1,16 @@
 // The layer for tokens that share experts: the same sums in the same order as in moe_decode.cu, over tiles of 128 weight rows x 64
-// tokens.  There a stage holds 16 weight rows and up to 24 tokens, so 64 tokens of an expert cost three passes over its weights and
-// 1.5 bytes of tokens a byte of weights; here one pass and half a byte.  Tiles are coarse: it takes many of them, or many tokens, to
-// win (see wide_form()).
+// tokens.  There a stage holds 16 weight rows and six tokens at most (three with 8-bit experts): every six tokens of an expert cost a
+// pass over its weights, and copies of the tokens a third of the bytes that an SM takes in.  Here it is one pass for 64 tokens.  Both
+// are bound by reading the weights: 32 tokens, 8 of 128 experts, hidden 2048, experts of 768 (with its router) 226 -> 182 us, 91% of
+// the measured HBM rate; 64 tokens, 32 of 256 experts in 8 bits, hidden 7168, experts of 2048 310 -> 229 us, 89%.  Experts of more
+// than 64 tokens are read again for the others: 256 tokens, 2 of 8 experts of 14336, 969 us for 437 us of weights.  Tiles are coarse,
+// so a few tokens are better off there (see kWideFrom).
 //
-// A block has four producer warps, which copy 128 bytes of each row per stage, and eight consumer warps of 32 rows x half of the tokens
-// each (mma.sync; tcgen05 would add the products of a tile in another order).  The few-token form cuts K into chunks that eight warps take
-// in turn and adds the warps' sums at the end.  Here every warp walks all of K, the chunks of one such warp after those of another,
-// and adds up where that one's end: a token's result is the same to the bit in either form.
+// A block has four producer warps, which copy 128 bytes of each row per stage, and eight consumer warps of 16 rows x all tokens (up
+// to 16) or 32 rows x half of the tokens each.  They use mma.sync, which takes a few percent of the time; tcgen05 would add the
+// products of a tile in another order.  The few-token form cuts K into chunks that eight warps take in turn and adds the warps' sums
+// at the end.  Here every warp walks all of K, the chunks of one such warp after those of another, and adds up where that one's end:
+// a token's result is the same to the bit in either form.
 //
 // The experts' parts of the output leave in fp32 and a last kernel adds them, shared expert first, then experts by number.
 #pragma once
