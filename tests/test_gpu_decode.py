@@ -228,6 +228,27 @@ def test_a_token_does_not_depend_on_its_batch(dev):
         assert all(torch.equal(a, b[part]) for a, b in zip(mok.route_decode(y[part], w, topk=5), whole))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H,I", [(4672, 2368), (2112, 5184), (576, 64)])
+def test_long_sums_do_not_depend_on_the_batch(dev, H, I, fp8):
+    """More chunks of the summed dimension than are kept apart, and ragged last ones: few tokens, tiles of few and of many tokens and
+    experts of more than one pass all add in one order."""
+    import mok
+    x, routes, weights, shared, routed = _layer(dev, 150, H, I, 3, 2, shared=128, fp8=fp8)
+    whole = _check(dev, (x, routes, weights, shared, routed))
+    for part in (slice(0, 1), slice(2, 9), slice(9, 17), slice(20, 52), slice(60, 150)):
+        assert torch.equal(mok.moe_decode(x[part], routes[part], weights[part], *shared, *routed), whole[part])
+
+
+@pytest.mark.parametrize("T", [7, 8, 256])
+def test_eight_bit_expert_takes_every_token(dev, T):
+    args = list(_layer(dev, T, 320, 192, 70, 2, shared=64, fp8=True))
+    args[1] = torch.full_like(args[1], 69)          # named twice by every token
+    args[1][0], args[1][T // 2, 1] = 3, 68
+    _check(dev, args)
+    _check(dev, args[:3] + [(None,) * 3] + args[4:], first=60)
+
+
 def test_expert_parallel_parts_add_up(dev):
     import mok
     x, routes, weights, shared, routed = _layer(dev, 30, 256, 128, 12, 4, shared=64)
@@ -310,9 +331,10 @@ def test_strides_and_streams_and_graphs(dev):
     assert all(torch.equal(out, e) for (_, _, out), e in zip(graphs, expect))
 
 
-def test_status_word_makes_the_output_nan(dev):
+@pytest.mark.parametrize("T", [4, 40])
+def test_status_word_makes_the_output_nan(dev, T):
     import mok
-    args = _layer(dev, 4, 128, 64, 2, 1)
+    args = _layer(dev, T, 128, 64, 2, 1)
     from mok._native import status_word
     status_word(dev).fill_(1)
     try:
