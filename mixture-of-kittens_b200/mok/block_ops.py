@@ -56,6 +56,11 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _new_codes(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     """[rows, cols] codes whose rows begin at multiples of 16 bytes."""
     ld = _round_up(cols, 16)
@@ -95,8 +100,8 @@ def _norm_forward(x, weight, residual, eps, want_y, want_codes, want_rms):
     hidden = None
     if residual is not None:
         residual = _rows(residual)
-        hidden = x.new_empty((T, H))
-    y = x.new_empty((T, H)) if want_y else None
+        hidden = _like(x)
+    y = _like(x) if want_y else None
     codes = _new_codes(x, T, H) if want_codes else None
     scales = _new_scales(x, T, H, 1) if want_codes else None
     rms = x.new_empty((T,), dtype=_F32) if want_rms else None
@@ -268,35 +273,38 @@ def quantize_blocks(x: torch.Tensor, *, tile_rows: int = 1, transpose: bool = Fa
 # ------------------------------------------------------------------------------------------------------------
 # product
 # ------------------------------------------------------------------------------------------------------------
-def _codes(name: str, q: torch.Tensor) -> torch.Tensor:
-    _require(q.ndim == 2 and q.is_cuda, name + " must be a two-dimensional CUDA tensor")
+def _codes(name: str, q: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """q, or a copy that the kernels can address, its shape, row stride and address."""
+    shape = q.shape
+    _require(len(shape) == 2 and q.is_cuda, name + " must be a two-dimensional CUDA tensor")
     _require(q.dtype is E4M3, name + " must be float8_e4m3fn", TypeError)
-    if q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1] and q.data_ptr() % 16 == 0:
-        return q
-    out = _new_codes(q, *q.shape)
-    out.copy_(q)
-    return out
+    (rows, cols), (ld, step), address = shape, q.stride(), q.data_ptr()
+    if step != 1 or ld % 16 or ld < cols or address % 16:
+        out = _new_codes(q, rows, cols)
+        out.copy_(q)
+        q, ld, address = out, out.stride(0), out.data_ptr()
+    return q, rows, cols, ld, address
 
 
 def _matmul(a, a_scales, b, b_scales):
-    a, b = _codes("a", a), _codes("b", b)
-    M, K = a.shape
-    N = b.shape[0]
-    _require(b.shape[1] == K and K > 0 and N > 0, "a and b must have shapes (M, K) and (N, K), N and K positive")
+    a, M, K, a_ld, a_address = _codes("a", a)
+    b, N, b_depth, b_ld, b_address = _codes("b", b)
+    _require(b_depth == K and K > 0 and N > 0, "a and b must have shapes (M, K) and (N, K), N and K positive")
     blocks = -(-K // BLOCK)
     _require(a_scales.shape == (M, blocks), "a_scales must have shape (M, ceil(K / 128))")
     tile_rows = BLOCK if b_scales.shape == (-(-N // BLOCK), blocks) else 1
     _require(tile_rows == BLOCK or b_scales.shape == (N, blocks),
              "b_scales must have shape (ceil(N / 128), ceil(K / 128)) or (N, ceil(K / 128))")
     _require(a_scales.dtype is _F32 and b_scales.dtype is _F32, "scales must be float32", TypeError)
-    _require(a.device == b.device == a_scales.device == b_scales.device, "a, b and their scales must be on one device")
+    dev = a.device
+    _require(dev == b.device == a_scales.device == b_scales.device, "a, b and their scales must be on one device")
     out = a.new_empty((M, N), dtype=_BF16)
     if M:
         size = _entry("mok_block_matmul_scratch_bytes")(M, N, K)
         scratch = a.new_empty((size // 4,), dtype=_F32) if size else None
-        launch("block_matmul", _entry("mok_block_matmul"), a.device, a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0),
-               a_scales.stride(1), b.data_ptr(), b.stride(0), b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), tile_rows,
-               M, N, K, out.data_ptr(), N, _address(scratch), status_word(a.device).data_ptr())
+        launch("block_matmul", _entry("mok_block_matmul"), dev, a_address, a_ld, a_scales.data_ptr(), *a_scales.stride(), b_address, b_ld,
+               b_scales.data_ptr(), *b_scales.stride(), tile_rows, M, N, K, out.data_ptr(), N, _address(scratch),
+               status_word(dev).data_ptr())
     return out
 
 

@@ -10,7 +10,7 @@ import torch
 
 from ._native import entry as _entry
 from ._native import launch, status_word
-from .block_ops import BLOCK, E4M3, _address, _rows, _traced
+from .block_ops import BLOCK, E4M3, _address, _like, _rows, _traced
 from .ops import _require
 
 MAX_TOKENS, MAX_TOPK, MAX_ROUTES, MAX_EXPERTS = 256, 32, 4096, 1024
@@ -107,7 +107,7 @@ def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert
     E, I = gate.shape[:2]
     _require(I > 0 and I % 64 == 0, "intermediate_size must be a positive multiple of 64")
     w8 = scales[0] is not None
-    _require(all((s is not None) == w8 for s in scales), "the routed weights must be all bfloat16 or all (codes, scales)", TypeError)
+    _require((scales[1] is not None) == w8 == (scales[2] is not None), "the routed weights must be all bfloat16 or all (codes, scales)", TypeError)
     dtype = E4M3 if w8 else _BF16
     up_shape, down_shape = (E, I, H), (E, H, I)
     weights = (_weight("w_routed_gate", gate, up_shape, dev, dtype), _weight("w_routed_up", up, up_shape, dev, dtype),
@@ -127,7 +127,7 @@ def _decode(x, top_experts, router_weights, shared, routed, scales, first_expert
         _require(shared_i > 0 and shared_i % 64 == 0, "shared_intermediate_size must be a positive multiple of 64")
         shared_weights = (_weight("w_shared_gate", sg, (shared_i, H), dev, _BF16), _weight("w_shared_up", su, (shared_i, H), dev, _BF16),
                           _weight("w_shared_down", sd, (H, shared_i), dev, _BF16))
-    out = x.new_empty((T, H))
+    out = _like(x)
     if T == 0:
         return out
     x = _rows(x)
