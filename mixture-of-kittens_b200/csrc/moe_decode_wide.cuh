@@ -74,10 +74,10 @@ struct Units {
             else n = mid;
         }
         u -= r.passes[a] * tiles;
-        const int passes = r.passes[a + 1] - r.passes[a];
+        const int passes = r.passes[a + 1] - r.passes[a], tile = passes == 1 ? u : u / passes;
         q.expert = r.active[a];
-        q.row = u / passes * kStep;
-        q.from = r.begin[a] + u % passes * kWideTokens;
+        q.row = tile * kStep;
+        q.from = r.begin[a] + (u - tile * passes) * kWideTokens;
         q.tokens = min(kWideTokens, r.begin[a + 1] - q.from);
         return q;
     }
@@ -345,6 +345,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
     mbar_arrive(smem_u32(&bars.routed));
     units.count_routed(r);
     if (DOWN) wait_previous_kernel();
+    float* scales = r.weights;   // W8: of the lists' token or hidden rows; the weights wait for the last kernel
+    if (W8) {
+        for (int i = threadIdx.x; i < r.begin[*r.num_active]; i += kConsumerThreads)
+            scales[i] = __ldcg(DOWN ? p.hidden_scale + r.list[i] : p.x_scale + r.token[i]);
+        consumer_barrier();
+    }
     const int g = lane >> 2, t = lane & 3;
     for (int u = blockIdx.x; u < units.total; u += gridDim.x) {
         const Unit q = units.get(p, r, u);
@@ -377,7 +383,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
                 if (c >= q.tokens) continue;
                 const int at = q.from + c;
                 if (DOWN) {
-                    const float scale = w8 ? __ldcg(p.hidden_scale + r.list[at]) : 1.0f;
+                    const float scale = w8 ? scales[at] : 1.0f;
                     float* out = p.parts + static_cast<long long>(shared ? p.tokens * p.topk + at : r.list[at]) * p.hidden_size + q.row + row + g;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
@@ -386,7 +392,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
                         out[16 * m + 8] = w8 ? total[m][n][2 + i] * scale : total[m][n][2 + i];
                     }
                 } else {
-                    const float scale = w8 ? __ldcg(p.x_scale + r.token[at]) : 1.0f;
+                    const float scale = w8 ? scales[at] : 1.0f;
                     bf16* out = (shared ? p.hidden_shared + static_cast<long long>(at) * p.shared_intermediate
                                         : p.hidden + static_cast<long long>(r.list[at]) * p.intermediate) + q.row + row / 2 + g;
 #pragma unroll
