@@ -46,17 +46,24 @@ struct WideBars {
 struct Unit {
     int expert, row, from, tokens;
 };
-template <bool DOWN>
+// Block b takes units b, b + gridDim.x, ..  A unit of the shared expert, which is bf16, takes the time of two of 8-bit experts: with
+// W8 its block's next turn is left out.
+template <bool W8, bool DOWN>
 struct Units {
-    int shared, shared_passes, tiles, total;
+    int shared, shared_passes, tiles, total, left_out;
     static constexpr int kStep = DOWN ? kWideRows : kWideRows / 2;
     __device__ __forceinline__ void count_shared(const Decode& p) {
         shared_passes = (p.tokens + kWideTokens - 1) / kWideTokens;
         shared = p.shared_gate == nullptr ? 0 : ((DOWN ? p.hidden_size : p.shared_intermediate) + kStep - 1) / kStep * shared_passes;
         tiles = ((DOWN ? p.hidden_size : p.intermediate) + kStep - 1) / kStep;
     }
-    __device__ __forceinline__ void count_routed(const Routing& r) { total = shared + r.passes[*r.num_active] * tiles; }
-    // The passes over a tile come one after the other: the later ones find its weights in L2.
+    __device__ __forceinline__ void count_routed(const Routing& r) {
+        total = shared + r.passes[*r.num_active] * tiles;
+        left_out = W8 && shared <= static_cast<int>(gridDim.x) && total > static_cast<int>(gridDim.x) ? shared : 0;
+        total += left_out;
+    }
+    // Unit u; no tokens: a turn that is left out.  The passes over a tile come one after the other: the later ones find its weights in
+    // L2.
     __device__ __forceinline__ Unit get(const Decode& p, const Routing& r, int u) const {
         Unit q;
         if (u < shared) {
@@ -65,6 +72,13 @@ struct Units {
             q.from = u % shared_passes * kWideTokens;
             q.tokens = min(kWideTokens, p.tokens - q.from);
             return q;
+        }
+        if (u >= static_cast<int>(gridDim.x)) {
+            u -= left_out;
+            if (u < static_cast<int>(gridDim.x)) {
+                q.tokens = 0;
+                return q;
+            }
         }
         u -= shared;
         int a = 0;
@@ -311,7 +325,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
     }
     __syncthreads();
     const Routing r = carve_routing(smem + p.stages * p.stage_bytes, p.experts, p.tokens * p.topk);
-    Units<DOWN> units;
+    Units<W8, DOWN> units;
     units.count_shared(p);
     // The down kernel has weights to fetch and experts to find while the last blocks before it finish; weights and routes are no
     // earlier kernel's of this call, and the gate / up kernel has waited for those of earlier ones.
@@ -329,8 +343,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
                 if (!produce_unit<false, DOWN, kEarly>(p, r, units.get(p, r, u), bars, base, early, stage, phase, producer, lane)) return;
             if (!mbar_wait(smem_u32(&bars.routed), 0, &bars.abort_flag, p.status)) return;
             units.count_routed(r);
-            for (; u < units.total; u += gridDim.x)
-                if (!produce_unit<W8, DOWN, kEarly>(p, r, units.get(p, r, u), bars, base, early, stage, phase, producer, lane)) return;
+            for (; u < units.total; u += gridDim.x) {
+                const Unit q = units.get(p, r, u);
+                if (q.tokens > 0 && !produce_unit<W8, DOWN, kEarly>(p, r, q, bars, base, early, stage, phase, producer, lane)) return;
+            }
         };
         if (DOWN) {
             produce(Flag<true>());
@@ -354,6 +370,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) moe_wide_kernel(const Decode 
     const int g = lane >> 2, t = lane & 3;
     for (int u = blockIdx.x; u < units.total; u += gridDim.x) {
         const Unit q = units.get(p, r, u);
+        if (q.tokens == 0) continue;
         const bool shared = q.expert < 0, w8 = W8 && !shared;
         const int depth = DOWN ? (shared ? p.shared_intermediate : p.intermediate) : p.hidden_size;
         // Up to 16 tokens: 16 rows a warp and all tokens.  More: 32 rows and half of the tokens (the last tile may hold nobody's).
