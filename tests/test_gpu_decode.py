@@ -110,6 +110,7 @@ CASES = [
     (8, 512, 256, 16, 4, 256), (9, 512, 256, 16, 4, 320), (16, 7168, 128, 6, 2, 0), (17, 256, 2048, 5, 5, 64), (31, 576, 320, 60, 6, 128),
     (32, 2048, 768, 16, 8, 768), (33, 192, 64, 3, 1, 64), (64, 640, 384, 40, 8, 0), (100, 448, 192, 9, 2, 192), (255, 256, 128, 12, 3, 64),
     (256, 1024, 128, 128, 16, 64), (128, 64, 64, 1024, 32, 0), (5, 16384, 64, 2, 1, 64),
+    (7, 64, 64, 1024, 32, 64), (9, 16384, 64, 2, 1, 64),
 ]
 
 
@@ -268,9 +269,10 @@ def test_same_as_the_layer(dev, dist_ctx):
     assert off <= 1e-2          # two bf16 computations: gate, up, hidden, expert rows and output rounded, 2^-8 at most each
 
 
-def test_weights_beyond_31_bits(dev):
+@pytest.mark.parametrize("T", [2, 9])
+def test_weights_beyond_31_bits(dev, T):
     H, I, E = 7168, 2048, 160
-    args = list(_layer(dev, 2, H, 64, 2, 2, shared=0))
+    args = list(_layer(dev, T, H, 64, 2, 2, shared=0))
     last = _layer(dev, 1, H, I, 2, 2, seed=3)[4]
     routed = []
     for w in last:
