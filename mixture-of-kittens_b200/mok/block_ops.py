@@ -226,16 +226,16 @@ def _quantize(x, tile_rows, normal, transpose):
     _require(normal or transpose, "at least one quantized layout must be requested")
     x = _rows(x)
     M, N = x.shape
+    across, down = -(-N // BLOCK), -(-M // BLOCK)
     q = s = qt = st = None
+    s_strides, st_strides = ((1, M), (1, N)) if tile_rows == 1 else ((across, 1), (down, 1))
     if normal:
         q, s = _new_codes(x, M, N), _new_scales(x, M, N, tile_rows)
     if transpose:
         qt, st = _new_codes(x, N, M), _new_scales(x, N, M, tile_rows)
     if M:
         launch("block_quantize", _entry("mok_block_quantize"), x.device, x.data_ptr(), x.stride(0), M, N, tile_rows,
-               _address(q), q.stride(0) if normal else 0, _address(s), s.stride(0) if normal else 0, s.stride(1) if normal else 0,
-               _address(qt), qt.stride(0) if transpose else 0, _address(st), st.stride(0) if transpose else 0,
-               st.stride(1) if transpose else 0)
+               _address(q), _round_up(N, 16), _address(s), *s_strides, _address(qt), _round_up(M, 16), _address(st), *st_strides)
     return q, s, qt, st
 
 
@@ -330,28 +330,32 @@ class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, quantized_weight):
         need_w, need_x = ctx.needs_input_grad[1], ctx.needs_input_grad[0]
-        w, w_t = quantized_weight if quantized_weight is not None else quantize_weight(weight, transpose=need_x)
-        if need_w:
-            xq, xt = quantize_blocks(x, transpose=True)
+        quantize, multiply = _implementations()
+        if quantized_weight is None:
+            w, w_scales, w_t, w_t_scales = quantize(weight, BLOCK, need_x)
         else:
-            xq, xt = quantize_blocks(x), (None, None)
-        ctx.save_for_backward(*(w_t if need_x else (None, None)), *xt)
-        return block_matmul(xq, w)
+            (w, w_scales), (w_t, w_t_scales) = quantized_weight
+        xq, x_scales, x_t, x_t_scales = quantize(x, 1, need_w)
+        ctx.save_for_backward(*((w_t, w_t_scales) if need_x else (None, None)), *((x_t, x_t_scales) if need_w else (None, None)))
+        return multiply(xq, x_scales, w, w_scales)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_y):
-        wt, wt_scales, xt, xt_scales = ctx.saved_tensors
+        w_t, w_t_scales, x_t, x_t_scales = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        d_x = d_w = None
-        if need_w:
-            q, q_t = quantize_blocks(d_y, transpose=True)
-            d_w = block_matmul(q_t, (xt, xt_scales))
-        else:
-            q = quantize_blocks(d_y)
-        if need_x:
-            d_x = block_matmul(q, (wt, wt_scales))
+        quantize, multiply = _implementations()
+        q, scales, q_t, scales_t = quantize(d_y, 1, need_w)
+        d_w = multiply(q_t, scales_t, x_t, x_t_scales) if need_w else None
+        d_x = multiply(q, scales, w_t, w_t_scales) if need_x else None
         return d_x, d_w, None
+
+
+def _implementations():
+    """Quantizer (x, tile_rows, transpose) and product: the ops where the call is traced, else what they run."""
+    if _traced():
+        return block_quantize, _block_matmul_op
+    return lambda x, tile_rows, transpose: _quantize(x, tile_rows, True, transpose), _matmul
 
 
 def quantize_weight(weight: torch.Tensor, *, transpose: bool = True):
