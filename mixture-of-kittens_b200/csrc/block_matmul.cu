@@ -31,8 +31,7 @@ constexpr int kGroup = 8;                     // m tiles that walk the columns t
 struct Layout {
     static constexpr int kFull = kStages * kStageBytes;
     static constexpr int kEmpty = kFull + 8 * kStages;
-    static constexpr int kAccFull = kEmpty + 8 * kStages;
-    static constexpr int kAccEmpty = kAccFull + 16;
+    static constexpr int kAccEmpty = kEmpty + 8 * kStages;
     static constexpr int kTmemPtr = kAccEmpty + 16;
     static constexpr int kAbort = kTmemPtr + 4;
     static constexpr int kScales = (kAbort + 4 + 127) / 128 * 128;   // [8 warps][2][128] fp32: column scales of a block
@@ -66,27 +65,12 @@ __device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
-// Two fp32 operations per instruction (sm_100).
-__device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) {
-    unsigned long long d;
-    // volatile: stays behind the wait for the tensor-memory load that fills its operands
-    asm volatile("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
+// A value that a tensor-memory load brought: its use stays behind the wait for that load.
+__device__ __forceinline__ float ordered(uint32_t v) {
+    float f;
+    asm volatile("mov.b32 %0, %1;" : "=f"(f) : "r"(v));
+    return f;
 }
-__device__ __forceinline__ unsigned long long pair_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ unsigned long long pair_mul(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ void pair_split(unsigned long long d, uint32_t& lo, uint32_t& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(d));
-}
-
 // mbar_wait that polls instead of suspending the thread: the accumulators change hands once per block of K.
 __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* status) {
     long long start = 0;
@@ -113,7 +97,7 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatil
 }
 
 // Arrival at the leader CTA's barrier that orders nothing but the tensor-memory loads before it (they are complete and fenced).  The
-// usual release at cluster scope also waits for the scales on their way from L2: 1100 clocks a block of K, where all else takes 550.
+// usual release at cluster scope also waits for the scales on their way from L2: 8192 x 7168 x 7168 took 926 us instead of 524 then.
 __device__ __forceinline__ void arrive_leader_relaxed(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar & kPairLeaderMask) : "memory");
 }
@@ -145,7 +129,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bar_full = base + Layout::kFull, bar_empty = base + Layout::kEmpty;
-    const uint32_t bar_acc_full = base + Layout::kAccFull, bar_acc_empty = base + Layout::kAccEmpty;
+    const uint32_t bar_acc_empty = base + Layout::kAccEmpty;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + Layout::kTmemPtr);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + Layout::kAbort);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -159,7 +143,6 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             mbar_init(bar_empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(bar_acc_full + 8 * b, 1);
             mbar_init(bar_acc_empty + 8 * b, 16);   // eight epilogue warps of both CTAs
         }
         *abort_flag = 0;
@@ -199,124 +182,134 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
-        } else if (warp == 1) {
-            if (cta == 0) {
-                int stage = 0;
-                uint32_t phase = 0, block = 0;   // block: blocks of K done so far; accumulator block & 1
-                bool ok = true;
-                for (int t = pair; t < tiles && ok; t += pairs) {
+        } else if (warp <= 2) {
+            // Two issuers take the blocks in turn, one accumulator each: what one waits for (400 clocks a block, beside 560 in which it
+            // hands over MMAs) is hidden behind the other's MMAs.  8192 x 7168 x 7168 444 -> 411 us.
+            if (cta == 0 && lane == 0) {
+                uint32_t blocks = 0;
+                for (int t = pair; t < tiles; t += pairs) {
                     const Work w = decode(p, t);
-                    for (int kb = w.kb0; kb < w.kb1; ++kb, ++block) {
-                        const uint32_t buf = block & 1u;
-                        ok = mbar_poll(bar_acc_empty + 8 * buf, ((block >> 1) & 1u) ^ 1u, abort_flag, p.status) &&
-                             mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status);
-                        if (!ok) break;
-                        tc_fence_after_sync();
-                        if (lane == 0) {
-                            const uint32_t a = base + stage * kStageBytes;
-                            const uint64_t a_desc = umma_smem_desc(a, 16, 1024), b_desc = umma_smem_desc(a + kOperandBytes, 16, 1024);
-    #pragma unroll
-                            for (int k = 0; k < BK / 32; ++k)
-                                umma_e4m3_pair(tmem + buf * BN, a_desc + k * 2u, b_desc + k * 2u, idesc_e4m3(BM, BN), k != 0 ? 1u : 0u);
-                            umma_commit_pair(bar_empty + 8 * stage);
-                            umma_commit_pair(bar_acc_full + 8 * buf);
-                        }
-                        __syncwarp();
-                        if (++stage == kStages) { stage = 0; phase ^= 1u; }
-                    }
+                    blocks += w.kb1 - w.kb0;
+                }
+                const uint32_t buf = warp - 1;
+                for (uint32_t block = buf; block < blocks; block += 2) {
+                    const uint32_t stage = block % kStages, phase = (block / kStages) & 1u;
+                    if (!mbar_poll(bar_full + 8 * stage, phase, abort_flag, p.status) ||
+                        !mbar_poll(bar_acc_empty + 8 * buf, ((block >> 1) & 1u) ^ 1u, abort_flag, p.status))
+                        break;
+                    tc_fence_after_sync();
+                    const uint32_t a = base + stage * kStageBytes;
+                    const uint64_t a_desc = umma_smem_desc(a, 16, 1024), b_desc = umma_smem_desc(a + kOperandBytes, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < BK / 32; ++k)
+                        umma_e4m3_pair(tmem + buf * BN, a_desc + k * 2u, b_desc + k * 2u, idesc_e4m3(BM, BN), k != 0 ? 1u : 0u);
+                    umma_commit_pair(bar_empty + 8 * stage);
                 }
             }
+            __syncwarp();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegisters));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         float* col_scales = reinterpret_cast<float*>(gen + Layout::kScales) + (warp - 4) * 256;
         uint8_t* patch = gen + Layout::kPatch + (warp - 4) * kEpiWarpBytes;
-        uint32_t block = 0;
+        const uint32_t accumulators = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+        // Scales of the next block, on their way.  COLUMN_SCALES: the lane fetches columns lane, lane + 32, ... of the warp's 128;
+        // otherwise there is one for all of them.
+        constexpr int kColumns = COLUMN_SCALES ? 4 : 1;
+        const float *a_at = p.sa, *b_at[kColumns];
+        float next_a, next_b[kColumns];
+        auto load_scales = [&] {
+            next_a = *a_at;
+            a_at += p.sa_block;
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j) {
+                next_b[j] = *b_at[j];
+                b_at[j] += p.sb_block;
+            }
+        };
+        auto first_scales = [&](const Work& q) {
+            a_at = p.sa + static_cast<long long>(min(q.m0 + cta * BM_CTA + quarter * 32 + lane, p.rows - 1)) * p.sa_row + q.kb0 * p.sa_block;
+            const int col0 = q.n0 + half * 128;
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j)
+                b_at[j] = p.sb + static_cast<long long>(COLUMN_SCALES ? min(col0 + 32 * j + lane, p.cols - 1) : min(col0, p.cols - 1) / 128) * p.sb_row +
+                          q.kb0 * p.sb_block;
+            load_scales();
+        };
+        uint32_t block = 0, stage = 0, phase = 0;
         bool ok = true;
+        Work w = decode(p, min(pair, tiles - 1));
+        first_scales(w);
         for (int t = pair; t < tiles; t += pairs) {
-            const Work w = decode(p, t);
             const int row0 = w.m0 + cta * BM_CTA + quarter * 32, row = row0 + lane;
-            const int col0 = w.n0 + half * 128;
-            const float* sa = p.sa + static_cast<long long>(min(row, p.rows - 1)) * p.sa_row;
-            // COLUMN_SCALES: the lane fetches columns lane, lane + 32, ... of the warp's 128; otherwise all four are the block's
-            const float* sb[4];
+            const int col0 = w.n0 + half * 128, split = w.split;
+            float acc[128];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sb[j] = p.sb + static_cast<long long>(COLUMN_SCALES ? min(col0 + 32 * j + lane, p.cols - 1) : min(col0, p.cols - 1) / 128) * p.sb_row;
-            float next_a = sa[w.kb0 * p.sa_block], next_b[4];
-#pragma unroll
-            for (int j = 0; j < (COLUMN_SCALES ? 4 : 1); ++j) next_b[j] = sb[j][w.kb0 * p.sb_block];
-            unsigned long long acc[64];
-#pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0ull;
-            for (int kb = w.kb0; kb < w.kb1; ++kb, ++block) {
-                const uint32_t buf = block & 1u;
+            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            // 32 columns at a time, in single fp32 operations: with pairs of them (fma.rn.f32x2) three quarters of the columns took 610
+            // clocks instead of 280.  Loads run while the columns before are added; the accumulator goes back to the MMAs when its last
+            // columns are read.
+            uint32_t v[2][32];
+            for (int left = w.kb1 - w.kb0; left > 0; --left, ++block) {
+                const uint32_t buf = block & 1u, taddr = accumulators + buf * BN;
                 float scale = next_a;
                 const float* cols = col_scales + buf * 128;
                 if (COLUMN_SCALES) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) col_scales[buf * 128 + 32 * j + lane] = next_b[j];
+                    for (int j = 0; j < kColumns; ++j) col_scales[buf * 128 + 32 * j + lane] = next_b[j];
                     __syncwarp();   // two buffers: this one was read before the previous block's barrier
                 } else {
                     scale *= next_b[0];
                 }
-                if (kb + 1 < w.kb1) {
-                    next_a = sa[(kb + 1) * p.sa_block];
-#pragma unroll
-                    for (int j = 0; j < (COLUMN_SCALES ? 4 : 1); ++j) next_b[j] = sb[j][(kb + 1) * p.sb_block];
-                }
-                ok = mbar_poll(bar_acc_full + 8 * buf, (block >> 1) & 1u, abort_flag, p.status);
+                if (left > 1) load_scales();
+                ok = mbar_poll(bar_empty + 8 * stage, phase, abort_flag, p.status);   // the MMAs that read a stage are its block's
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 if (!ok) break;
                 tc_fence_after_sync();
-                const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * 128;
-                const unsigned long long s2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
-                // 32 columns at a time: the next load runs while the columns before are added, and the accumulator goes back to the
-                // MMAs before its last columns are
-                uint32_t v[2][32];
                 tmem_ld_32x32(taddr, v[0]);
                 tmem_ld_32x32(taddr + 32, v[1]);
                 tmem_ld_wait();
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    if (q >= 2) tmem_ld_wait();
-                    if (q == 3) {
+                    if (q == 2) {
+                        tmem_ld_wait();
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) arrive_leader_relaxed(bar_acc_empty + 8 * buf);
                     }
-                    if (q == 2) tmem_ld_32x32(taddr + 96, v[1]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const unsigned long long d0 = pair_of(v[q & 1][4 * i], v[q & 1][4 * i + 1]);
-                        const unsigned long long d1 = pair_of(v[q & 1][4 * i + 2], v[q & 1][4 * i + 3]);
-                        unsigned long long f0 = s2, f1 = s2;
+                        float4 f = make_float4(scale, scale, scale, scale);
                         if (COLUMN_SCALES) {
-                            const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(cols + q * 32 + 4 * i);
-                            f0 = pair_mul(cs.x, s2);
-                            f1 = pair_mul(cs.y, s2);
+                            const float4 cs = *reinterpret_cast<const float4*>(cols + q * 32 + 4 * i);
+                            f.x *= cs.x; f.y *= cs.y; f.z *= cs.z; f.w *= cs.w;
                         }
-                        acc[q * 16 + 2 * i] = pair_fma(d0, f0, acc[q * 16 + 2 * i]);
-                        acc[q * 16 + 2 * i + 1] = pair_fma(d1, f1, acc[q * 16 + 2 * i + 1]);
+                        acc[q * 32 + 4 * i] = fmaf(ordered(v[q & 1][4 * i]), f.x, acc[q * 32 + 4 * i]);
+                        acc[q * 32 + 4 * i + 1] = fmaf(ordered(v[q & 1][4 * i + 1]), f.y, acc[q * 32 + 4 * i + 1]);
+                        acc[q * 32 + 4 * i + 2] = fmaf(ordered(v[q & 1][4 * i + 2]), f.z, acc[q * 32 + 4 * i + 2]);
+                        acc[q * 32 + 4 * i + 3] = fmaf(ordered(v[q & 1][4 * i + 3]), f.w, acc[q * 32 + 4 * i + 3]);
                     }
-                    if (q == 0) tmem_ld_32x32(taddr + 64, v[0]);
+                    if (q < 2) tmem_ld_32x32(taddr + 64 + 32 * q, v[q]);
                 }
             }
+            if (t + pairs < tiles) {   // the next tile's scales arrive while this one is stored
+                w = decode(p, t + pairs);
+                first_scales(w);
+            }
             if (!ok) {   // a wait ran out (reported in the status word): this tile and the ones that follow are NaN
-                const unsigned long long nan2 = 0x7FC000007FC00000ull;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) acc[i] = nan2;
+                for (int i = 0; i < 128; ++i) acc[i] = __uint_as_float(0x7FC00000u);
             }
             if (p.splits > 1) {
                 // one row per lane, 16 bytes at a time; a line is filled by eight stores of one lane and merges in L2
                 if (row < p.rows) {
-                    float* out = p.partial + (static_cast<long long>(w.split) * p.rows + row) * p.cols;
+                    float* out = p.partial + (static_cast<long long>(split) * p.rows + row) * p.cols;
                     const bool whole = (p.cols & 3) == 0;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         uint32_t f[4];
-                        pair_split(acc[2 * i], f[0], f[1]);
-                        pair_split(acc[2 * i + 1], f[2], f[3]);
+                        f[0] = __float_as_uint(acc[4 * i]); f[1] = __float_as_uint(acc[4 * i + 1]); f[2] = __float_as_uint(acc[4 * i + 2]); f[3] = __float_as_uint(acc[4 * i + 3]);
                         const int col = col0 + 4 * i;
                         if (whole && col < p.cols) {
                             *reinterpret_cast<uint4*>(out + col) = make_uint4(f[0], f[1], f[2], f[3]);
@@ -336,7 +329,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     for (int i = 0; i < 8; ++i) {
                         uint32_t f[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) pair_split(acc[h * 32 + i * 4 + j], f[2 * j], f[2 * j + 1]);
+                        for (int j = 0; j < 8; ++j) f[j] = __float_as_uint(acc[h * 64 + i * 8 + j]);
                         mine[i] = pack8_bf16(f);
                     }
                     __syncwarp();

@@ -117,6 +117,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------
 // Programmatic dependent launch: a kernel launched with launch_early() may begin while the one before it in the stream still runs.
 // It has to wait_previous_kernel() before it touches anything that one may write; allow_next_kernel() lets the next one begin.

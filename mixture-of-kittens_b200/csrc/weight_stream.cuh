@@ -56,9 +56,6 @@ struct Form {
     __device__ static __forceinline__ int chunks(int k_total) { return (k_total + kChunk - 1) / kChunk; }
 };
 
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 // One arrival once every copy that this thread has issued so far is done.
 __device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
