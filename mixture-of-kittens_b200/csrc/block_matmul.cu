@@ -3,9 +3,13 @@
 //
 // The scales are fp32 numbers of any value, so the tensor cores cannot apply them: every block of 128 along K is accumulated on
 // its own in tensor memory (four tcgen05.mma of K = 32, kind::f8f6f4) and added, scaled, to fp32 registers.  CTA pairs own 256 x
-// 256 tiles, each CTA stages 128 rows of A and 128 of B per block by TMA (32 KB, 5 stages); two 256-column accumulators let the
-// MMAs of one block run while eight epilogue warps scale the block before (a warp: 32 rows x 128 columns, 128 registers of
-// sums).  Rows, columns and depth that are not multiples of the tile are zeros from TMA and are not stored.
+// 256 tiles, each CTA stages 128 rows of A and 128 of B per block by TMA (32 KB, 4 stages); two 256-column accumulators, each with
+// a thread that issues its MMAs, let the MMAs of one block run while eight epilogue warps scale the block before (a warp: 32 rows x
+// 128 columns, 128 registers of sums).  Rows, columns and depth that are not multiples of the tile are zeros from TMA and are not
+// stored.
+//
+// Bound by that scaling: about 950 clocks a block where the MMAs alone take 512, and 2300 more a tile for packing and storing.  8192 x
+// 7168 x 7168 388 us (2.2 PFLOP/s), 8192 x 7168 x 2048 141 us (1.7), with a scale per column of B 4096 x 2048 x 4096 79 us.
 //
 // Few tiles (a short grid and a long K): the blocks along K are cut into `splits` shares, every share writes its fp32 sums, and
 // a second kernel adds them in order.
@@ -19,25 +23,27 @@ namespace {
 using namespace tiles;
 
 constexpr int BK = 128;
-constexpr int kStages = 5;
-constexpr int kThreads = 384;                 // one warpgroup with the TMA producer and the MMA issuer, two of the epilogue
+constexpr int kStages = 4;
+constexpr int kThreads = 384;                 // one warpgroup with the TMA producer and the MMA issuers, two of the epilogue
 // Registers of the warpgroups: 384 threads start with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
 constexpr int kIssueRegisters = 40;
 constexpr int kEpilogueRegisters = 232;
 constexpr int kOperandBytes = 128 * BK;       // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kGroup = 8;                     // m tiles that walk the columns together
+constexpr int kBoxBytes = 32 * 128;           // output of an epilogue warp: two boxes of 32 rows x 64 columns
 
 struct Layout {
-    static constexpr int kFull = kStages * kStageBytes;
+    static constexpr int kPatch = kStages * kStageBytes;              // [8 warps][2 boxes]; 1024-byte aligned
+    static constexpr int kScales = kPatch + 8 * 2 * kBoxBytes;        // [8 warps][2][128] fp32: column scales of a block
+    static constexpr int kFull = kScales + 8 * 2 * 128 * 4;
     static constexpr int kEmpty = kFull + 8 * kStages;
     static constexpr int kAccEmpty = kEmpty + 8 * kStages;
     static constexpr int kTmemPtr = kAccEmpty + 16;
     static constexpr int kAbort = kTmemPtr + 4;
-    static constexpr int kScales = (kAbort + 4 + 127) / 128 * 128;   // [8 warps][2][128] fp32: column scales of a block
-    static constexpr int kPatch = kScales + 8 * 2 * 128 * 4;
-    static constexpr int kBytes = kPatch + 8 * kEpiWarpBytes;
+    static constexpr int kBytes = kAbort + 4;
 };
+static_assert(kEpiWarpBytes <= 2 * kBoxBytes, "the patch of outputs that TMA cannot address");
 static_assert(Layout::kBytes + 1024 <= kMaxDynamicSmem, "shared memory");
 
 struct Product {
@@ -48,6 +54,7 @@ struct Product {
     long long out_stride;
     int rows, cols, k_blocks;
     int m_tiles, n_tiles, splits;
+    int box_out;             // rows of out are 16-byte aligned: boxes leave by TMA
     uint32_t* status;
 };
 
@@ -65,6 +72,12 @@ __device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc,
         : "memory");
 }
 
+// A box of shared memory to the output, rows and columns beyond its end left out.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t src, int col, int row) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(col), "r"(row), "r"(0)
+                 : "memory");
+}
 // A value that a tensor-memory load brought: its use stays behind the wait for that load.
 __device__ __forceinline__ float ordered(uint32_t v) {
     float f;
@@ -106,25 +119,31 @@ struct Work {
     int m0, n0, split, kb0, kb1;
 };
 // Tile t: groups of kGroup m tiles walk the columns together (their A panels stay in L2), the shares of K innermost.
-__device__ __forceinline__ Work decode(const Product& p, int t) {
+__device__ __forceinline__ Work decode(const Product& p, uint32_t t) {
     Work w;
-    w.split = t % p.splits;
-    t /= p.splits;
-    const int per_group = kGroup * p.n_tiles;
-    const int g = t / per_group, rem = t - g * per_group;
-    const int width = min(kGroup, p.m_tiles - g * kGroup);
-    const int n = rem / width;
+    w.split = 0;
+    w.kb0 = 0;
+    w.kb1 = p.k_blocks;
+    if (p.splits > 1) {   // k_blocks * splits < 2^31
+        w.split = t % p.splits;
+        t /= p.splits;
+        w.kb0 = p.k_blocks * w.split / p.splits;
+        w.kb1 = p.k_blocks * (w.split + 1) / p.splits;
+    }
+    const uint32_t per_group = kGroup * p.n_tiles;
+    const uint32_t g = t / per_group, rem = t - g * per_group;
+    const uint32_t width = min(kGroup, p.m_tiles - static_cast<int>(g) * kGroup);
+    const uint32_t n = width == kGroup ? rem / kGroup : rem / width;
     w.m0 = (g * kGroup + rem - n * width) * BM;
     w.n0 = n * BN;
-    w.kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * w.split / p.splits);
-    w.kb1 = static_cast<int>(static_cast<long long>(p.k_blocks) * (w.split + 1) / p.splits);
     return w;
 }
 
 // COLUMN_SCALES: sb holds one scale per column instead of one per 128.
 template <bool COLUMN_SCALES>
 __global__ void __launch_bounds__(kThreads, 1)
-block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product p) {
+block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
+                    const Product p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -212,7 +231,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegisters));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         float* col_scales = reinterpret_cast<float*>(gen + Layout::kScales) + (warp - 4) * 256;
-        uint8_t* patch = gen + Layout::kPatch + (warp - 4) * kEpiWarpBytes;
+        uint8_t* patch = gen + Layout::kPatch + (warp - 4) * 2 * kBoxBytes;
         const uint32_t accumulators = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
         // Scales of the next block, on their way.  COLUMN_SCALES: the lane fetches columns lane, lane + 32, ... of the warp's 128;
         // otherwise there is one for all of them.
@@ -320,6 +339,25 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         }
                     }
                 }
+            } else if (p.box_out) {
+                // The boxes leave while the next tile is on its way.
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // those of the tile before
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    uint32_t f[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = __float_as_uint(acc[i * 8 + j]);
+                    *reinterpret_cast<uint4*>(patch + (i >> 3) * kBoxBytes + lane * 128 + (((i & 7) ^ (lane & 7)) << 4)) = pack8_bf16(f);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (row0 < p.rows && col0 + 64 * h < p.cols) store_box(&map_out, smem_u32(patch) + h * kBoxBytes, col0 + 64 * h, row0);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             } else {
                 const bool whole = (p.out_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
@@ -354,6 +392,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     if (*abort_flag) {
@@ -470,16 +509,23 @@ extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_
     p.status = status;
     if (p.splits > 1 && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0)) return MOK_ERR_INVALID_ARGUMENT;
     if (static_cast<long long>(p.m_tiles) * p.n_tiles * p.splits > 0x7fffffffLL) return MOK_ERR_TOO_LARGE;
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_a, map_b, map_out{};
     MOK_TRY(code_map(&map_a, a, a_stride, rows, depth));
     MOK_TRY(code_map(&map_b, b, b_stride, cols, depth));
+    p.box_out = p.splits == 1 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_stride % 8 == 0;
+    if (p.box_out) {
+        const cuuint64_t dims[4] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 1, 1};
+        const cuuint64_t row_bytes = static_cast<cuuint64_t>(out_stride) * 2, strides[3] = {row_bytes, row_bytes * rows, row_bytes * rows};
+        const cuuint32_t box[4] = {64, 32, 1, 1};
+        MOK_TRY(encode_map(&map_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
+    }
     const int tiles = p.m_tiles * p.n_tiles * p.splits;
     if (b_tile_rows == 1) {
         static int resident[16] = {0};
-        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<true>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, p));
+        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<true>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, map_out, p));
     } else {
         static int resident[16] = {0};
-        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<false>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, p));
+        MOK_TRY(launch_pairs<kThreads>(block_matmul_kernel<false>, "block_matmul_kernel", resident, Layout::kBytes + 1024, tiles, s, map_a, map_b, map_out, p));
     }
     if (p.splits > 1) {
         const long long count = rows * cols;
