@@ -457,8 +457,17 @@ int shares(int tiles, int k_blocks) {
     return s < 2 || k_blocks - k_blocks / s < 16 ? 1 : s;
 }
 
+// Whether the streaming form is the faster one.  Its time grows with the rows, that of a tile does not; streaming against tiles, us:
+//   rows                    8         16         24          with a scale per column    8         16         24
+//   4096 x 7168     18.4/20.4  22.5/22.5  24.6/20.5                             20.5/24.6  22.5/24.5  24.6/24.6
+//   7168 x 2048     14.3/18.4  16.4/18.4  18.4/18.4                             14.3/22.5  16.4/22.5  20.4/22.5
+//   7168 x 16384    51.2/43.0  59.4/43.0  67.6/45.1                             51.2/63.5  59.4/61.5  67.6/63.5
+bool few_rows(long long rows, int cols, int depth, int b_tile_rows) {
+    return rows <= kFewRows && (b_tile_rows == 1 || rows * cols * depth <= 1LL << 29);
+}
+
 int plan_splits(long long rows, int cols, int depth) {
-    if (rows <= kFewRows) return 1;
+    if (few_rows(rows, cols, depth, 128)) return 1;
     return shares(div_up(rows, BM) * div_up(cols, BN), div_up(depth, BK));
 }
 
@@ -484,7 +493,7 @@ extern "C" int mok_block_matmul(const void* a, int64_t a_stride, const float* a_
         a_stride < depth || b_stride < depth || out_stride < cols)
         return MOK_ERR_INVALID_ARGUMENT;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (rows <= kFewRows) {
+    if (few_rows(rows, cols, depth, b_tile_rows)) {
         const BlockProduct few{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), a_stride, b_stride, a_scales, b_scales,
                                a_scale_row_stride, a_scale_block_stride, b_scale_row_stride, b_scale_block_stride, b_tile_rows,
                                static_cast<int>(rows), cols, depth, static_cast<bf16*>(out), out_stride, status};

@@ -17,7 +17,7 @@ struct BlockProduct {
     uint32_t* status;
 };
 
-// Rows of A that the form for a few rows takes.
+// Most rows of A that the form for a few rows takes.
 constexpr int kFewRows = 24;
 int launch_block_matmul_few(const BlockProduct& p, cudaStream_t stream);
 

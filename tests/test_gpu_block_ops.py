@@ -273,7 +273,7 @@ def _check_product(got, a, sa, b, sb, b_rows):
 
 PRODUCTS = [(1, 1, 16), (1, 128, 128), (1, 2048, 2048), (5, 264, 304), (16, 4096, 1024), (17, 130, 4096), (31, 129, 144), (32, 768, 2048),
             (33, 640, 1040), (64, 2048, 512), (65, 300, 8192), (128, 256, 256), (200, 257, 400), (255, 512, 128), (256, 256, 2048), (257, 1100, 640),
-            (1000, 1544, 1808), (2304, 2048, 384)]
+            (1000, 1544, 1808), (2304, 2048, 384), (20, 4096, 7168), (5000, 1032, 272), (4900, 1500, 400)]
 
 
 @pytest.mark.parametrize("b_rows", [1, 128])
