@@ -44,38 +44,46 @@ __device__ __forceinline__ void load_weight(const void* w, int col, float (&f)[8
 
 // Sum over the block, the same value in every thread, in a fixed order.  `part` holds one value per warp; the caller alternates
 // between two of them, so that one barrier per sum is enough.
-template <class T = float>   // of the last step, over the warps
-__device__ __forceinline__ T block_sum(float v, float* part) {
+template <class T>
+__device__ __forceinline__ T block_sum(T v, T* part) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
     const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    T s = (threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : 0.0f;
+    v = (threadIdx.x & 31) < warps ? part[threadIdx.x & 31] : T(0);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    return s;
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
 }
 
 // y / scale in fp32 is a few units off in its last place, which decides the code only where it comes that close to the middle
-// between two codes: with 20 bits below e4m3's mantissa, one value in 130 000.  Those are made from 64 bits, so that a code is off
-// its neighbour's side about ten times as rarely.  (Codes below 2^-6 have their middles elsewhere; half a step there is 2^-18 of the
+// between two codes: with 20 bits below e4m3's mantissa, one value in 130 000.  Those are made from 64 bits (in fp32, sums of 32
+// squares of bf16 values come out 4e-8 too small on average, which alone turned one code of 5 million).  (Codes below 2^-6 have their middles elsewhere; half a step there is 2^-18 of the
 // largest value.)
 __device__ __forceinline__ uint32_t from_middle(float v) { return (__float_as_uint(v) - 0x7FFFCu) & 0xFFFFFu; }
 constexpr uint32_t kNearMiddle = 8;
+template <bool WIDE>
+struct Sum {
+    typedef float type;
+};
+template <>
+struct Sum<true> {
+    typedef double type;
+};
+
 // One row per block; a thread holds V vectors of 8 columns, so 16 adjacent lanes hold one block of 128.  With codes the bounds
 // below ask for more blocks an SM than registers allow without spills, which all lie on the rare path: 16384 x 7168 in 195 us, 207
 // with four blocks.  z kept in shared memory (225 us) and the rare values listed there for the block's end (221 us) took longer.
 template <int V, int THREADS, bool W32, bool CODES>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : !CODES ? 1 : V == 4 ? 5 : V == 2 ? 6 : 7)
     rms_norm_forward_kernel(const NormForward p) {
-    __shared__ float part[32];
+    __shared__ typename Sum<CODES>::type part[32];   // codes: sums of eight squares are added in 64 bits
     const long long row = blockIdx.x;
     const int vectors = p.cols >> 3;
     const bf16* x = p.x + row * p.x_stride;
     const bf16* r = p.residual == nullptr ? nullptr : p.residual + row * p.residual_stride;
     float z[V][8];
-    float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int i = v * blockDim.x + threadIdx.x;
@@ -99,17 +107,22 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : !CODES ? 1 : V =
             }
         }
     }
+    typename Sum<CODES>::type sum = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < V; ++v) {
+        float eight = CODES ? 0.0f : static_cast<float>(sum);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(z[v][j], z[v][j], sum);
+        for (int j = 0; j < 8; ++j) eight = fmaf(z[v][j], z[v][j], eight);
+        sum = CODES ? sum + eight : eight;
+    }
     float rho;
     double mean = 0.0;
+    const typename Sum<CODES>::type squares = block_sum<typename Sum<CODES>::type>(sum, part);
     if (CODES) {
-        mean = block_sum<double>(sum, part) * p.inv_cols + p.eps;
+        mean = squares * p.inv_cols + p.eps;
         rho = __frsqrt_rn(static_cast<float>(mean));
     } else {
-        rho = __frsqrt_rn(__fdiv_rn(block_sum(sum, part), static_cast<float>(p.cols)) + p.eps);
+        rho = __frsqrt_rn(__fdiv_rn(static_cast<float>(squares), static_cast<float>(p.cols)) + p.eps);
     }
     if (p.inv_rms != nullptr && threadIdx.x == 0) p.inv_rms[row] = rho;
 #pragma unroll
