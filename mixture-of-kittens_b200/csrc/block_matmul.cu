@@ -448,8 +448,8 @@ int code_map(CUtensorMap* map, const void* base, long long stride, long long row
 int div_up(long long a, int b) { return static_cast<int>((a + b - 1) / b); }
 
 // Shares of K: enough to give every CTA pair a tile, each at least four blocks long, where that takes 16 blocks or more (0.4 us each)
-// off the longest chain: writing, reading and adding the shares costs 6 us.  1000 x 1544 x 1808 (28 tiles, 15 blocks) takes 20.5 us in
-// one share and 24.5 in two.
+// off the longest chain: writing, reading and adding the shares costs 6 us.  1000 x 1544 x 1808 has 28 tiles of 15 blocks and stays
+// in one share (18.4 us; two shares took 4 us longer).
 int shares(int tiles, int k_blocks) {
     const int pairs = sm_count() / 2;
     int s = pairs / tiles;
