@@ -99,6 +99,13 @@ def moe_layer(x: torch.Tensor, top_experts: torch.Tensor, router_weights: torch.
                                    w_routed_down, config, workspace, schedule, swiglu_limit, recompute, mxfp8, quantized_weights)
 
 
+def _capturing(device: torch.device) -> bool:
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class MoKMoE(torch.nn.Module):
     """Expert-parallel MoE layer with a softmax top-k router (weights renormalised over the selected experts), one
     shared expert and `num_experts / ep_size` routed experts on this rank."""
@@ -155,19 +162,23 @@ class MoKMoE(torch.nn.Module):
                          quantized_weights=self._quantized_weights() if self.mxfp8 else None)
 
     def _block_weights(self):
-        """8-bit copies of the routed weights with scales per 128 x 128, kept like those of `_quantized_weights`."""
+        """8-bit copies of the routed weights with scales per 128 x 128, kept like those of `_quantized_weights`.  A call under capture
+        would only record them: without valid copies it quantizes for itself, in every replay, and keeps nothing."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
         key = tuple((p.data_ptr(), p._version) for p in params)
-        if not self.cache_quantized or self._quantized_blocks is None or self._quantized_blocks[0] != key:
-            with torch.no_grad():
-                self._quantized_blocks = (key, tuple(quantize_blocks(p, tile_rows=128) for p in params))
-        return self._quantized_blocks[1]
+        if self.cache_quantized and self._quantized_blocks is not None and self._quantized_blocks[0] == key:
+            return self._quantized_blocks[1]
+        with torch.no_grad():
+            copies = tuple(quantize_blocks(p, tile_rows=128) for p in params)
+        if self.cache_quantized and not _capturing(params[0].device):
+            self._quantized_blocks = (key, copies)
+        return copies
 
     @torch.no_grad()
     def decode(self, x: torch.Tensor, *, fp8: bool = False) -> torch.Tensor:
         """The layer for a serving step of 1 to 256 tokens (`moe_decode`), router included; not differentiable.  With `fp8` the
         routed experts are read from 8-bit copies with a scale per 128 x 128, made on the first call and again after a weight
-        changed.
+        changed.  Capture a step after such a call: a captured one would make them in every replay.
 
         With several expert-parallel ranks every rank passes the same tokens; each adds its own experts' part, rank 0 the shared
         expert's, and the parts (rounded to bf16, as they travel) are summed over the group."""

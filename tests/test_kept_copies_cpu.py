@@ -1,0 +1,64 @@
+"""The 8-bit copies of the weights that `MoKMoE.decode(fp8=True)` keeps between calls, with the quantizer replaced by its formula on the
+CPU and the answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
+import os
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def layer(monkeypatch):
+    """A module with what its copies were last filled with: `recorded` stands for graph memory that no replay has filled."""
+    import torch.distributed as dist
+    import mok
+    from mok import module
+    own = not dist.is_initialized()
+    if own:
+        dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{29911 + os.getpid() % 80}", rank=0, world_size=1)
+    state = {"capturing": False, "made": 0}
+
+    def quantize(w, *, tile_rows):
+        assert tile_rows == 128
+        state["made"] += 1
+        codes = torch.full_like(w, float("nan")) if state["capturing"] else w.detach().clone()
+        return codes, torch.ones(w.shape[0], 1, 1)
+    monkeypatch.setattr(module, "quantize_blocks", quantize)
+    monkeypatch.setattr(module, "_capturing", lambda device: state["capturing"], raising=False)
+    m = mok.MoKMoE(64, 64, 2, 1)
+    m.state = state
+    yield m
+    if own:
+        dist.destroy_process_group()
+
+
+def _params(m):
+    return m.w_routed_gate, m.w_routed_up, m.w_routed_down
+
+
+def _right(m, copies):
+    return all(torch.equal(c[0], p) for c, p in zip(copies, _params(m)))
+
+
+def test_copies_are_kept_until_a_weight_changes(layer):
+    first = layer._block_weights()
+    assert _right(layer, first) and layer._block_weights() is first and layer.state["made"] == 3
+    with torch.no_grad():
+        layer.w_routed_up.add_(1.0)
+    assert _right(layer, layer._block_weights()) and layer.state["made"] == 6
+    layer.invalidate_quantized()
+    assert _right(layer, layer._block_weights()) and layer.state["made"] == 9
+    layer.cache_quantized = False
+    assert _right(layer, layer._block_weights()) and layer.state["made"] == 12
+
+
+def test_a_capture_leaves_no_copies_behind(layer):
+    layer.state["capturing"] = True
+    layer._block_weights()
+    layer.state["capturing"] = False
+    assert _right(layer, layer._block_weights())             # eager, before any replay
+    with torch.no_grad():
+        layer.w_routed_down.mul_(2.0)
+    layer.state["capturing"] = True
+    layer._block_weights()                                   # the first call after an update is captured
+    layer.state["capturing"] = False
+    assert _right(layer, layer._block_weights())
