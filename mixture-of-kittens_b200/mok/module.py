@@ -124,6 +124,7 @@ class MoKMoE(torch.nn.Module):
         self.swiglu_limit, self.recompute, self.mxfp8 = swiglu_limit, recompute, mxfp8
         self._quantized = None
         self._quantized_blocks = None
+        self._block_buffers = None
         self.cache_quantized = cache_quantized
         e_loc = num_experts // ep
 
@@ -138,7 +139,7 @@ class MoKMoE(torch.nn.Module):
     def invalidate_quantized(self) -> None:
         """Drops the cached 8-bit copies of the routed weights; the next forward or decode quantizes again.  Call it after any
         weight update the version counters cannot see: writes through `param.data` (fused or foreach optimizers that
-        hold flat buffers, ZeRO-style shards, `param.data.copy_`)."""
+        hold flat buffers, ZeRO-style shards, `param.data.copy_`) and replays of a captured optimizer step."""
         self._quantized = None
         self._quantized_blocks = None
 
@@ -162,23 +163,41 @@ class MoKMoE(torch.nn.Module):
                          quantized_weights=self._quantized_weights() if self.mxfp8 else None)
 
     def _block_weights(self):
-        """8-bit copies of the routed weights with scales per 128 x 128, kept like those of `_quantized_weights`.  A call under capture
-        would only record them: without valid copies it quantizes for itself, in every replay, and keeps nothing."""
+        """8-bit copies of the routed weights with scales per 128 x 128, made again after one of them changed (see
+        `_quantized_weights` for what counts as a change).
+
+        They are refilled in place, so that a captured decode reads the present ones.  Once per update the host waits for the device
+        before a refill, because calls on other streams may still read the copies, and for the refill, because the next call may be
+        on any stream.  A call under capture would only record a refill: without valid copies it quantizes for itself, in every
+        replay, and keeps nothing."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
         key = tuple((p.data_ptr(), p._version) for p in params)
         if self.cache_quantized and self._quantized_blocks is not None and self._quantized_blocks[0] == key:
             return self._quantized_blocks[1]
         with torch.no_grad():
             copies = tuple(quantize_blocks(p, tile_rows=128) for p in params)
-        if self.cache_quantized and not _capturing(params[0].device):
-            self._quantized_blocks = (key, copies)
+        if not self.cache_quantized or _capturing(params[0].device):
+            return copies
+        self._quantized_blocks = None
+        kept = self._block_buffers
+        if kept is not None and all(k.shape == c.shape and k.device == c.device for k, c in zip(sum(kept, ()), sum(copies, ()))):
+            if params[0].is_cuda:
+                torch.cuda.synchronize(params[0].device)
+            for k, c in zip(sum(kept, ()), sum(copies, ())):
+                k.copy_(c)
+            copies = kept
+        if params[0].is_cuda:
+            torch.cuda.current_stream(params[0].device).synchronize()
+        self._block_buffers = copies
+        self._quantized_blocks = (key, copies)
         return copies
 
     @torch.no_grad()
     def decode(self, x: torch.Tensor, *, fp8: bool = False) -> torch.Tensor:
         """The layer for a serving step of 1 to 256 tokens (`moe_decode`), router included; not differentiable.  With `fp8` the
         routed experts are read from 8-bit copies with a scale per 128 x 128, made on the first call and again after a weight
-        changed.  Capture a step after such a call: a captured one would make them in every replay.
+        changed (these calls wait for the copies).  Capture a step after such a call; the captured step then reads the same
+        copies, which the next call outside of a capture brings up to date after a weight changed.
 
         With several expert-parallel ranks every rank passes the same tokens; each adds its own experts' part, rank 0 the shared
         expert's, and the parts (rounded to bf16, as they travel) are summed over the group."""

@@ -438,6 +438,79 @@ def test_module(dev, dist_ctx):
     assert layer._quantized_blocks is None
 
 
+def _tuples(copies):
+    return [t for pair in copies for t in pair]
+
+
+def test_module_copies_across_streams(dev, dist_ctx):
+    """Copies made on one stream, behind other work of it, are there for a call on another."""
+    import mok
+    torch.manual_seed(1)
+    layer = mok.MoKMoE(512, 256, 8, 2, device=dev)
+    x = _normal(dev, 5, 512)
+    layer.decode(x, fp8=True)
+    first, second = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    with torch.no_grad():
+        for _ in range(3):
+            layer.w_routed_up.mul_(-1.5)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(first):
+                torch.cuda._sleep(20_000_000)   # 10 ms
+                layer.decode(x, fp8=True)
+            with torch.cuda.stream(second):
+                got = layer.decode(x, fp8=True)
+            torch.cuda.synchronize()
+            layer.invalidate_quantized()
+            assert torch.equal(got, layer.decode(x, fp8=True))
+
+
+def test_module_captured_with_copies(dev, dist_ctx):
+    """A captured step reads the module's copies: still there, and up to date, after the weights changed and memory was reused."""
+    import mok
+    torch.manual_seed(2)
+    layer = mok.MoKMoE(512, 256, 8, 2, device=dev)
+    x = _normal(dev, 5, 512)
+    layer.decode(x, fp8=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = layer.decode(x, fp8=True)
+    places = [t.data_ptr() for t in _tuples(layer._quantized_blocks[1])]
+    for change in (1.0, -3.0, 0.5):
+        with torch.no_grad():
+            layer.w_routed_gate.mul_(change)
+            layer.w_routed_down.mul_(change)
+        want = layer.decode(x, fp8=True)
+        waste = [torch.full_like(t.view(torch.uint8), 0x7E) for t in _tuples(layer._quantized_blocks[1])]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and [t.data_ptr() for t in _tuples(layer._quantized_blocks[1])] == places
+        del waste
+
+
+def test_module_captured_without_copies(dev, dist_ctx):
+    """The first 8-bit call is captured: an eager call before the replay makes its own copies, and the replay gives the same."""
+    import mok
+    torch.manual_seed(3)
+    layer, x = mok.MoKMoE(512, 256, 8, 2, device=dev), _normal(dev, 5, 512)
+    layer.decode(x)
+    mok.quantize_blocks(layer.w_routed_up.detach(), tile_rows=128)
+    other = mok.MoKMoE(512, 256, 8, 2, device=dev)
+    other.decode(x, fp8=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = layer.decode(x, fp8=True)
+    want = layer.decode(x, fp8=True)
+    assert bool(want.isfinite().all()) and layer._quantized_blocks is not None
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    with torch.no_grad():
+        layer.w_routed_up.mul_(2.0)
+    g.replay()   # quantizes for itself
+    torch.cuda.synchronize()
+    assert torch.equal(out, layer.decode(x, fp8=True))
+
+
 def test_traced_calls_match(dev):
     import mok
     x, routes, weights, shared, routed = _layer(dev, 6, 256, 128, 4, 2, shared=64)

@@ -62,3 +62,17 @@ def test_a_capture_leaves_no_copies_behind(layer):
     layer._block_weights()                                   # the first call after an update is captured
     layer.state["capturing"] = False
     assert _right(layer, layer._block_weights())
+
+
+def test_a_captured_decode_reads_the_present_copies(layer):
+    layer._block_weights()
+    layer.state["capturing"] = True
+    captured = layer._block_weights()                        # valid copies: read as they are
+    layer.state["capturing"] = False
+    assert layer.state["made"] == 3
+    places = [t.data_ptr() for c in captured for t in c]
+    for change in (lambda: layer.w_routed_gate.mul_(3.0), lambda: layer.invalidate_quantized()):
+        with torch.no_grad():
+            change()
+        now = layer._block_weights()
+        assert _right(layer, now) and _right(layer, captured) and [t.data_ptr() for c in now for t in c] == places
