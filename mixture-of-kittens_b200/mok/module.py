@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import torch
 import torch.distributed as dist
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import functional as F
 from . import ops
@@ -106,6 +107,23 @@ def _capturing(device: torch.device) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
+class _WeightsSeen:
+    """The contents of some weights that copies were made of: storages, addresses and version counters.  Storages are held weakly:
+    a new one at the address of a freed one (`param.data = ..`) is another."""
+
+    def __init__(self, params):
+        self.storages = [StorageWeakRef(p.untyped_storage()) for p in params]
+        self.places = [(p.data_ptr(), p._version) for p in params]
+
+    def still(self, params) -> bool:
+        return len(params) == len(self.places) and all(
+            s.cdata == p.untyped_storage()._cdata and place == (p.data_ptr(), p._version)
+            for s, place, p in zip(self.storages, self.places, params))
+
+    def __reduce__(self):   # a copy of the module has weights of its own
+        return _WeightsSeen, ((),)
+
+
 class MoKMoE(torch.nn.Module):
     """Expert-parallel MoE layer with a softmax top-k router (weights renormalised over the selected experts), one
     shared expert and `num_experts / ep_size` routed experts on this rank."""
@@ -171,9 +189,9 @@ class MoKMoE(torch.nn.Module):
         on any stream.  A call under capture would only record a refill: without valid copies it quantizes for itself, in every
         replay, and keeps nothing."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
-        key = tuple((p.data_ptr(), p._version) for p in params)
-        if self.cache_quantized and self._quantized_blocks is not None and self._quantized_blocks[0] == key:
+        if self.cache_quantized and self._quantized_blocks is not None and self._quantized_blocks[0].still(params):
             return self._quantized_blocks[1]
+        seen = _WeightsSeen(params)
         with torch.no_grad():
             copies = tuple(quantize_blocks(p, tile_rows=128) for p in params)
         if not self.cache_quantized or _capturing(params[0].device):
@@ -189,7 +207,7 @@ class MoKMoE(torch.nn.Module):
         if params[0].is_cuda:
             torch.cuda.current_stream(params[0].device).synchronize()
         self._block_buffers = copies
-        self._quantized_blocks = (key, copies)
+        self._quantized_blocks = (seen, copies)
         return copies
 
     @torch.no_grad()

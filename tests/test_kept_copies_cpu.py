@@ -1,5 +1,6 @@
 """The 8-bit copies of the weights that `MoKMoE.decode(fp8=True)` keeps between calls, with the quantizer replaced by its formula on the
 CPU and the answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
+import copy
 import os
 
 import pytest
@@ -76,3 +77,21 @@ def test_a_captured_decode_reads_the_present_copies(layer):
             change()
         now = layer._block_weights()
         assert _right(layer, now) and _right(layer, captured) and [t.data_ptr() for c in now for t in c] == places
+
+
+def test_new_storage_at_the_same_address_is_noticed(layer):
+    memory = torch.randn(2 * 64 * 64).to(torch.bfloat16).view(torch.int16).numpy()
+    with torch.no_grad():
+        layer.w_routed_gate.data = torch.from_numpy(memory).view(torch.bfloat16).view(2, 64, 64)
+    assert _right(layer, layer._block_weights())
+    version, address = layer.w_routed_gate._version, layer.w_routed_gate.data_ptr()
+    memory += 1                                              # the allocator hands the address out again
+    layer.w_routed_gate.data = torch.from_numpy(memory).view(torch.bfloat16).view(2, 64, 64)
+    assert (layer.w_routed_gate._version, layer.w_routed_gate.data_ptr()) == (version, address)
+    assert _right(layer, layer._block_weights())
+
+
+def test_a_copied_key_matches_nothing(layer):
+    layer._block_weights()
+    seen = layer._quantized_blocks[0]
+    assert seen.still(_params(layer)) and not copy.deepcopy(seen).still(_params(layer))
