@@ -165,13 +165,17 @@ class MoKMoE(torch.nn.Module):
         """MXFP8 copies of the routed weights, rebuilt only after one of them changed (optimizer step, load_state_dict).
         The change is detected through the parameters' version counters, which in-place updates of the Parameter bump
         and writes through `.data` do not: after those call `invalidate_quantized()`, or construct the module with
-        `cache_quantized=False` to quantize in every forward."""
+        `cache_quantized=False` to quantize in every forward.  Copies made under capture are only recorded: they are the graph's
+        and are not kept."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
-        key = tuple((p.data_ptr(), p._version) for p in params)
-        if not self.cache_quantized or self._quantized is None or self._quantized[0] != key:
-            with torch.no_grad():
-                self._quantized = (key, quantize_routed_weights(*params))
-        return self._quantized[1]
+        if self.cache_quantized and self._quantized is not None and self._quantized[0].still(params):
+            return self._quantized[1]
+        seen = _WeightsSeen(params)
+        with torch.no_grad():
+            copies = quantize_routed_weights(*params)
+        if self.cache_quantized and not _capturing(params[0].device):
+            self._quantized = (seen, copies)
+        return copies
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         experts, weights = route(x, self.router, topk=self.topk)

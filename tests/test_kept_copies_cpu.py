@@ -1,5 +1,4 @@
-"""The 8-bit copies of the weights that `MoKMoE.decode(fp8=True)` keeps between calls, with the quantizer replaced by its formula on the
-CPU and the answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
+"""The 8-bit copies of the weights that `MoKMoE` keeps between calls, with the quantizers replaced by plain copies on the CPU and the answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
 import copy
 import os
 
@@ -24,6 +23,7 @@ def layer(monkeypatch):
         codes = torch.full_like(w, float("nan")) if state["capturing"] else w.detach().clone()
         return codes, torch.ones(w.shape[0], 1, 1)
     monkeypatch.setattr(module, "quantize_blocks", quantize)
+    monkeypatch.setattr(module, "quantize_routed_weights", lambda *weights: tuple(quantize(w, tile_rows=128) for w in weights))
     monkeypatch.setattr(module, "_capturing", lambda device: state["capturing"], raising=False)
     m = mok.MoKMoE(64, 64, 2, 1)
     m.state = state
@@ -95,3 +95,17 @@ def test_a_copied_key_matches_nothing(layer):
     layer._block_weights()
     seen = layer._quantized_blocks[0]
     assert seen.still(_params(layer)) and not copy.deepcopy(seen).still(_params(layer))
+
+
+def test_mxfp8_copies_of_a_capture_are_not_kept(layer):
+    layer.state["capturing"] = True
+    layer._quantized_weights()
+    layer.state["capturing"] = False
+    kept = layer._quantized_weights()
+    assert _right(layer, kept) and layer._quantized_weights() is kept
+    with torch.no_grad():
+        layer.w_routed_gate.mul_(2.0)
+    layer.state["capturing"] = True
+    layer._quantized_weights()
+    layer.state["capturing"] = False
+    assert _right(layer, layer._quantized_weights())
