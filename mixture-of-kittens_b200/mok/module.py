@@ -109,14 +109,17 @@ def _capturing(device: torch.device) -> bool:
 
 class _WeightsSeen:
     """The contents of some weights that copies were made of: storages, addresses and version counters.  Storages are held weakly:
-    a new one at the address of a freed one (`param.data = ..`) is another."""
+    a new one at the address of a freed one (`param.data = ..`) is another.  Inference tensors count no versions: they are never
+    known to be the same."""
 
     def __init__(self, params):
+        if any(p.is_inference() for p in params):
+            params = ()
         self.storages = [StorageWeakRef(p.untyped_storage()) for p in params]
         self.places = [(p.data_ptr(), p._version) for p in params]
 
     def still(self, params) -> bool:
-        return len(params) == len(self.places) and all(
+        return len(params) == len(self.places) and not any(p.is_inference() for p in params) and all(
             s.cdata == p.untyped_storage()._cdata and place == (p.data_ptr(), p._version)
             for s, place, p in zip(self.storages, self.places, params))
 
@@ -165,8 +168,8 @@ class MoKMoE(torch.nn.Module):
         """MXFP8 copies of the routed weights, rebuilt only after one of them changed (optimizer step, load_state_dict).
         The change is detected through the parameters' version counters, which in-place updates of the Parameter bump
         and writes through `.data` do not: after those call `invalidate_quantized()`, or construct the module with
-        `cache_quantized=False` to quantize in every forward.  Copies made under capture are only recorded: they are the graph's
-        and are not kept."""
+        `cache_quantized=False` to quantize in every forward.  Weights created under `torch.inference_mode` have no such counters
+        and are quantized in every call.  Copies made under capture are only recorded: they are the graph's and are not kept."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
         if self.cache_quantized and self._quantized is not None and self._quantized[0].still(params):
             return self._quantized[1]

@@ -1,4 +1,5 @@
-"""The 8-bit copies of the weights that `MoKMoE` keeps between calls, with the quantizers replaced by plain copies on the CPU and the answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
+"""The 8-bit copies of the weights that `MoKMoE` keeps between calls, with the quantizers replaced by plain copies on the CPU and the
+answer to "is this stream being captured" by a switch: a capture records work and runs none of it."""
 import copy
 import os
 
@@ -109,3 +110,15 @@ def test_mxfp8_copies_of_a_capture_are_not_kept(layer):
     layer._quantized_weights()
     layer.state["capturing"] = False
     assert _right(layer, layer._quantized_weights())
+
+
+@pytest.mark.parametrize("copies", ("_block_weights", "_quantized_weights"))
+def test_weights_without_version_counters(layer, copies):
+    """Parameters created under inference mode: every call makes copies of what they hold then."""
+    import mok
+    with torch.inference_mode():
+        serving = mok.MoKMoE(64, 64, 2, 1)
+        for _ in range(2):
+            assert _right(serving, getattr(serving, copies)())
+            serving.w_routed_up.add_(1.0)
+        assert _right(serving, getattr(serving, copies)())
