@@ -199,7 +199,7 @@ class MoKMoE(torch.nn.Module):
         if self.cache_quantized and self._quantized_blocks is not None and self._quantized_blocks[0].still(params):
             return self._quantized_blocks[1]
         seen = _WeightsSeen(params)
-        with torch.no_grad():
+        with torch.inference_mode(False), torch.no_grad():   # normal tensors, which a later call may refill in any mode
             copies = tuple(quantize_blocks(p, tile_rows=128) for p in params)
         if not self.cache_quantized or _capturing(params[0].device):
             return copies

@@ -122,3 +122,15 @@ def test_weights_without_version_counters(layer, copies):
             assert _right(serving, getattr(serving, copies)())
             serving.w_routed_up.add_(1.0)
         assert _right(serving, getattr(serving, copies)())
+
+
+def test_copies_are_refilled_in_every_mode(layer):
+    """Made by a call under inference mode, refilled outside of it, and the other way round."""
+    with torch.inference_mode():
+        first = layer._block_weights()
+    for mode in (False, True, False):
+        with torch.no_grad():
+            layer.w_routed_up.add_(1.0)
+        with torch.inference_mode(mode):
+            assert layer._block_weights() is first
+        assert _right(layer, first)
