@@ -54,6 +54,12 @@ const char* mok_last_error(void);
 /* Kernels this library has launched in this process so far (all threads). */
 long long mok_launch_count(void);
 
+/*
+ * A status word of the library's own on the current device, for hosts that have none to give: zero when the library is loaded there,
+ * afterwards as kernels and the host leave it.  No fill has to run first, so the first call that takes it may be one that is captured.
+ */
+int mok_status_word(uint32_t** word);
+
 /* Debugging aid: with MOK_TRACE=1 in the environment the layer entry points time their phases (pull / compute /
  * push per chunk, wgrad, shared expert) with CUDA events; this call synchronises the device, writes one line per
  * phase ("name chunk stream start_ms end_ms") to `path` and clears the record. */

@@ -7,6 +7,7 @@
 
 namespace mok {
 namespace {
+__device__ uint32_t g_status_word;   // zero when the library is loaded on a device
 thread_local char g_last_error[512] = "";
 std::atomic<long long> g_launches{0};
 }
@@ -40,3 +41,16 @@ extern "C" int mok_version(void) { return MOK_VERSION; }
 extern "C" const char* mok_last_error(void) { return mok::g_last_error; }
 
 extern "C" long long mok_launch_count(void) { return mok::g_launches.load(); }
+
+// Finding the address loads the library on the device, which a capture in the calling thread would forbid in its strict modes.
+extern "C" int mok_status_word(uint32_t** word) {
+    if (word == nullptr) return MOK_ERR_INVALID_ARGUMENT;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    MOK_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    void* address = nullptr;
+    const cudaError_t err = cudaGetSymbolAddress(&address, mok::g_status_word);
+    MOK_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    if (err != cudaSuccess) return mok::fail_cuda("cudaGetSymbolAddress", err);
+    *word = static_cast<uint32_t*>(address);
+    return MOK_OK;
+}

@@ -100,6 +100,8 @@ def lib() -> ctypes.CDLL:
                                             c_int, c_void_p, c_void_p]
         L.mok_grouped_wgrad_bf16.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              c_void_p, c_void_p]
+        L.mok_status_word.argtypes = [POINTER(c_void_p)]
+        L.mok_status_word.restype = c_int
         L.mok_trace_dump.argtypes = [c_char_p]
         L.mok_trace_dump.restype = c_int
         L.mok_dispatch_rows.argtypes = [POINTER(c_uint64), POINTER(c_uint64), c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
@@ -192,12 +194,24 @@ def ptr_array(values) -> ctypes.Array:
 _STATUS: dict[int, torch.Tensor] = {}
 
 
+class _DeviceWord:
+    """One int32 in device memory that outlives the process's tensors, as `torch.as_tensor` takes it."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 2}
+
+
 def status_word(device: torch.device) -> torch.Tensor:
-    """uint32-sized device word the kernels OR their error bits into (one per device)."""
+    """uint32-sized device word the kernels OR their error bits into (one per device).  It is a variable of the library, zero from its
+    loading on: a fill here would only be recorded where the first call of an operator is captured, and every replay would clear
+    the bits that others have set."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     word = _STATUS.get(index)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        address = c_void_p()
+        with torch.cuda.device(index):
+            check(lib().mok_status_word(ctypes.byref(address)), "status_word")
+            word = torch.as_tensor(_DeviceWord(address.value), device=torch.device("cuda", index))
         _STATUS[index] = word
     return word
 
