@@ -16,6 +16,7 @@
 #include "block_matmul.cuh"
 #include "block_scale.cuh"
 #include "gemm_tiles.cuh"
+#include "ring_turn.cuh"
 
 namespace mok {
 namespace {
@@ -256,8 +257,8 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                           q.kb0 * p.sb_block;
             load_scales();
         };
-        uint32_t block = 0, stage = 0, phase = 0;
-        bool ok = true;
+        uint32_t block = 0;
+        RingTurn<kStages> turn;
         Work w = decode(p, min(pair, tiles - 1));
         first_scales(w);
         for (int t = pair; t < tiles; t += pairs) {
@@ -282,9 +283,9 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     scale *= next_b[0];
                 }
                 if (left > 1) load_scales();
-                ok = mbar_poll(bar_empty + 8 * stage, phase, abort_flag, p.status);   // the MMAs that read a stage are its block's
-                if (++stage == kStages) { stage = 0; phase ^= 1u; }
-                if (!ok) break;
+                // the MMAs that read a stage are its block's
+                if (!turn.next([&](uint32_t stage, uint32_t phase) { return mbar_poll(bar_empty + 8 * stage, phase, abort_flag, p.status); }))
+                    break;
                 tc_fence_after_sync();
                 tmem_ld_32x32(taddr, v[0]);
                 tmem_ld_32x32(taddr + 32, v[1]);
@@ -316,7 +317,7 @@ block_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 w = decode(p, t + pairs);
                 first_scales(w);
             }
-            if (!ok) {   // a wait ran out (reported in the status word): this tile and the ones that follow are NaN
+            if (!turn.ok) {   // a wait ran out (reported in the status word): this tile and the ones that follow are NaN
 #pragma unroll
                 for (int i = 0; i < 128; ++i) acc[i] = __uint_as_float(0x7FC00000u);
             }
