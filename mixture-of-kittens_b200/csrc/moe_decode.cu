@@ -14,6 +14,7 @@
 // finish.
 // Every block finds out by itself which experts are in use and by whom, while its producers already copy the shared expert's
 // weights; hidden rows are kept by route number, so the order in which that happens does not matter.
+#include "row_slice.cuh"
 #include "swiglu_math.cuh"
 #include "weight_stream.cuh"
 
@@ -402,14 +403,6 @@ __global__ void __launch_bounds__(kThreads, 2) moe_gate_up_kernel(const Decode p
 }
 
 // ---- down -------------------------------------------------------------------------------------------------------------
-// Rows of the output's slice that this block owns, in `pieces` pieces.
-struct Slice {
-    int first, end, pieces;
-    __device__ __forceinline__ explicit Slice(const Decode& p)
-        : first(static_cast<int>(static_cast<long long>(p.hidden_size) * blockIdx.x / gridDim.x)),
-          end(static_cast<int>(static_cast<long long>(p.hidden_size) * (blockIdx.x + 1) / gridDim.x)), pieces((end - first + kRows - 1) / kRows) {}
-    __device__ __forceinline__ int row(int i) const { return first + (end - first) * i / pieces; }
-};
 // Calls f for every piece of rows [row, row + count), in order, until it returns false.  `shared_only`: those that need no routing.
 template <typename F>
 __device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, int row, int count, bool shared_only, F&& f) {
@@ -430,7 +423,8 @@ __device__ __forceinline__ bool for_experts(const Decode& p, const Routing& r, i
 
 // The producers.  Until the gate / up kernel is done the stages of the empty ring get their weights only; the hidden rows follow.
 template <bool W8>
-__device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, const Slice& slice, const Ring& start, Bars& bars, int producer, int lane) {
+__device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, const RowSlice& slice, const Ring& start, Bars& bars, int producer,
+                                             int lane) {
     auto depth_of = [&](const Piece& q) { return q.expert < 0 ? p.shared_intermediate : p.intermediate; };
     auto weights_of = [&](const Piece& q, Feed& f) {
         const bool shared = q.expert < 0;
@@ -470,7 +464,7 @@ __device__ __forceinline__ void produce_down(const Decode& p, const Routing& r, 
     };
     auto early_pieces = [&](bool shared_only, int done) {
         met = 0;
-        for (int i = 0; i < (shared_only ? 1 : slice.pieces); ++i)
+        for (int i = 0; i < slice.at_most(shared_only ? 1 : slice.pieces); ++i)
             if (!for_experts(p, r, slice.row(i), slice.row(i + 1) - slice.row(i), shared_only, [&](const Piece& q) {
                     return W8 && q.expert >= 0 ? early(q, done, Form<W8, false>()) : early(q, done, Form<false, false>());
                 }))
@@ -515,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) moe_down_kernel(const Decode p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Slice slice(p);
+    const RowSlice slice(p.hidden_size, kRows, blockIdx.x, gridDim.x);   // of the output's columns
     Ring ring = set_up_ring(bars, smem, p.stage_bytes, p.stages, kConsumerThreads);
     Deposit sums;
     sums.scratch = reinterpret_cast<float*>(smem + p.stages * p.stage_bytes);
