@@ -18,8 +18,18 @@ namespace {
 constexpr int kMaxRouterExperts = 1024;   // 32 logits per lane
 constexpr int kMaxRouterTopk = 32;
 
-// (value, index) order of torch.topk with ties broken towards the lower index
-__device__ __forceinline__ bool better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
+// Logits as unsigned integers in the order of torch.topk: NaN above everything, -inf above 0, which stands for a choice that is taken
+// or none at all.  With floats a NaN never won and left a route behind the last expert, and a masked expert (-inf) could not be told
+// from one that had been chosen.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
+    if (u == 0x80000000u) return 0x80000000u;   // zeros are equal
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key); }
+// ties go to the lower index
+__device__ __forceinline__ bool better(uint32_t v, int i, uint32_t bv, int bi) { return v > bv || (v == bv && i < bi); }
 
 template <int PER_LANE>
 __global__ void __launch_bounds__(256) topk_softmax_kernel(const float* __restrict__ logits, const float* __restrict__ bias,
@@ -30,33 +40,33 @@ __global__ void __launch_bounds__(256) topk_softmax_kernel(const float* __restri
     wait_previous_kernel();
     allow_next_kernel();
     for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < tokens; t += warps) {
-        float v[PER_LANE];
+        uint32_t v[PER_LANE];
 #pragma unroll
         for (int j = 0; j < PER_LANE; ++j) {      // lane owns experts lane, lane + 32, ... : coalesced reads
             const int e = lane + 32 * j;
-            v[j] = e < experts ? logits[static_cast<long long>(t) * ld + e] + (bias != nullptr ? bias[e] : 0.0f) : -INFINITY;
+            v[j] = e < experts ? ordered(logits[static_cast<long long>(t) * ld + e] + (bias != nullptr ? bias[e] : 0.0f)) : 0u;
         }
         float top_v = 0.0f, sum = 0.0f, mine_v = 0.0f;
         int mine_e = 0;
         for (int k = 0; k < topk; ++k) {
-            float bv = -INFINITY;
+            uint32_t bv = 0;
             int bi = 0x7fffffff;
 #pragma unroll
             for (int j = 0; j < PER_LANE; ++j)
                 if (better(v[j], lane + 32 * j, bv, bi)) { bv = v[j]; bi = lane + 32 * j; }
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) {
-                const float ov = __shfl_xor_sync(0xffffffffu, bv, off);
+                const uint32_t ov = __shfl_xor_sync(0xffffffffu, bv, off);
                 const int oi = __shfl_xor_sync(0xffffffffu, bi, off);
                 if (better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
             }
-            if (k == 0) top_v = bv;
-            const float ex = expf(bv - top_v);
+            if (k == 0) top_v = logit_of(bv);
+            const float ex = expf(logit_of(bv) - top_v);
             sum += ex;
             if (lane == k) { mine_v = ex; mine_e = bi; }      // lane k keeps the k-th choice
 #pragma unroll
             for (int j = 0; j < PER_LANE; ++j)
-                if (lane + 32 * j == bi) v[j] = -INFINITY;     // the winner leaves the pool
+                if (lane + 32 * j == bi) v[j] = 0;             // the winner leaves the pool
         }
         if (lane < topk) {
             routes[static_cast<long long>(t) * topk + lane] = mine_e;

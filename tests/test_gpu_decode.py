@@ -385,6 +385,49 @@ def test_router_ties_go_to_the_lower_index(dev):
     assert bool(((weights - 0.25).abs() < 1e-6).all())
 
 
+@pytest.mark.parametrize("T", [1, 5, 40, 512])
+def test_router_not_finite(dev, T):
+    """A token of NaNs chooses experts that there are and its output is NaN, without a shared expert too; experts masked with -inf are
+    chosen last, each once, with weight 0.  512: `mok.route`, the same kernel behind another product."""
+    import mok
+    E, K = 10, 4
+    x, w = _normal(dev, T, 256), _normal(dev, E, 256, std=0.05, seed=1, dtype=torch.float32)
+    x[T // 2] = float("nan")
+    route = mok.route if T == 512 else mok.route_decode
+    routes, weights = (t.detach() for t in route(x, w, topk=K))
+    assert bool(((routes >= 0) & (routes < E)).all()) and all(len(set(r)) == K for r in routes.tolist())
+    assert routes[T // 2].tolist() == [0, 1, 2, 3]                              # alike: the lower index
+    bad = torch.zeros(T, dtype=torch.bool, device=dev)
+    bad[T // 2] = True
+    assert torch.equal(weights.isnan().any(1), bad) and torch.equal(weights.isnan().all(1), bad)
+    if T <= 256:
+        _, _, _, shared, routed = _layer(dev, T, 256, 64, E, K)
+        out = mok.moe_decode(x, routes, weights, *shared, *routed)
+        assert torch.equal(out.isnan().all(1), bad) and torch.equal(out.isnan().any(1), bad)
+    bias = torch.full((E,), -float("inf"), device=dev)
+    bias[[7, 2]] = 0.5
+    x[T // 2] = 1.0
+    routes, weights = (t.detach() for t in route(x, w, bias, topk=K))
+    assert torch.equal(routes[:, :2].sort(1).values, torch.tensor([[2, 7]], dtype=torch.int32, device=dev).expand(T, 2))
+    assert torch.equal(routes[:, 2:], torch.tensor([[0, 1]], dtype=torch.int32, device=dev).expand(T, 2))
+    # the last one's sum of two exponentials and its division: a few units of 2^-23
+    assert bool((weights[:, 2:] == 0).all()) and bool(((weights.sum(1) - 1.0).abs() <= 8 * 2.0 ** -23).all())
+
+
+def test_router_nan_in_the_matrix(dev):
+    """An expert whose logit is NaN comes first, as in torch.topk, and the token's weights are NaN."""
+    import mok
+    x, w = _normal(dev, 6, 256), _normal(dev, 70, 256, std=0.05, seed=1, dtype=torch.float32)
+    w[41] = float("nan")
+    routes, weights = mok.route_decode(x, w, topk=3)
+    logits = x.double() @ w.double().t()
+    assert torch.equal(routes[:, 0], torch.full((6,), 41, dtype=torch.int32, device=dev)) and bool(weights.isnan().all())
+    logits[:, 41] = -float("inf")
+    best = torch.topk(logits, 2, dim=1)
+    gap = (torch.topk(logits, 3, dim=1).values.diff(dim=1).abs().min() > 1e-5).item()
+    assert not gap or torch.equal(routes[:, 1:].long(), best.indices)
+
+
 # ---- as a model uses them ---------------------------------------------------------------------------------------------
 def test_serving_step(dev):
     """norm -> router -> experts in 8 bits, and the shared part as 8-bit products, as one captured step with a residual stream."""
