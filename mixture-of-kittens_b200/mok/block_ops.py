@@ -369,10 +369,18 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, quantized_weight=None) 
     gradient in the backward, are quantized per 1 x 128 along the dimension that is summed, the weight per 128 x 128.
     The gradient of x uses the 8-bit weight, that of the weight the 8-bit x and gradient, as if quantization were the identity.
     With `quantized_weight` (from `quantize_weight`) the weight is not quantized again: once per optimizer step, or once for
-    inference."""
+    inference.  Its transposed half is needed where x requires a gradient."""
     _require(weight.ndim == 2 and x.ndim == 2 and x.shape[1] == weight.shape[1], "x and weight must have shapes (T, K) and (N, K)")
     _require(weight.shape[0] > 0 and weight.shape[0] % 8 == 0, "weight's first dimension must be a positive multiple of 8")
     _require(weight.dtype is _BF16, "weight must be bfloat16", TypeError)
+    if quantized_weight is not None:
+        (w, _), (w_t, _) = quantized_weight
+        _require(w.shape == weight.shape, "quantized_weight must be that of weight: codes (N, K)")
+        if w_t is None:
+            _require(not (torch.is_grad_enabled() and x.requires_grad),
+                     "x requires a gradient, for which quantized_weight must hold the transpose (quantize_weight(weight))")
+        else:
+            _require(w_t.shape == weight.shape[::-1], "quantized_weight must be that of weight: codes of its transpose (K, N)")
     if x.shape[0] == 0:
         return x @ weight.t()
     return _Fp8Linear.apply(x, weight, quantized_weight)

@@ -87,3 +87,22 @@ def test_shape_functions():
         q1, s1, _, _ = torch.ops.mok.block_quantize(x, 1, False)
         out = torch.ops.mok.block_matmul(q1, s1, q, s)
         assert (out.shape, out.dtype) == ((24, 24), torch.bfloat16)
+
+
+def test_linear_refuses_another_weights_codes():
+    import mok
+    x, w = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(128, 256, dtype=torch.bfloat16)
+
+    def codes(rows, cols):
+        return torch.zeros(rows, cols).to(torch.float8_e4m3fn), torch.ones(-(-rows // 128), -(-cols // 128))
+    for bad in ((codes(64, 256), (None, None)), (codes(256, 128), codes(128, 256)), (codes(128, 256), codes(128, 256))):
+        with pytest.raises(ValueError, match="must be that of weight"):
+            mok.fp8_linear(x, w, quantized_weight=bad)
+    # the transposed half is missed by the call that asks for it, not by its backward
+    half = (codes(128, 256), (None, None))
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(ValueError, match="transpose"):
+        mok.fp8_linear(leaf, w, quantized_weight=half)
+    for call in (lambda: mok.fp8_linear(x, w, quantized_weight=half), lambda: torch.no_grad()(mok.fp8_linear)(leaf, w, quantized_weight=half)):
+        with pytest.raises(ValueError, match="CUDA"):   # got as far as the kernels' own checks
+            call()
