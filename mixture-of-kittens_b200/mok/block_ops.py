@@ -13,6 +13,7 @@ are what `torch.compile` sees.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from ._native import entry as _entry
 from ._native import launch, status_word
@@ -31,6 +32,13 @@ def _traced() -> bool:
     if _traced_impl is None:
         from .functional import _traced as _traced_impl
     return _traced_impl()
+
+
+def _differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd has to see a call on these tensors: a gradient may be asked for, or they may have tangents (which the autograd
+    functions here refuse)."""
+    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+            or _forward_ad._current_level >= 0)
 
 
 def _round_up(n: int, m: int) -> int:
@@ -383,4 +391,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, *, quantized_weight=None) 
             _require(w_t.shape == weight.shape[::-1], "quantized_weight must be that of weight: codes of its transpose (K, N)")
     if x.shape[0] == 0:
         return x @ weight.t()
-    return _Fp8Linear.apply(x, weight, quantized_weight)
+    if _differentiated(x, weight):
+        return _Fp8Linear.apply(x, weight, quantized_weight)
+    quantize, multiply = _implementations()   # no gradient will be asked for: nothing is made for one
+    w, w_scales = quantize(weight, BLOCK, False)[:2] if quantized_weight is None else quantized_weight[0]
+    xq, x_scales = quantize(x, 1, False)[:2]
+    return multiply(xq, x_scales, w, w_scales)

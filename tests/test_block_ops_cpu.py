@@ -106,3 +106,39 @@ def test_linear_refuses_another_weights_codes():
     for call in (lambda: mok.fp8_linear(x, w, quantized_weight=half), lambda: torch.no_grad()(mok.fp8_linear)(leaf, w, quantized_weight=half)):
         with pytest.raises(ValueError, match="CUDA"):   # got as far as the kernels' own checks
             call()
+
+
+@pytest.mark.parametrize("x_grad", [False, True])
+@pytest.mark.parametrize("w_grad", [False, True])
+@pytest.mark.parametrize("kept", [False, True])
+def test_linear_makes_what_its_gradients_need(monkeypatch, x_grad, w_grad, kept):
+    """Which matrices are quantized, and which of them in both orientations, with and without gradients: requires_grad alone asks
+    for nothing."""
+    import mok
+    from mok import block_ops
+    x, w = torch.randn(4, 256).to(torch.bfloat16), torch.randn(128, 256).to(torch.bfloat16)
+    calls = []
+
+    def quantize(m, tile_rows, normal, transpose):
+        calls.append(("x" if tile_rows == 1 else "w", transpose))
+        one = torch.ones(1, 1)
+        return m, one, (m.t() if transpose else None), (one if transpose else None)
+    monkeypatch.setattr(block_ops, "_quantize", quantize)
+    monkeypatch.setattr(block_ops, "_matmul", lambda a, a_scales, b, b_scales: a @ b.t())
+    weight = ((w, torch.ones(1, 2)), (w.t(), torch.ones(2, 1))) if kept else None
+    leaves = x.clone().requires_grad_(x_grad), w.clone().requires_grad_(w_grad)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            out = mok.fp8_linear(*leaves, quantized_weight=weight)
+        assert calls == ([] if kept else [("w", False)]) + [("x", False)] and not out.requires_grad
+        calls.clear()
+    out = mok.fp8_linear(*leaves, quantized_weight=weight)
+    assert calls == ([] if kept else [("w", x_grad)]) + [("x", w_grad)] and out.requires_grad == (x_grad or w_grad)
+    if out.requires_grad:
+        out.sum().backward()
+        assert [t.grad is not None for t in leaves] == [x_grad, w_grad]
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward mode AD"):
+                mok.fp8_linear(dual, leaves[1], quantized_weight=weight)
