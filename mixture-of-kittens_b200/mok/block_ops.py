@@ -206,7 +206,7 @@ class _RmsNorm(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
     """Root-mean-square norm of x + residual, differentiable: y bf16 [T, H], or (y, hidden) with a residual, where hidden =
     x + residual (rounded to bf16) is the stream that the next block adds to.  The norm is taken of the unrounded sum."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+    if _differentiated(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, eps)
     if _traced():
         y, hidden, _ = rms_norm_fwd(x, weight, residual, eps)

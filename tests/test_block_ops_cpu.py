@@ -142,3 +142,20 @@ def test_linear_makes_what_its_gradients_need(monkeypatch, x_grad, w_grad, kept)
         for mode in (torch.no_grad, torch.enable_grad):
             with mode(), pytest.raises(RuntimeError, match="forward mode AD"):
                 mok.fp8_linear(dual, leaves[1], quantized_weight=weight)
+
+
+def test_norm_refuses_tangents(monkeypatch):
+    """Forward-mode tangents of any input, with and without gradients: there is no rule for them, and none may be lost."""
+    import mok
+    from mok import block_ops
+    from torch.autograd import forward_ad
+    x, w, r = torch.randn(4, 256).to(torch.bfloat16), torch.ones(256), torch.randn(4, 256).to(torch.bfloat16)
+    monkeypatch.setattr(block_ops, "_norm_forward", lambda x, w, r, *rest: (x + r, None, None, x + r, w[:4] + 0.0))
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for inputs in ((dual(x), w, r), (x, dual(w), r), (x, w, dual(r))):
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(RuntimeError, match="forward mode AD"):
+                    mok.rms_norm(*inputs)
+        assert not mok.rms_norm(x, w, r)[0].requires_grad       # nothing with a tangent: as ever
