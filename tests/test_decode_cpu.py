@@ -127,3 +127,21 @@ def test_module_sums_over_ranks():
     assert torch.equal(a, b)
     # two parts of half the terms, each rounded to bf16 (2^-8), their sum rounded once more
     assert bool(((a - want).abs() <= 2.0 ** -8 * 3 * (want.abs().max() + 1)).all()) and (a - want).norm() <= 0.02 * want.norm()
+
+
+def test_tangents_are_refused():
+    import mok
+    from torch.autograd import forward_ad
+    x, w = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(8, 256)
+    r, weights = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    g, d = torch.zeros(3, 128, 256, dtype=torch.bfloat16), torch.zeros(3, 256, 128, dtype=torch.bfloat16)
+    s = torch.zeros(4, 2)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: mok.route_decode(dual(x), w, topk=2), lambda: mok.route_decode(x, w, dual(w[:, 0].contiguous()), topk=2),
+                     lambda: mok.moe_decode(x, r, dual(weights), None, None, None, g, g, d),
+                     lambda: mok.moe_decode(x, r, weights, None, None, None, g, g, dual(d)),
+                     lambda: mok.rms_norm_quantized(x, dual(w[0])), lambda: mok.block_matmul((x, dual(s)), (x, s))):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangents"):
+                call()

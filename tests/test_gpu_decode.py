@@ -566,3 +566,35 @@ def test_traced_calls_match(dev):
     got = f(x)
     r, w = mok.route_decode(x, w_router, topk=2)
     assert torch.equal(got[0], mok.moe_decode(x, r, w, *shared, *routed, swiglu_limit=2.0)) and torch.equal(got[1], r)
+
+
+def test_gradients_are_not_lost_silently(dev):
+    """Inputs that require gradients give outputs whose backward raises, and the same values as without; tangents are refused."""
+    import mok
+    from torch.autograd import forward_ad
+    x, routes, weights, shared, routed = _layer(dev, 6, 256, 128, 4, 2, shared=64)
+    w_router, norm = _normal(dev, 4, 256, std=0.05, dtype=torch.float32), _normal(dev, 256)
+    a, b = mok.quantize_blocks(x), mok.quantize_blocks(routed[0][0], tile_rows=128)
+    calls = [
+        (lambda x, w: mok.moe_decode(x, routes, w, *shared, *routed), (x, weights)),
+        (lambda x, w: mok.moe_decode(x, routes, weights, *shared, routed[0], w, routed[2]), (x, routed[1])),
+        (lambda x, w: mok.route_decode(x, w, topk=2)[1], (x, w_router)),
+        (lambda x, w: mok.rms_norm_quantized(x, w, x)[1], (x, norm)),
+        (lambda s, t: mok.block_matmul((a[0], s), (b[0], t)), (a[1], b[1])),
+    ]
+    for call, inputs in calls:
+        want = call(*inputs)
+        for which in (0, 1):
+            leaves = [t.detach().clone(memory_format=torch.preserve_format).requires_grad_(i == which) for i, t in enumerate(inputs)]
+            with torch.no_grad():
+                assert not call(*leaves).requires_grad
+            out = call(*leaves)
+            assert out.requires_grad and torch.equal(out, want)
+            with pytest.raises(RuntimeError, match="no autograd formula"):
+                out.float().sum().backward()
+            with forward_ad.dual_level():
+                leaves[which] = forward_ad.make_dual(inputs[which], torch.ones_like(inputs[which]))
+                for mode in (torch.no_grad, torch.enable_grad):
+                    with mode(), pytest.raises(RuntimeError, match="tangents"):
+                        call(*leaves)
+        assert torch.equal(call(*inputs), want) and not want.requires_grad
