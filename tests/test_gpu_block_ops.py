@@ -467,3 +467,27 @@ def test_traced_calls_match(dev):
     (q, s), hidden = mok.rms_norm_quantized(x, w, r)
     want = mok.block_matmul((q, s), weight), hidden, mok.rms_norm(x, w, r)[0]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_traced_training_step_matches(dev, residual):
+    """Norm and linear layer under torch.compile, forward and both gradients: the eager call's to the bit."""
+    import mok
+    x, r = (_normal(dev, 40, 256, seed=i).requires_grad_() for i in range(2))
+    w, a = _normal(dev, 256, seed=3).requires_grad_(), _normal(dev, 64, 256, std=0.06, seed=4).requires_grad_()
+    kept = mok.quantize_weight(a.detach())
+
+    def step(x, r, w, a):
+        y, hidden = mok.rms_norm(x, w, r) if residual else (mok.rms_norm(x, w), x * 2)
+        return mok.fp8_linear(y, a), mok.fp8_linear(hidden, a, quantized_weight=kept)
+    args = (x, r, w, a)
+    leaves = args if residual else (x, w, a)
+    want = step(*args)
+    ends = [_normal(dev, *t.shape, seed=5 + i) for i, t in enumerate(want)]
+    grads = torch.autograd.grad(want, leaves, ends)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(*args)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(got, leaves, ends), grads))
+    with torch.no_grad():
+        again = torch.compile(step, fullgraph=True, backend="aot_eager")(*args)
+    assert all(torch.equal(p, q) for p, q in zip(again, want)) and not again[0].requires_grad
