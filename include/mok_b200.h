@@ -438,8 +438,8 @@ int mok_block_matmul(const void* a, int64_t a_stride, const float* a_scales, int
 
 /*
  * Router for 1 to 256 tokens, in fp32 throughout: logits [num_tokens, num_experts] (scratch / output, without the bias) = x * w^T
- * with w fp32 or bf16 [num_experts, hidden]; routes and weights as mok_router_forward.  hidden % 8 == 0, num_experts <= 1024,
- * topk <= 32.
+ * with w fp32 or bf16 [num_experts, hidden]; routes and weights as mok_router_forward: NaN logits come first, experts whose bias is
+ * -inf last.  hidden % 8 == 0, num_experts <= 1024, topk <= 32.
  */
 int mok_router_decode(const void* x, int64_t x_stride, const void* w, int w_is_f32, const float* bias, int num_tokens, int hidden,
                       int num_experts, int topk, float* logits, int32_t* top_experts, float* router_weights, mok_stream_t stream);
@@ -448,9 +448,10 @@ int mok_router_decode(const void* x, int64_t x_stride, const void* w, int w_is_f
  * The layer for 1 to 256 tokens (num_tokens * topk <= 4096), without workspace or schedule: out bf16 [num_tokens, hidden] =
  * shared(x) + sum over k of router_weights[t, k] * expert(top_experts[t, k])(x).  Routed weights are bf16 (the three scale arrays
  * NULL) or e4m3 with an fp32 scale per 128 x 128 of every expert ([num_experts, ceil(rows / 128), ceil(columns / 128)]); the shared
- * ones are bf16, or NULL with shared_intermediate 0.  Sizes are multiples of 64, addresses of 16 bytes.  Routes outside [first_expert, first_expert +
- * num_experts) contribute nothing; an expert that a token names twice counts with both weights.  scratch:
- * mok_moe_decode_scratch_bytes().  `out` is NaN while the status word is not zero (see mok_fwd_epilogue).
+ * ones are bf16, or NULL with shared_intermediate 0.  Sizes are multiples of 64, addresses of 16 bytes.  Routes outside
+ * [first_expert, first_expert + num_experts) contribute nothing; an expert that a token names twice counts with both weights.  The
+ * hidden rows are rounded to bf16 between the products.  scratch: mok_moe_decode_scratch_bytes().  `out` is NaN while the status
+ * word is not zero (see mok_fwd_epilogue).
  */
 int64_t mok_moe_decode_scratch_bytes(int num_tokens, int topk, int hidden, int intermediate, int shared_intermediate, int fp8);
 int mok_moe_decode(const void* x, int64_t x_stride, const int32_t* top_experts, const float* router_weights, int num_tokens, int topk,

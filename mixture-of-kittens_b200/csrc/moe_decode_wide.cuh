@@ -1,10 +1,12 @@
 // The layer for tokens that share experts: the same sums in the same order as in moe_decode.cu, over tiles of 128 weight rows x 64
 // tokens.  There a stage holds 16 weight rows and six tokens at most (three with 8-bit experts): every six tokens of an expert cost a
 // pass over its weights, and copies of the tokens a third of the bytes that an SM takes in.  Here it is one pass for 64 tokens.  Both
-// are bound by reading the weights: 32 tokens, 8 of 128 experts, hidden 2048, experts of 768 (with its router) 226 -> 182 us, 91% of
-// the measured HBM rate; 64 tokens, 32 of 256 experts in 8 bits, hidden 7168, experts of 2048 310 -> 229 us, 89%.  Experts of more
-// than 64 tokens are read again for the others: 256 tokens, 2 of 8 experts of 14336, 969 us for 437 us of weights.  Tiles are coarse,
-// so a few tokens are better off there (see kWideFrom).
+// are bound by reading the weights in bf16: 32 tokens, 8 of 128 experts, hidden 2048, experts of 768 (with its router) 226 -> 170 to
+// 186 us, 90 to 93 % of the measured HBM rate for the 104 to 116 experts that were chosen.  In 8 bits the conversions and products of
+// eight consumer warps take longer than the bytes: 64 tokens, 32 of 256 experts, hidden 7168, experts of 2048 310 -> 225 to 258 us,
+// 58 to 68 % (17 to 22 experts chosen, and a shared one), 298 us with balanced routes, 69 %.  Experts of more than 64 tokens are
+// read again for the others: 256 tokens, 2 of 8 experts of 14336, 969 us for 437 us of weights.  Tiles are coarse, so a few tokens
+// are better off there (see kWideFrom).
 //
 // A block has four producer warps, which copy 128 bytes of each row per stage, and eight consumer warps of 16 rows x all tokens (up
 // to 16) or 32 rows x half of the tokens each.  They use mma.sync, which takes a few percent of the time; tcgen05 would add the

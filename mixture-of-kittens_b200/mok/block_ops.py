@@ -219,7 +219,8 @@ class _RmsNorm(torch.autograd.Function):
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
     """Root-mean-square norm of x + residual, differentiable: y bf16 [T, H], or (y, hidden) with a residual, where hidden =
-    x + residual (rounded to bf16) is the stream that the next block adds to.  The norm is taken of the unrounded sum."""
+    x + residual (rounded to bf16) is the stream that the next block adds to.  The norm is taken of the unrounded sum; the backward
+    reads the sum from `hidden`, so that one tensor is kept for it instead of two."""
     if _differentiated(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, eps)
     if _traced():
@@ -273,7 +274,8 @@ def block_quantize(x: torch.Tensor, tile_rows: int, transpose: bool
 
 
 def quantize_blocks(x: torch.Tensor, *, tile_rows: int = 1, transpose: bool = False):
-    """(codes, scales) of a bf16 matrix, or ((codes, scales), (codes, scales) of x.T) with `transpose`, read once for both.
+    """(codes, scales) of a bf16 matrix, or ((codes, scales), (codes, scales) of x.T) with `transpose`, read once for both; without
+    gradients.
     [E, M, N] weights of several experts (tile_rows 128, without `transpose`) give [E, M, N] codes and a scale per 128 x 128 of
     every expert."""
     if x.ndim == 3:

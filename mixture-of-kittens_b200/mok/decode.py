@@ -67,7 +67,7 @@ def router_decode(x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor | 
 
 
 def route_decode(x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor | None = None, *, topk: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """`mok.route` for a few tokens: (top_experts int32 [T, topk], router_weights fp32 [T, topk]).  Not
+    """`mok.route` for a few tokens: (top_experts int32 [T, topk], router_weights fp32 [T, topk]), chosen as torch.topk does.  Not
     differentiable: a backward through it raises."""
     if _traced() or _through_op("route_decode", x, w_router, bias):
         return router_decode(x, w_router, bias, topk)
@@ -170,7 +170,7 @@ def moe_decode(x: torch.Tensor, top_experts: torch.Tensor, router_weights: torch
     The routed weights are those of experts first_expert .. first_expert + E - 1.  Routes to other experts (other ranks', or any
     number that is no expert's, such as -1) contribute nothing: expert-parallel ranks sum their outputs.  An expert that a token
     names twice counts with the sum of both weights.  With `swiglu_limit` gate is clamped from above and up from both sides.
-    hidden is rounded to bf16 between the products; sums are fp32.  The output is NaN while the device status word reports a
+    hidden is rounded to bf16 between the products, as in the layer; sums are fp32.  The output is NaN while the device status word reports a
     problem, like that of `mok.functional.forward`.  Not differentiable: a backward through it raises."""
     (g, gs), (u, us), (d, ds) = _pair(w_routed_gate), _pair(w_routed_up), _pair(w_routed_down)
     if _traced() or _through_op("moe_decode", x, router_weights, w_shared_gate, w_shared_up, w_shared_down, g, gs, u, us, d, ds):
