@@ -41,9 +41,20 @@ def _differentiated(*tensors: torch.Tensor | None) -> bool:
             or _forward_ad._current_level >= 0)
 
 
-def _through_op(what: str, *tensors: torch.Tensor | None) -> bool:
-    """For a call without derivatives: whether it goes through its op, whose outputs carry the gradient's request to a backward that
-    raises.  Tangents are refused."""
+class _NoDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, call, *tensors):
+        ctx.what = what
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(ctx.what + " has no derivatives: no autograd formula was written for it")
+
+
+def _without_derivative(what: str, call, *tensors: torch.Tensor | None):
+    """call(), which reads these tensors: where one of them requires a gradient the outputs ask for it in a backward that raises (as
+    those of the ops do; 7 to 14 us of host time instead of 20 to 34), and tangents are refused."""
     if _forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
@@ -51,8 +62,8 @@ def _through_op(what: str, *tensors: torch.Tensor | None) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                return True
-    return False
+                return _NoDerivative.apply(what, call, *tensors)
+    return call()
 
 
 def _round_up(n: int, m: int) -> int:
@@ -233,10 +244,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
 def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
     """The norm's output in 8 bits, ready for `block_matmul`: ((codes, scales), hidden), hidden None without a residual.  Not
     differentiable, a backward through it raises: `fp8_linear` quantizes inside and has one."""
-    if _traced() or _through_op("rms_norm_quantized", x, weight, residual):
+    if _traced():
         codes, scales, hidden = rms_norm_fp8_fwd(x, weight, residual, eps)
         return (codes, scales), hidden if residual is not None else None
-    _, codes, scales, hidden, _ = _norm_forward(x, weight, residual, eps, False, True, False)
+    _, codes, scales, hidden, _ = _without_derivative(
+        "rms_norm_quantized", lambda: _norm_forward(x, weight, residual, eps, False, True, False), x, weight, residual)
     return (codes, scales), hidden
 
 
@@ -345,9 +357,9 @@ def _block_matmul_op(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b
 def block_matmul(a: tuple[torch.Tensor, torch.Tensor], b: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
     """bf16 [M, N] product of a [M, K] and the transpose of b [N, K], both (codes, scales): a with scales per 1 x 128, b per 128 x
     128 or per 1 x 128.  fp32 sums, one rounding.  Not differentiable, a backward through it raises (see `fp8_linear`)."""
-    if _traced() or _through_op("block_matmul", *a, *b):
+    if _traced():
         return _block_matmul_op(*a, *b)
-    return _matmul(*a, *b)
+    return _without_derivative("block_matmul", lambda: _matmul(*a, *b), *a, *b)
 
 
 class _Fp8Linear(torch.autograd.Function):

@@ -10,7 +10,7 @@ import torch
 
 from ._native import entry as _entry
 from ._native import launch, status_word
-from .block_ops import BLOCK, E4M3, _address, _like, _rows, _through_op, _traced
+from .block_ops import BLOCK, E4M3, _address, _like, _rows, _traced, _without_derivative
 from .ops import _require
 
 MAX_TOKENS, MAX_TOPK, MAX_ROUTES, MAX_EXPERTS = 256, 32, 4096, 1024
@@ -69,9 +69,9 @@ def router_decode(x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor | 
 def route_decode(x: torch.Tensor, w_router: torch.Tensor, bias: torch.Tensor | None = None, *, topk: int) -> tuple[torch.Tensor, torch.Tensor]:
     """`mok.route` for a few tokens: (top_experts int32 [T, topk], router_weights fp32 [T, topk]), chosen as torch.topk does.  Not
     differentiable: a backward through it raises."""
-    if _traced() or _through_op("route_decode", x, w_router, bias):
+    if _traced():
         return router_decode(x, w_router, bias, topk)
-    return _route(x, w_router, bias, topk)
+    return _without_derivative("route_decode", lambda: _route(x, w_router, bias, topk), x, w_router, bias)
 
 
 # ------------------------------------------------------------------------------------------------------------
@@ -173,8 +173,9 @@ def moe_decode(x: torch.Tensor, top_experts: torch.Tensor, router_weights: torch
     hidden is rounded to bf16 between the products, as in the layer; sums are fp32.  The output is NaN while the device status word reports a
     problem, like that of `mok.functional.forward`.  Not differentiable: a backward through it raises."""
     (g, gs), (u, us), (d, ds) = _pair(w_routed_gate), _pair(w_routed_up), _pair(w_routed_down)
-    if _traced() or _through_op("moe_decode", x, router_weights, w_shared_gate, w_shared_up, w_shared_down, g, gs, u, us, d, ds):
-        return _moe_decode_op(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, g, gs, u, us, d, ds, first_expert,
-                              swiglu_limit)
-    return _decode(x, top_experts, router_weights, (w_shared_gate, w_shared_up, w_shared_down), (g, u, d), (gs, us, ds), first_expert,
-                   swiglu_limit)
+    shared = (w_shared_gate, w_shared_up, w_shared_down)
+    if _traced():
+        return _moe_decode_op(x, top_experts, router_weights, *shared, g, gs, u, us, d, ds, first_expert, swiglu_limit)
+    return _without_derivative(
+        "moe_decode", lambda: _decode(x, top_experts, router_weights, shared, (g, u, d), (gs, us, ds), first_expert, swiglu_limit),
+        x, router_weights, *shared, g, gs, u, us, d, ds)
