@@ -146,6 +146,7 @@ class MoKMoE(torch.nn.Module):
         self._quantized = None
         self._quantized_blocks = None
         self._block_buffers = None
+        self._captured = []   # MXFP8 copies that graphs read
         self.cache_quantized = cache_quantized
         e_loc = num_experts // ep
 
@@ -158,9 +159,10 @@ class MoKMoE(torch.nn.Module):
         self.w_routed_down = param(e_loc, hidden_size, intermediate_size)
 
     def invalidate_quantized(self) -> None:
-        """Drops the cached 8-bit copies of the routed weights; the next forward or decode quantizes again.  Call it after any
-        weight update the version counters cannot see: writes through `param.data` (fused or foreach optimizers that
-        hold flat buffers, ZeRO-style shards, `param.data.copy_`) and replays of a captured optimizer step."""
+        """Drops the cached 8-bit copies of the routed weights; the next forward or decode quantizes again (decode into the same
+        memory, which captured steps read).  Call it after any weight update the version counters cannot see: writes through
+        `param.data` (fused or foreach optimizers that hold flat buffers, ZeRO-style shards, `param.data.copy_`) and replays of
+        a captured optimizer step."""
         self._quantized = None
         self._quantized_blocks = None
 
@@ -169,10 +171,15 @@ class MoKMoE(torch.nn.Module):
         The change is detected through the parameters' version counters, which in-place updates of the Parameter bump
         and writes through `.data` do not: after those call `invalidate_quantized()`, or construct the module with
         `cache_quantized=False` to quantize in every forward.  Weights created under `torch.inference_mode` have no such counters
-        and are quantized in every call.  Copies made under capture are only recorded: they are the graph's and are not kept."""
+        and are quantized in every call.  Copies made under capture are only recorded: they are the graph's and are not kept.  A graph
+        that was captured with valid copies goes on reading those, so they live as long as the module: capture again after a weight
+        update."""
         params = (self.w_routed_gate, self.w_routed_up, self.w_routed_down)
         if self.cache_quantized and self._quantized is not None and self._quantized[0].still(params):
-            return self._quantized[1]
+            copies = self._quantized[1]
+            if _capturing(params[0].device) and not any(c is copies for c in self._captured):
+                self._captured.append(copies)
+            return copies
         seen = _WeightsSeen(params)
         with torch.no_grad():
             copies = quantize_routed_weights(*params)

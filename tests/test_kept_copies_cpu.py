@@ -134,3 +134,18 @@ def test_copies_are_refilled_in_every_mode(layer):
         with torch.inference_mode(mode):
             assert layer._block_weights() is first
         assert _right(layer, first)
+
+
+def test_mxfp8_copies_that_a_graph_reads_stay(layer):
+    """A graph captured with valid copies: their memory is not handed out again when the weights change."""
+    import weakref
+    layer._quantized_weights()
+    layer.state["capturing"] = True
+    places = [weakref.ref(c[0]) for _ in range(2) for c in layer._quantized_weights()]
+    layer.state["capturing"] = False
+    for change in (lambda: layer.w_routed_gate.mul_(2.0), lambda: layer.invalidate_quantized()):
+        with torch.no_grad():
+            change()
+        assert _right(layer, layer._quantized_weights())
+        assert all(p() is not None for p in places)
+    assert len(layer._captured) == 1
